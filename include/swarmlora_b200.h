@@ -418,6 +418,67 @@ int swl_paged_attention_shrink(int nseg, const int* rows, const void* const* blo
                                int hq, int hkv, int head_dim, int page, float scale, int max_len,
                                const void* q_rot, float* part, const void* const* A_o, int r,
                                float* ws_o, const void* pf, int64_t pf_bytes, void* stream);
+/* Causal GQA attention over whole prompts (no counterpart in the reference,
+ * whose prompts go through flash_attn_with_kvcache): nseg sequences packed one
+ * behind the other, sequence i with q_lens[i] query rows and k_lens[i] key
+ * rows (host arrays). Row r of a sequence sees its keys 0 .. r + k_len - q_len,
+ * so k_len > q_len is a chunk behind a prefix, q_len 1 a single token; a row
+ * that sees no key gives zeros. q [sum q_lens, hq, head_dim], k and v
+ * [sum k_lens, hkv, head_dim], out like q, bf16, heads contiguous; the row strides (elements,
+ * multiples of 8) may be those of a fused projection. head_dim 64 or 128, hq a
+ * multiple of hkv (at most 128 query heads each), scale positive. Rows behind
+ * the last sequence are neither read nor written, and a key or value that a row does not
+ * see cannot reach it, not even as NaN or infinity. `part`: scratch of
+ * swl_prompt_attention_part_floats fp32 values (0: may be NULL), used by this
+ * call alone while it runs. */
+int64_t swl_prompt_attention_part_floats(int nseg, const int* q_lens, const int* k_lens, int hq, int hkv,
+                                         int head_dim);
+int swl_prompt_attention(int nseg, const int* q_lens, const int* k_lens, const void* q, int64_t q_stride,
+                         const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* out,
+                         int64_t out_stride, int hq, int hkv, int head_dim, float scale, float* part,
+                         void* stream);
+
+/* ---- key/value cache held in 4 bits (no counterpart in the reference) ------
+ * A cache is [num_pages][page / 16][hkv][swl_kv4_block_bytes(head_dim)] bytes
+ * (16-byte aligned); a block holds K and V of 16 tokens of one kv head: codes
+ * 0..15 and, per 64 dimensions of a token, a bf16 scale s and minimum m, value =
+ * s * code + m (4.5 bits a value, 3.6 times less than bf16). A group
+ * with a NaN or an infinity reads back as NaN throughout. head_dim 64 or
+ * 128; page 16, 32, 64 .. 1024 tokens. Block tables are device arrays of
+ * table_len page ids per slot; entries outside 0..num_pages-1 and positions
+ * outside the table are treated as absent: nothing is written for them, a gather gives
+ * zeros and attention leaves their tokens out. seqlens[i] points to the
+ * tokens cached before this step (device int). The slots of one call must not share
+ * a page that the call writes. */
+int64_t swl_kv4_block_bytes(int head_dim); /* 18 * head_dim; 0 for another head_dim */
+/* Appends rows[i] new tokens to slot i at positions *seqlens[i] + t: q and k
+ * are rotated (NeoX, cos/sin bf16 as swl_rope_append's table, arithmetic in fp32 and
+ * one rounding where swl_rope_append rounds each product), k and v quantised. qkv
+ * rows are [hq | hkv | hkv] heads (stride in elements, a multiple of 8);
+ * q_rot [total rows, hq * head_dim] and, unless NULL, k_rot [total rows,
+ * hkv * head_dim] receive the rotated rows in bf16. Rows at positions outside
+ * 0..max_pos-1 give zeros and are not cached. */
+int swl_kv4_append(int nseg, const int* rows, const void* const* qkv, int64_t qkv_stride,
+                   const void* const* block_tables, int table_len, void* const* caches, int64_t num_pages,
+                   const void* const* seqlens, int hq, int hkv, int head_dim, int page, const void* cos_sin,
+                   int max_pos, void* q_rot, void* k_rot, void* stream);
+/* Reads tokens starts[i] .. starts[i] + lens[i] - 1 of each slot (host arrays)
+ * back as packed bf16 rows [sum lens, hkv, head_dim] of K and of V: what
+ * swl_prompt_attention reads for a chunk behind a cached prefix. */
+int swl_kv4_gather(int nseg, const int* starts, const int* lens, const void* const* block_tables, int table_len,
+                   const void* const* caches, int64_t num_pages, int hkv, int head_dim, int page, void* k_out,
+                   void* v_out, void* stream);
+/* Causal GQA attention over the 4-bit cache: rows[i] new rows of slot i, whose K and V are
+ * already appended, at positions *seqlens[i] + t, as swl_paged_attention. hq a multiple
+ * of hkv; out rows [rows[i], hq * head_dim] (stride a multiple of 8). max_len
+ * bounds *seqlens[i] + rows[i]; longer contexts are cut there. `part`: scratch
+ * of swl_kv4_part_floats fp32 values (0: may be NULL), used by this call alone
+ * while it runs. */
+int64_t swl_kv4_part_floats(int nseg, const int* rows, int hq, int hkv, int head_dim, int max_len);
+int swl_paged_attention_kv4(int nseg, const int* rows, const void* const* block_tables, int table_len,
+                            const void* const* caches, int64_t num_pages, const void* const* seqlens,
+                            void* const* out, int64_t out_stride, int hq, int hkv, int head_dim, int page,
+                            float scale, int max_len, const void* q_rot, float* part, void* stream);
 /* LlamaRMSNorm (HF modeling_llama; worker_sync.py:1346, 1380, 1416). */
 int swl_rms_norm(int nseg, const int* rows, const void* const* x, int64_t x_stride,
                  void* const* out, int64_t out_stride, const void* w, int64_t hidden, float eps,

@@ -1,0 +1,79 @@
+// The paged key/value cache held in 4 bits: block layout and host tables.
+//
+// A block holds 16 consecutive tokens of one kv head (K and V) in 18 * D bytes;
+// a cache is [pages][page / 16][hkv][18 * D] bytes. Groups of 64 dimensions of
+// one token share a scale s and a minimum m (bf16 each): value = s * code + m,
+// code in 0..15, so a value costs 4.5 bits.
+//
+//   bytes [0, 8D)     K codes: word (t * 4 + (d / 8) % 4) * W + d / 32, nibble d % 8
+//   bytes [8D, 9D)    K pairs: (s, m) of token t, group g at 4 * (t * D / 64 + g)
+//   bytes [9D, 17D)   V codes: word ((t / 8) * 32 + (d / 4) % 8 * 4 + (t % 8) / 2) * W + d / 32,
+//                     16-bit half t % 2, nibble d % 4
+//   bytes [17D, 18D)  V pairs, as K's
+// with W = D / 32 words (of 8 codes) per entry. The order is the one in which the
+// attention's matrix fragments want the codes: lane (g, c) of a warp reads
+// the K codes of tokens g and g + 8 (dimensions 32 j + 8 c ..) and the V codes of
+// tokens 2c, 2c + 1, 2c + 8, 2c + 9 (dimensions 32 u + 4 g ..) as single aligned vectors, and
+// a word's nibbles become pairs of bf16 by one shift and one logic operation.
+// Every code of a token lies in whole 16-bit pieces, so tokens of one block
+// are written without reading their neighbours.
+#pragma once
+
+#include <cstdint>
+
+#include "worker_ops.h"
+
+namespace swl {
+namespace kv4 {
+
+constexpr int kBlockTok = 16;
+constexpr int kGroup = 64;
+
+__host__ __device__ constexpr int block_bytes(int d) { return 18 * d; }
+__host__ __device__ constexpr int k_pair_off(int d) { return 8 * d; }
+__host__ __device__ constexpr int v_code_off(int d) { return 9 * d; }
+__host__ __device__ constexpr int v_pair_off(int d) { return 17 * d; }
+
+// Byte offset of the word holding dimensions d..d+7 (d % 8 == 0) of token t's K.
+template <int D>
+__device__ __forceinline__ int k_word(int t, int d) {
+  return 4 * ((t * 4 + (d >> 3 & 3)) * (D / 32) + (d >> 5));
+}
+// Byte offset of the 16-bit piece holding dimensions d..d+3 (d % 4 == 0) of token t's V.
+template <int D>
+__device__ __forceinline__ int v_piece(int t, int d) {
+  return v_code_off(D) + 4 * (((t >> 3) * 32 + (d >> 2 & 7) * 4 + (t >> 1 & 3)) * (D / 32) + (d >> 5)) + 2 * (t & 1);
+}
+
+// What a launch over slots reads: slot i's block table (page ids), cache and
+// cached length. table_len entries per table and num_pages pages per cache bound every access.
+struct Cache {
+  const int* block_table[kMaxSlots];
+  uint8_t* cache[kMaxSlots];
+  const int* seqlen[kMaxSlots];  // device int: tokens cached before this step
+  int table_len;
+  int page_shift;                // log2(page / 16)
+  int64_t num_pages;
+  int hkv;
+};
+
+// The block of tile `tile` (tokens 16 tile ..) of head h, or nullptr where the
+// table has no such entry or names no page of the cache.
+template <int D>
+__device__ __forceinline__ uint8_t* block_of(const Cache& c, int s, int64_t tile, int h) {
+  const int64_t pi = tile >> c.page_shift;
+  if (tile < 0 || pi >= c.table_len) return nullptr;
+  const int64_t page = c.block_table[s][pi];
+  if (page < 0 || page >= c.num_pages) return nullptr;
+  const int64_t sub = tile & ((int64_t{1} << c.page_shift) - 1);
+  return c.cache[s] + (((page << c.page_shift) + sub) * c.hkv + h) * block_bytes(D);
+}
+
+// Checks and fills the parts every entry point shares.
+int fill_cache(Cache* c, const char* what, int nseg, const void* const* block_tables, int table_len,
+               void* const* caches, int64_t num_pages, const void* const* seqlens, int hkv, int head_dim, int page);
+// Row counts to row starts; the total is bounded so that row indices stay in 31 bits.
+int fill_rows(RowSegments* s, const char* what, int nseg, const int* rows);
+
+}  // namespace kv4
+}  // namespace swl
