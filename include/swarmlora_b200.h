@@ -438,6 +438,10 @@ int swl_prompt_attention(int nseg, const int* q_lens, const int* k_lens, const v
                          int64_t out_stride, int hq, int hkv, int head_dim, float scale, float* part,
                          void* stream);
 
+/* Bounded-wait status of swl_prompt_attention and swl_paged_attention_kv4 on
+ * the current device (0 = no wait ran out; cleared by reading); synchronous. */
+int swl_attention_device_error(unsigned int* code);
+
 /* ---- key/value cache held in 4 bits (no counterpart in the reference) ------
  * A cache is [num_pages][page / 16][hkv][swl_kv4_block_bytes(head_dim)] bytes
  * (16-byte aligned); a block holds K and V of 16 tokens of one kv head: codes

@@ -136,6 +136,7 @@ SIGNATURES: dict[str, tuple] = {
     "swl_prompt_attention_part_floats": (_i64, [_i32, _pi32, _pi32, _i32, _i32, _i32]),
     "swl_prompt_attention": (_i32, [_i32, _pi32, _pi32, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _i32, _i32, _f32,
                                     _p, _p]),
+    "swl_attention_device_error": (_i32, [_pu32]),
     "swl_kv4_block_bytes": (_i64, [_i32]),
     "swl_kv4_append": (_i32, [_i32, _pi32, _pp, _i64, _pp, _i32, _pp, _i64, _pp, _i32, _i32, _i32, _i32, _p, _i32, _p,
                               _p, _p]),

@@ -824,6 +824,21 @@ int encode_kv_page_tmap(CUtensorMap* map, const void* cache, int64_t tokens, int
   return SWL_OK;
 }
 
+int encode_heads_tmap(CUtensorMap* map, const void* base, int64_t rows, int heads, int head_dim, int64_t row_stride,
+                      int box_heads, int box_rows) {
+  auto enc = tmap_encoder();
+  if (!enc) return set_error(SWL_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_dim) * 2, static_cast<cuuint64_t>(row_stride) * 2};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(SWL_ERR_CUDA, "heads tensor map: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return SWL_OK;
+}
+
 int launch_slot_round(const SlotTable& tab, const RoundShape& shape, const void* W,
                       const CUtensorMap* tmap, int algo, int splits, cudaStream_t stream) {
   if (tab.nslots <= 0 || tab.total_rows <= 0) return SWL_OK;  // nothing to do

@@ -111,6 +111,10 @@ int encode_weight_tmap(CUtensorMap* map, const void* W, int64_t N, int64_t K);
 // bf16 with `tokens` rows (pages x page tokens): box 64 dims x 1 head x 16
 // tokens, 128-byte swizzle (one kv head's half of a page per load).
 int encode_kv_page_tmap(CUtensorMap* map, const void* cache, int64_t tokens, int hkv);
+// Encodes the TMA descriptor of packed bf16 rows [rows][heads][head_dim] (row
+// stride in elements): box 64 dims x box_heads x box_rows, 128-byte swizzle.
+int encode_heads_tmap(CUtensorMap* map, const void* base, int64_t rows, int heads, int head_dim, int64_t row_stride,
+                      int box_heads, int box_rows);
 
 // Launches one round on `stream`. `tmap` may be nullptr (encoded on the fly).
 // `splits` <= 0 picks the split-K factor automatically.
