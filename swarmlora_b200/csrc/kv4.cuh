@@ -74,6 +74,8 @@ int fill_cache(Cache* c, const char* what, int nseg, const void* const* block_ta
                void* const* caches, int64_t num_pages, const void* const* seqlens, int hkv, int head_dim, int page);
 // Row counts to row starts; the total is bounded so that row indices stay in 31 bits.
 int fill_rows(RowSegments* s, const char* what, int nseg, const int* rows);
+// The attention kernel's bounded-wait status on the current device; synchronous.
+int read_and_clear_error(unsigned int* code);
 
 }  // namespace kv4
 }  // namespace swl

@@ -1,6 +1,35 @@
 // Causal GQA attention of each slot's newest rows over its paged 4-bit cache.
+//
+// The work is the cache's bytes: 18 D per 16 tokens and kv head, read once. One
+// block (16 tokens of one kv head) is one contiguous piece, which a warp fetches with a single
+// bulk copy into its own ring and turns into matrix fragments without any
+// value being scaled on its own: a nibble v becomes the bf16 number 128 + v by
+// one logic operation on two nibbles (0x4300 | v), and scales and minima are
+// applied where they are cheap.
+//
+//   scores   q.k = sum over groups  s (sum q (128 + v)) + (m - 128 s) sum q
+//            per token and query column, after the product; sum q is known per piece.
+//   values   o = sum over tokens  p s (128 + v) + p m - 128 p s
+//            p s is rounded to bf16 as the second operand; the product with a
+//            row of ones gives the sum of the same rounded numbers, so the 128 cancels
+//            exactly but for fp32's sums. p m is summed in fp32.
+//
+// Tokens are the M dimension of the score product and dimensions that of the value
+// product; the columns are the slot's new rows times the query heads of the kv
+// head (8 NT of them a pass). The weights go from one layout to the other as fp16
+// (2^-11; they are at most 2^8 by the lazy reference) through a transposing
+// register move. The reference maximum moves only when a score passes it by 2^8,
+// so the common step needs one vote instead of a reduction.
+//
+// Work is shared out on the device, which alone knows the context lengths: with
+// few blocks per (slot, kv head) a CTA takes whole pairs; otherwise every CTA takes an equal
+// contiguous range of all blocks, a pair cut by a range boundary leaves partial
+// records (at most two a CTA) and a second launch joins them.
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
+#include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "common.h"
@@ -13,82 +42,637 @@ namespace kv4 {
 
 namespace {
 
+__device__ unsigned int g_kv4_error_word = 0;
+constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr unsigned kErrBlock = 111;
+constexpr float kRescaleLog2 = 8.f;
+constexpr int kWarps = 8;
+
 struct AttnTable4 {
   RowSegments seg;
   __nv_bfloat16* out[kMaxSlots];
   Cache c;
 };
 struct AttnParams4 {
-  int hq;
+  int hq, group;           // query heads, query heads per kv head
   int64_t out_stride;
-  float scale;
+  float scale_log2;
+  int max_len;
   const __nv_bfloat16* q;  // [total_rows, hq * D]
+  int whole;               // 1: CTAs take whole pairs; 0: equal ranges
+  float* part;             // equal ranges: O [record][column][D], then (m, l) [record][column][2]
 };
 
-// CTA = one (row, query head); a thread takes a key of each chunk of D tokens for the
-// scores, then a dimension for the values.
-template <int D>
-__global__ void __launch_bounds__(D) kv4_attention_kernel(const __grid_constant__ AttnTable4 tab, const AttnParams4 p) {
-  ptx::grid_dep_wait();
-  ptx::grid_dep_launch();
-  const int gr = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-  int s = 0;
-  while (tab.seg.row_start[s + 1] <= gr) ++s;
-  const int local = gr - tab.seg.row_start[s], hk = h / (p.hq / tab.c.hkv);
-  const int64_t len = static_cast<int64_t>(*tab.c.seqlen[s]) + local + 1;
-  __shared__ float q[D], pr[D], red[D / 32];
-  q[tid] = __bfloat162float(p.q[(static_cast<int64_t>(gr) * p.hq + h) * D + tid]) * p.scale;
-  float m = -INFINITY, l = 0.f, o = 0.f;
-  for (int64_t t0 = 0; t0 < len; t0 += D) {
-    __syncthreads();
-    const int64_t pos = t0 + tid;
-    const uint8_t* blk = pos < len ? block_of<D>(tab.c, s, pos >> 4, hk) : nullptr;
-    float sc = -INFINITY;
-    if (blk) {
-      const int t = static_cast<int>(pos & 15);
-      sc = 0.f;
-      for (int d = 0; d < D; d += 8) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(blk + k_word<D>(t, d));
-        const uint32_t pp = *reinterpret_cast<const uint32_t*>(blk + k_pair_off(D) + 4 * (t * (D / kGroup) + d / kGroup));
-        for (int e = 0; e < 8; ++e)
-          sc += q[d + e] * (__uint_as_float(pp << 16) * static_cast<float>(w >> (4 * e) & 15u) + __uint_as_float(pp & 0xffff0000u));
+template <int D, int NT>
+struct Cfg4 {
+  static constexpr int W = D / 32, NG = D / kGroup, kBlock = block_bytes(D);
+  static constexpr int kStages = (NT == 1 ? 4 : 6) * (128 / D);
+  static constexpr int kCols = 8 * NT;
+  static constexpr int kLd = D + 4;  // floats between columns of the merge buffer: no bank twice in a quarter warp
+  static constexpr int kRing = kWarps * kStages * kBlock;
+  static constexpr int kMerge = kWarps * 8 * kLd * 4;
+  static constexpr int kSmem = kRing + kMerge;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Two nibbles (bits 0-3 of each half) as bf16 128 + v.
+__device__ __forceinline__ uint32_t codes2(uint32_t w) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(r) : "r"(w));  // (w & mask) | 128.0 twice
+  return r;
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <int N>
+__device__ __forceinline__ void lds(const uint8_t* p, uint32_t* r) {
+  if constexpr (N == 4) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    r[0] = u.x; r[1] = u.y; r[2] = u.z; r[3] = u.w;
+  } else if constexpr (N == 2) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    r[0] = u.x; r[1] = u.y;
+  } else {
+    r[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+__device__ __forceinline__ float scale_of(uint32_t pair) { return __uint_as_float(pair << 16); }
+__device__ __forceinline__ float min_of(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
+
+// The division of the work, the same in every CTA and in the joining launch.
+struct Shares {
+  int blocks[kMaxSlots];          // cache blocks of each slot's context
+  int passes[kMaxSlots];          // column passes
+  int64_t unit[kMaxSlots + 1];    // blocks x kv heads x passes ahead of slot i
+  int pair[kMaxSlots + 1];        // kv heads x passes ahead of slot i
+  int64_t per_cta;
+};
+// A piece: blocks [b0, b1) of one (slot, kv head, pass).
+struct Piece {
+  int slot, head, pass, b0, b1, blocks;
+};
+
+template <int D, int NT>
+__device__ __forceinline__ void share_out(const AttnTable4& tab, const AttnParams4& p, Shares* sh, int ctas) {
+  if (threadIdx.x < 32) {
+    int64_t u = 0;
+    int pr = 0;
+    for (int s0 = 0; s0 < tab.seg.nseg; s0 += 32) {
+      const int s = s0 + threadIdx.x;
+      int nb = 0, np = 0;
+      if (s < tab.seg.nseg) {
+        const int rows = tab.seg.row_start[s + 1] - tab.seg.row_start[s];
+        if (rows > 0) {
+          const int64_t len = min(static_cast<int64_t>(*tab.c.seqlen[s]) + rows, static_cast<int64_t>(p.max_len));
+          nb = static_cast<int>((max(len, int64_t{1}) + kBlockTok - 1) / kBlockTok);
+          np = (rows * p.group + 8 * NT - 1) / (8 * NT) * tab.c.hkv;
+        }
+        sh->blocks[s] = nb;
+        sh->passes[s] = np / tab.c.hkv;
       }
+      int64_t a = static_cast<int64_t>(nb) * np;
+      int b = np;
+      const int64_t a0 = a;
+      const int b0 = b;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, a, o);
+        const int y = __shfl_up_sync(0xffffffffu, b, o);
+        if (static_cast<int>(threadIdx.x) >= o) {
+          a += x;
+          b += y;
+        }
+      }
+      if (s < tab.seg.nseg) {
+        sh->unit[s] = u + a - a0;
+        sh->pair[s] = pr + b - b0;
+      }
+      u += __shfl_sync(0xffffffffu, a, 31);
+      pr += __shfl_sync(0xffffffffu, b, 31);
     }
-    float mx = sc;
-    for (int x = 16; x; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-    if ((tid & 31) == 0) red[tid >> 5] = mx;
-    __syncthreads();
-    float mn = m;
-    for (int w = 0; w < D / 32; ++w) mn = fmaxf(mn, red[w]);
-    pr[tid] = sc == -INFINITY ? 0.f : expf(sc - mn);
-    __syncthreads();
-    const float corr = mn == -INFINITY ? 1.f : expf(m - mn);
-    l *= corr;
-    o *= corr;
-    m = mn;
-    const int n = static_cast<int>(min(static_cast<int64_t>(D), len - t0));
-    for (int i = 0; i < n; ++i) {
-      const uint8_t* b = block_of<D>(tab.c, s, (t0 + i) >> 4, hk);
-      if (!b) continue;
-      const int t = static_cast<int>((t0 + i) & 15);
-      const uint32_t pp = *reinterpret_cast<const uint32_t*>(b + v_pair_off(D) + 4 * (t * (D / kGroup) + tid / kGroup));
-      const uint32_t code = *reinterpret_cast<const uint16_t*>(b + v_piece<D>(t, tid & ~3)) >> (4 * (tid & 3)) & 15u;
-      l += pr[i];
-      o += pr[i] * (__uint_as_float(pp << 16) * static_cast<float>(code) + __uint_as_float(pp & 0xffff0000u));
+    if (threadIdx.x == 0) {
+      sh->unit[tab.seg.nseg] = u;
+      sh->pair[tab.seg.nseg] = pr;
+      sh->per_cta = max((u + ctas - 1) / ctas, int64_t{kWarps});
     }
   }
-  tab.out[s][static_cast<int64_t>(local) * p.out_stride + h * D + tid] = __float2bfloat16_rn(l == 0.f ? 0.f : o / l);
+  __syncthreads();
+}
+
+__device__ __forceinline__ int find_pair(const Shares& sh, int n, int pair) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (sh.pair[mid] <= pair) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Walks the pieces of this CTA.
+struct Walk {
+  int64_t u, end;  // equal ranges: next unit; whole pairs: next pair
+  int whole, step;
+  __device__ __forceinline__ Walk(const Shares& sh, int n, int whole_) : whole(whole_), step(gridDim.x) {
+    if (whole) {
+      u = blockIdx.x;
+      end = sh.pair[n];
+    } else {
+      u = min(blockIdx.x * sh.per_cta, sh.unit[n]);
+      end = min(u + sh.per_cta, sh.unit[n]);
+    }
+  }
+  __device__ __forceinline__ bool next(const Shares& sh, int n, Piece* x) {
+    if (u >= end) return false;
+    if (whole) {
+      const int s = find_pair(sh, n, static_cast<int>(u)), i = static_cast<int>(u) - sh.pair[s];
+      x->slot = s;
+      x->head = i / sh.passes[s];
+      x->pass = i % sh.passes[s];
+      x->blocks = x->b1 = sh.blocks[s];
+      x->b0 = 0;
+      u += step;
+      return true;
+    }
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (sh.unit[mid] <= u) lo = mid;
+      else hi = mid - 1;
+    }
+    const int64_t r = u - sh.unit[lo];
+    const int nb = sh.blocks[lo], i = static_cast<int>(r / nb);
+    x->slot = lo;
+    x->head = i / sh.passes[lo];
+    x->pass = i % sh.passes[lo];
+    x->blocks = nb;
+    x->b0 = static_cast<int>(r - static_cast<int64_t>(i) * nb);
+    x->b1 = static_cast<int>(min(static_cast<int64_t>(nb), x->b0 + (end - u)));
+    u += x->b1 - x->b0;
+    return true;
+  }
+};
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
+    kv4_attention_kernel(const __grid_constant__ AttnTable4 tab, const __grid_constant__ AttnParams4 p) {
+  using C = Cfg4<D, NT>;
+  constexpr int W = C::W, NG = C::NG, ST = C::kStages;
+  extern __shared__ __align__(128) uint8_t dyn[];
+  __shared__ Shares sh;
+  __shared__ __align__(8) uint64_t bars[kWarps][ST];
+  __shared__ float ml_sm[kWarps][8][2], corr_sm[kWarps][8][NG];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, c = lane & 3;
+  uint8_t* const ring = dyn + warp * ST * C::kBlock;
+  float* const merge = reinterpret_cast<float*>(dyn + C::kRing);
+  if (lane == 0) {
+    for (int i = 0; i < ST; ++i) ptx::mbar_init(&bars[warp][i], 1);
+    ptx::fence_mbar_init();
+  }
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch();
+  share_out<D, NT>(tab, p, &sh, gridDim.x);
+  const int nseg = tab.seg.nseg;
+
+  // ---- loads: this warp's blocks in the order in which it will use them ----
+  Walk lw(sh, nseg, p.whole);
+  Piece lp;
+  bool more = lw.next(sh, nseg, &lp);
+  int lb = more ? lp.b0 + warp : 0;       // next block of the load piece that is not in the batch
+  const uint8_t* addr = nullptr;          // lane i: the batch's i-th block (nullptr: no such page)
+  int batch = 0, taken = 0, issued = 0;
+  uint32_t ring_ok = 0;                   // bit per stage: the block exists
+  auto issue = [&]() {
+    while (more && taken == batch) {      // the next up to 32 blocks of this warp
+      const int left = lp.b1 > lb ? (lp.b1 - lb + kWarps - 1) / kWarps : 0;
+      if (left == 0) {
+        more = lw.next(sh, nseg, &lp);
+        lb = lp.b0 + warp;
+        continue;
+      }
+      batch = min(left, 32);
+      taken = 0;
+      addr = lane < batch ? block_of<D>(tab.c, lp.slot, lb + lane * kWarps, lp.head) : nullptr;
+      lb += batch * kWarps;
+    }
+    if (!more) return;
+    const uint64_t a = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(addr), taken);
+    const int st = issued % ST;
+    ring_ok = a ? ring_ok | 1u << st : ring_ok & ~(1u << st);
+    if (lane == 0 && a) {
+      ptx::mbar_arrive_expect_tx(&bars[warp][st], C::kBlock);
+      ptx::bulk_load(ring + st * C::kBlock, reinterpret_cast<const void*>(a), C::kBlock, &bars[warp][st]);
+    } else if (lane == 0) {
+      ptx::mbar_arrive(&bars[warp][st]);
+    }
+    ++taken;
+    ++issued;
+  };
+#pragma unroll 1
+  for (int i = 0; i < ST - 1; ++i) issue();
+
+  int used = 0;
+  uint64_t limit = kWaitNs;  // after a wait that gave up the others give up soon
+  Walk cw(sh, nseg, p.whole);
+  Piece x;
+  while (cw.next(sh, nseg, &x)) {
+    const int row0 = tab.seg.row_start[x.slot], rows = tab.seg.row_start[x.slot + 1] - row0;
+    const int ncols = rows * p.group, col0 = x.pass * C::kCols;
+    const int64_t len0 = *tab.c.seqlen[x.slot];
+    // ---- this piece's query columns: B fragments, sums per group, visible lengths ----
+    uint32_t qb[NT][2 * W][2];
+    float qs[NT][NG][2];
+    int seen[NT][2], seen_g[NT];  // tokens that columns 2c, 2c + 1 and column g see
+    int all_see = 0x7fffffff;     // tokens that every column sees
+    auto sees = [&](int col) {
+      const int64_t n = min(len0 + col / p.group + 1, static_cast<int64_t>(p.max_len));
+      return col < ncols ? static_cast<int>(max(n, int64_t{0})) : 0;
+    };
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int col = col0 + nt * 8 + g;
+      const __nv_bfloat16* src =
+          p.q + (static_cast<int64_t>(row0 + col / p.group) * p.hq + x.head * p.group + col % p.group) * D;
+      float part[NG];
+#pragma unroll
+      for (int i = 0; i < NG; ++i) part[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const uint4 u = col < ncols ? *reinterpret_cast<const uint4*>(src + 32 * j + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
+        qb[nt][2 * j][0] = __byte_perm(u.x, u.z, 0x5410);
+        qb[nt][2 * j][1] = __byte_perm(u.x, u.z, 0x7632);
+        qb[nt][2 * j + 1][0] = __byte_perm(u.y, u.w, 0x5410);
+        qb[nt][2 * j + 1][1] = __byte_perm(u.y, u.w, 0x7632);
+        const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          part[j / 2] += __uint_as_float(w4[e] << 16) + __uint_as_float(w4[e] & 0xffff0000u);
+      }
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        part[i] += __shfl_xor_sync(0xffffffffu, part[i], 1);
+        part[i] += __shfl_xor_sync(0xffffffffu, part[i], 2);
+        qs[nt][i][0] = __shfl_sync(0xffffffffu, part[i], 8 * c);
+        qs[nt][i][1] = __shfl_sync(0xffffffffu, part[i], 8 * c + 4);
+      }
+      seen[nt][0] = sees(col0 + nt * 8 + 2 * c);
+      seen[nt][1] = sees(col0 + nt * 8 + 2 * c + 1);
+      seen_g[nt] = sees(col);
+    }
+    all_see = sees(col0);  // the pass's first column belongs to its first row
+    float o[NT][2 * W][4], ps[NT][NG][4], corr[NT][NG], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < 2 * W; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        ps[nt][i][0] = ps[nt][i][1] = ps[nt][i][2] = ps[nt][i][3] = 0.f;
+        corr[nt][i] = 0.f;
+      }
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+#pragma unroll 1
+    for (int b = x.b0 + warp; b < x.b1; b += kWarps) {
+      const int st = used % ST;
+      const uint8_t* const blk = ring + st * C::kBlock;
+      const bool there = ring_ok >> st & 1u;
+      if (!ptx::mbar_wait(&bars[warp][st], (used / ST) & 1, &g_kv4_error_word, kErrBlock, limit)) limit = 1000000;
+      ++used;
+      issue();  // into the stage that the previous block left
+      if (!there) continue;
+      const int tok0 = b * kBlockTok;
+      const bool edge = tok0 + kBlockTok > all_see;  // some column ends in this block
+      uint32_t kw[2][W], kp[2][NG];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        lds<W>(blk + (h * 32 + lane) * W * 4, kw[h]);
+        lds<NG>(blk + k_pair_off(D) + (h * 8 + g) * NG * 4, kp[h]);
+      }
+      float acc[NT][NG][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < NG; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t a0 = codes2(kw[0][j] >> (8 * e)), a1 = codes2(kw[1][j] >> (8 * e));
+          const uint32_t a2 = codes2(kw[0][j] >> (8 * e + 4)), a3 = codes2(kw[1][j] >> (8 * e + 4));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma16816(acc[nt][j / 2], a0, a1, a2, a3, qb[nt][2 * j + e][0], qb[nt][2 * j + e][1]);
+        }
+      // scores of tokens g, g + 8 and columns 2c, 2c + 1, in units of log2
+      float sc[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[nt][i] = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          const float s = scale_of(kp[h][i]), mp = fmaf(-128.f, s, min_of(kp[h][i]));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              sc[nt][2 * h + k] += fmaf(s, acc[nt][i][2 * h + k], mp * qs[nt][i][k]);
+        }
+      bool grow = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sc[nt][i] *= p.scale_log2;
+          if (edge && tok0 + g + 8 * (i >> 1) >= seen[nt][i & 1]) sc[nt][i] = -INFINITY;
+          grow |= sc[nt][i] > m[nt][i & 1] + kRescaleLog2;
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float f[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float mx = fmaxf(sc[nt][k], sc[nt][2 + k]);
+#pragma unroll
+            for (int q = 4; q < 32; q <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, q));
+            const float mn = fmaxf(m[nt][k], mx);
+            f[k] = m[nt][k] == mn ? 1.f : ex2(m[nt][k] - mn);
+            m[nt][k] = mn;
+            l[nt][k] *= f[k];
+          }
+#pragma unroll
+          for (int i = 0; i < 2 * W; ++i) {
+            o[nt][i][0] *= f[0];
+            o[nt][i][1] *= f[1];
+            o[nt][i][2] *= f[0];
+            o[nt][i][3] *= f[1];
+          }
+          const float fe = __shfl_sync(0xffffffffu, f[0], g >> 1), fo = __shfl_sync(0xffffffffu, f[1], g >> 1);
+#pragma unroll
+          for (int i = 0; i < NG; ++i) {
+            ps[nt][i][0] *= f[0];
+            ps[nt][i][1] *= f[1];
+            corr[nt][i] *= (g & 1) ? fo : fe;
+          }
+        }
+      }
+      uint32_t vw[2][W], vp[2][2 * NG];  // vp[h]: tokens 2c, 2c + 1 (+ 8 h)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        lds<W>(blk + v_code_off(D) + (h * 32 + lane) * W * 4, vw[h]);
+        lds<2 * NG>(blk + v_pair_off(D) + (h * 8 + 2 * c) * NG * 4, vp[h]);
+      }
+      uint32_t pb[NT][NG][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float pe = ex2(sc[nt][2 * h] - m0), po = ex2(sc[nt][2 * h + 1] - m1);
+          l[nt][0] += pe;
+          l[nt][1] += po;
+          const __half2 hp = __floats2half2_rn(pe, po);
+          const uint32_t tr = transpose8x8(*reinterpret_cast<const uint32_t*>(&hp));
+          const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&tr));  // column g, tokens 2c, 2c + 1 (+ 8 h)
+          const bool hide0 = edge && tok0 + 8 * h + 2 * c >= seen_g[nt], hide1 = edge && tok0 + 8 * h + 2 * c + 1 >= seen_g[nt];
+#pragma unroll
+          for (int i = 0; i < NG; ++i) {
+            // a hidden token's pair may be anything, a NaN too: its weight of 0 does not meet it
+            const uint32_t w0 = hide0 ? 0u : vp[h][i], w1 = hide1 ? 0u : vp[h][NG + i];
+            pb[nt][i][h] = pack_bf16x2(w.x * scale_of(w0), w.y * scale_of(w1));
+            corr[nt][i] = fmaf(w.x, min_of(w0), fmaf(w.y, min_of(w1), corr[nt][i]));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+          mma16816(ps[nt][i], 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, pb[nt][i][0], pb[nt][i][1]);
+      }
+#pragma unroll
+      for (int u = 0; u < W; ++u)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t a0 = codes2(vw[0][u] >> (8 * e)), a1 = codes2(vw[0][u] >> (8 * e + 4));
+          const uint32_t a2 = codes2(vw[1][u] >> (8 * e)), a3 = codes2(vw[1][u] >> (8 * e + 4));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][2 * u + e], a0, a1, a2, a3, pb[nt][u / 2][0], pb[nt][u / 2][1]);
+        }
+      __syncwarp();  // every lane has read the stage before it is filled again
+    }
+    // ---- the warps' results joined ----
+    const bool full = x.b0 == 0 && x.b1 == x.blocks;
+    const int rec = 2 * blockIdx.x + (p.whole || static_cast<int64_t>(blockIdx.x) * sh.per_cta ==
+                                                     cw.u - (x.b1 - x.b0) ? 0 : 1);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      if (col0 + nt * 8 >= ncols) break;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float s = l[nt][k];
+#pragma unroll
+        for (int q = 4; q < 32; q <<= 1) s += __shfl_xor_sync(0xffffffffu, s, q);
+        if (g == 0) {
+          ml_sm[warp][2 * c + k][0] = m[nt][k];
+          ml_sm[warp][2 * c + k][1] = s;
+        }
+        float* dst = merge + (warp * 8 + 2 * c + k) * C::kLd + 4 * g;
+#pragma unroll
+        for (int u = 0; u < W; ++u) {
+          const float z = 128.f * ps[nt][u / 2][k];
+          *reinterpret_cast<float4*>(dst + 32 * u) = make_float4(o[nt][2 * u][k] - z, o[nt][2 * u][2 + k] - z,
+                                                                 o[nt][2 * u + 1][k] - z, o[nt][2 * u + 1][2 + k] - z);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        float s = corr[nt][i];
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        if (c == 0) corr_sm[warp][g][i] = s;
+      }
+      __syncthreads();
+      const int mc = threadIdx.x / (D / 4), d4 = threadIdx.x % (D / 4) * 4;  // column of the 8, dimensions
+      const int col = col0 + nt * 8 + mc;
+      if (mc < 8 && col < ncols) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml_sm[w][mc][0]);
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float mw = ml_sm[w][mc][0], lw_ = ml_sm[w][mc][1];
+          // no reference: nothing seen (no sum), or nothing but NaN, which stays
+          const float f = mw == -INFINITY ? (lw_ == 0.f ? 0.f : 1.f) : ex2(mw - top);
+          if (f == 0.f) continue;
+          const float4 v = *reinterpret_cast<const float4*>(merge + (w * 8 + mc) * C::kLd + d4);
+          const float z = corr_sm[w][mc][d4 / kGroup];
+          sum += f * lw_;
+          a.x += f * (v.x + z);
+          a.y += f * (v.y + z);
+          a.z += f * (v.z + z);
+          a.w += f * (v.w + z);
+        }
+        if (full) {
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          uint2 w2;
+          w2.x = pack_bf16x2(a.x * inv, a.y * inv);
+          w2.y = pack_bf16x2(a.z * inv, a.w * inv);
+          *reinterpret_cast<uint2*>(tab.out[x.slot] + static_cast<int64_t>(col / p.group) * p.out_stride +
+                                    (x.head * p.group + col % p.group) * D + d4) = w2;
+        } else {
+          const int64_t r = static_cast<int64_t>(rec) * C::kCols + nt * 8 + mc;
+          *reinterpret_cast<float4*>(p.part + r * D + d4) = a;
+          if (d4 == 0) {
+            float* ml = p.part + static_cast<int64_t>(2 * gridDim.x) * C::kCols * D + r * 2;
+            ml[0] = top;
+            ml[1] = sum;
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Joins the partial records of one (slot, kv head, pass).
+template <int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32)
+    kv4_join_kernel(const __grid_constant__ AttnTable4 tab, const __grid_constant__ AttnParams4 p, int ctas) {
+  using C = Cfg4<D, NT>;
+  __shared__ Shares sh;
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch();
+  share_out<D, NT>(tab, p, &sh, ctas);
+  const int pair = blockIdx.x, n = tab.seg.nseg;
+  if (pair >= sh.pair[n]) return;
+  const int s = find_pair(sh, n, pair), i = pair - sh.pair[s];
+  const int64_t u0 = sh.unit[s] + static_cast<int64_t>(i) * sh.blocks[s], u1 = u0 + sh.blocks[s];
+  const int c0 = static_cast<int>(u0 / sh.per_cta), c1 = static_cast<int>((u1 - 1) / sh.per_cta);
+  if (c0 == c1) return;  // written whole
+  const int head = i / sh.passes[s], pass = i % sh.passes[s];
+  const int ncols = (tab.seg.row_start[s + 1] - tab.seg.row_start[s]) * p.group;
+  const float* mls = p.part + static_cast<int64_t>(2 * ctas) * C::kCols * D;
+  for (int k = threadIdx.x; k < C::kCols * (D / 4); k += blockDim.x) {
+    const int mc = k / (D / 4), d4 = k % (D / 4) * 4, col = pass * C::kCols + mc;
+    if (col >= ncols) continue;
+    auto record = [&](int cta) {
+      return (2 * static_cast<int64_t>(cta) + (cta == c0 && u0 != c0 * sh.per_cta ? 1 : 0)) * C::kCols + mc;
+    };
+    float top = -INFINITY;
+    for (int cta = c0; cta <= c1; ++cta) top = fmaxf(top, mls[record(cta) * 2]);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+    for (int cta = c0; cta <= c1; ++cta) {
+      const int64_t r = record(cta);
+      const float mw = mls[2 * r], lw = mls[2 * r + 1];
+      const float f = mw == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : ex2(mw - top);
+      if (f == 0.f) continue;
+      const float4 v = *reinterpret_cast<const float4*>(p.part + r * D + d4);
+      sum += f * lw;
+      a.x += f * v.x;
+      a.y += f * v.y;
+      a.z += f * v.z;
+      a.w += f * v.w;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    uint2 w2;
+    w2.x = pack_bf16x2(a.x * inv, a.y * inv);
+    w2.y = pack_bf16x2(a.z * inv, a.w * inv);
+    *reinterpret_cast<uint2*>(tab.out[s] + static_cast<int64_t>(col / p.group) * p.out_stride +
+                              (head * p.group + col % p.group) * D + d4) = w2;
+  }
+}
+
+struct Plan4 {
+  int nt, ctas, whole;
+  int64_t pairs;
+};
+
+int sm_count4() {
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n > 0 ? n : 148;
+}
+
+Plan4 make_plan4(int nseg, const int* rows, int hq, int hkv, int max_len) {
+  Plan4 pl;
+  const int group = hq / hkv;
+  int most = 0;
+  for (int i = 0; i < nseg; ++i) most = std::max(most, rows[i]);
+  pl.nt = static_cast<int64_t>(most) * group > 8 ? 2 : 1;
+  pl.pairs = 0;
+  for (int i = 0; i < nseg; ++i) pl.pairs += (static_cast<int64_t>(rows[i]) * group + 8 * pl.nt - 1) / (8 * pl.nt) * hkv;
+  const int64_t blocks = (max_len + kBlockTok - 1) / kBlockTok;
+  const int64_t slots = static_cast<int64_t>(sm_count4()) * (pl.nt == 1 ? 2 : 1);  // CTAs at a time
+  // whole pairs where cutting them would at most halve what a CTA has to do
+  pl.whole = blocks <= 2 * std::max<int64_t>((pl.pairs * blocks + slots - 1) / slots, kWarps) ? 1 : 0;
+  pl.ctas = static_cast<int>(std::max<int64_t>(
+      1, std::min<int64_t>(slots, pl.whole ? pl.pairs : (pl.pairs * blocks + kWarps - 1) / kWarps)));
+  return pl;
+}
+
+template <int D, int NT>
+int launch_kv4(const AttnTable4& t, const AttnParams4& p, const Plan4& pl, cudaStream_t st) {
+  int dev = 0;
+  SWL_CUDA_TRY(cudaGetDevice(&dev));
+  static std::atomic<uint64_t> done{0};  // devices whose kernel has its shared memory limit raised
+  const uint64_t bit = uint64_t{1} << (dev & 63);
+  if (!(done.load(std::memory_order_relaxed) & bit)) {
+    SWL_CUDA_TRY(cudaFuncSetAttribute(kv4_attention_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      Cfg4<D, NT>::kSmem));
+    done.fetch_or(bit);
+  }
+  SWL_CUDA_TRY(launch_kernel(kv4_attention_kernel<D, NT>, dim3(pl.ctas), dim3(kWarps * 32), Cfg4<D, NT>::kSmem, st, 1, t, p));
+  if (!pl.whole)
+    SWL_CUDA_TRY(launch_kernel(kv4_join_kernel<D, NT>, dim3(static_cast<unsigned>(pl.pairs)), dim3(kWarps * 32), 0, st, 1, t, p,
+                               pl.ctas));
+  return SWL_OK;
 }
 
 }  // namespace
+
+int read_and_clear_error(unsigned int* code) {
+  const unsigned int zero = 0;
+  SWL_CUDA_TRY(cudaMemcpyFromSymbol(code, g_kv4_error_word, sizeof(zero)));
+  if (*code) SWL_CUDA_TRY(cudaMemcpyToSymbol(g_kv4_error_word, &zero, sizeof(zero)));
+  return SWL_OK;
+}
+
 }  // namespace kv4
 }  // namespace swl
 
 using namespace swl;
 
 SWL_EXPORT int64_t swl_kv4_part_floats(int nseg, const int* rows, int hq, int hkv, int head_dim, int max_len) {
-  (void)nseg; (void)rows; (void)hq; (void)hkv; (void)head_dim; (void)max_len;
-  return 0;
+  RowSegments seg;
+  if (kv4::fill_rows(&seg, "attention_kv4", nseg, rows) != SWL_OK || hkv < 1 || hq < 1 || hq % hkv || max_len < 1) return 0;
+  if (head_dim != 64 && head_dim != 128) return 0;
+  const kv4::Plan4 pl = kv4::make_plan4(nseg, rows, hq, hkv, max_len);
+  return pl.whole ? 0 : static_cast<int64_t>(2 * pl.ctas) * 8 * pl.nt * (head_dim + 2);
 }
 
 SWL_EXPORT int swl_paged_attention_kv4(int nseg, const int* rows, const void* const* block_tables, int table_len,
@@ -112,16 +696,21 @@ SWL_EXPORT int swl_paged_attention_kv4(int nseg, const int* rows, const void* co
     if (!t.out[i] || (reinterpret_cast<uintptr_t>(t.out[i]) & 15))
       return set_error(SWL_ERR_ARG, "attention_kv4: outputs must be 16-byte aligned");
   }
-  (void)part;
   if (t.seg.total_rows == 0) return SWL_OK;
+  const kv4::Plan4 pl = kv4::make_plan4(nseg, rows, hq, hkv, max_len);
+  if (static_cast<int64_t>(t.seg.total_rows) * hq > (1 << 30)) return set_error(SWL_ERR_ARG, "attention_kv4: too many rows");
+  if (!pl.whole && (!part || (reinterpret_cast<uintptr_t>(part) & 15)))
+    return set_error(SWL_ERR_ARG, "attention_kv4: missing or unaligned scratch");
   kv4::AttnParams4 p;
   p.hq = hq;
+  p.group = hq / hkv;
   p.out_stride = out_stride;
-  p.scale = scale;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.max_len = max_len;
   p.q = static_cast<const __nv_bfloat16*>(q_rot);
-  const dim3 grid(t.seg.total_rows, hq);
+  p.whole = pl.whole;
+  p.part = part;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  SWL_CUDA_TRY(head_dim == 128 ? launch_kernel(kv4::kv4_attention_kernel<128>, grid, dim3(128), 0, st, 1, t, p)
-                               : launch_kernel(kv4::kv4_attention_kernel<64>, grid, dim3(64), 0, st, 1, t, p));
-  return SWL_OK;
+  if (head_dim == 128) return pl.nt == 1 ? kv4::launch_kv4<128, 1>(t, p, pl, st) : kv4::launch_kv4<128, 2>(t, p, pl, st);
+  return pl.nt == 1 ? kv4::launch_kv4<64, 1>(t, p, pl, st) : kv4::launch_kv4<64, 2>(t, p, pl, st);
 }

@@ -591,5 +591,8 @@ SWL_EXPORT int swl_attention_device_error(unsigned int* code) {
   const unsigned int zero = 0;
   SWL_CUDA_TRY(cudaMemcpyFromSymbol(code, g_prompt_error_word, sizeof(zero)));
   if (*code) SWL_CUDA_TRY(cudaMemcpyToSymbol(g_prompt_error_word, &zero, sizeof(zero)));
+  unsigned int other = 0;
+  SWL_TRY(kv4::read_and_clear_error(&other));
+  if (!*code) *code = other;
   return SWL_OK;
 }
