@@ -13,10 +13,13 @@
 // registers. The two tiles alternate, so the tensor cores work on one while
 // the warps of the other compute exponentials.
 //
-//   warps 0-3, 4-7   softmax of tile 0 and tile 1, and their epilogue
-//   warp 8           TMA: Q once, K and V tiles through a ring; also looks over the V tiles
-//                    of the masked range (below)
-//   warp 9           issues every MMA (one lane); owns the tensor memory
+//   warps 0-3, 4-7   softmax of row tile 0 and 1, and their epilogue
+//   warp 8           TMA: Q, and K and V tiles through a ring
+//   warps 9, 10      issue the products of row tile 0 and 1 (one lane); 9 owns the tensor memory
+//   warp 11          looks over the V tiles of the masked range (below)
+//
+// A CTA stays and takes one item after the other: the copies and score products
+// of the next item run while the rows of the last one are written.
 //
 // O is rescaled only when a row's maximum passes its reference by more than
 // 2^8 (then by the softmax warps themselves, which have just seen the MMA
@@ -50,6 +53,7 @@ __device__ unsigned int g_prompt_error_word = 0;
 constexpr uint64_t kWaitNs = 2000000000ull;
 enum : unsigned { kErrSoftmax = 101, kErrMma = 102, kErrTma = 103 };
 
+constexpr int kThreads = 384;        // three warpgroups; the last has its registers moved to the others
 constexpr int kTile = 128;           // query rows of a tile, keys of a step
 constexpr float kRescaleLog2 = 8.f;  // a row's weights may pass its reference by 2^8
 
@@ -64,7 +68,8 @@ struct PromptParams {
   int64_t out_stride, v_stride;
   int hq, hkv, group, tokens;  // query heads per kv head, tokens per tile
   float scale_log2;
-  int splits;                  // CTAs that share a block's keys
+  int items;                   // blocks x kv heads x splits
+  int splits;                  // items that share a block's keys
   float* part;                 // splits > 1: O [row][head][split][D], then (m, l) pairs
   int64_t part_rows;           // rows * heads * splits
 };
@@ -72,9 +77,9 @@ struct PromptParams {
 template <int D>
 struct Cfg {
   static constexpr int kHalves = D / 64;
-  static constexpr int kSlots = D == 128 ? 4 : 6;
+  static constexpr int kStages = D == 128 ? 2 : 4;  // tiles of K, and of V
   static constexpr int kTileBytes = kTile * D * 2;
-  static constexpr int kSmem = (2 + kSlots) * kTileBytes + 1024;
+  static constexpr int kSmem = (2 + 2 * kStages) * kTileBytes + 1024;
   static constexpr uint32_t kS = 0, kO = 2 * kTile, kCols = 512;  // tensor memory columns
 };
 
@@ -83,23 +88,41 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)), "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// What the CTA of blockIdx.x works on.
+// One unit of a CTA's work: a block of queries of one sequence and kv head, over a range of its keys.
 struct Item {
   int seq, head, split;
   int t0[2], nt[2];   // first token and token count of each tile (0: no rows)
   int first[2];       // keys the first row of a tile sees (may be negative)
-  int kb, ke[2];      // key tiles [kb, ke) of each tile
-  int clean;          // key tiles from here on hold keys that some row does not see
+  int kb;             // first key tile
+  int n[2], nk;       // key tiles of each row tile, and of the item
+  int clean;          // key tiles of the item from this one on hold keys that some row does not see
 };
 
-__device__ __forceinline__ Item find_item(const PromptTable& t, const PromptParams& p) {
+__device__ __forceinline__ Item find_item(const PromptTable& t, const PromptParams& p, int i) {
   Item it;
-  int i = blockIdx.x;
   it.split = i % p.splits;
   i /= p.splits;
   it.head = i % p.hkv;
@@ -127,25 +150,49 @@ __device__ __forceinline__ Item find_item(const PromptTable& t, const PromptPara
   it.kb = static_cast<int>(static_cast<int64_t>(all) * it.split / p.splits);
   const int ke = static_cast<int>(static_cast<int64_t>(all) * (it.split + 1) / p.splits);
 #pragma unroll
-  for (int x = 0; x < 2; ++x) it.ke[x] = max(it.kb, min(n[x], ke));
-  it.clean = max(0, it.first[0]) / kTile;
+  for (int x = 0; x < 2; ++x) it.n[x] = max(0, min(n[x], ke) - it.kb);
+  it.nk = max(it.n[0], it.n[1]);
+  it.clean = max(0, max(0, it.first[0]) / kTile - it.kb);
   return it;
 }
 
+// The items of a CTA, from the heaviest: every second round runs the other way
+// round, so that no CTA always gets the heavier end of one.
+struct Rounds {
+  int round = 0;
+  __device__ __forceinline__ bool next(int items, int* i) {
+    for (;;) {
+      const int64_t base = static_cast<int64_t>(round) * gridDim.x;
+      if (base >= items) return false;
+      const int at = (round & 1) ? static_cast<int>(gridDim.x - 1 - blockIdx.x) : static_cast<int>(blockIdx.x);
+      ++round;
+      if (base + at < items) {
+        *i = static_cast<int>(base + at);
+        return true;
+      }
+    }
+  }
+};
+
 template <int D>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(kThreads, 1)
     prompt_attention_kernel(const __grid_constant__ PromptTable tab, const __grid_constant__ PromptParams p,
                             const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                             const __grid_constant__ CUtensorMap vmap) {
   using C = Cfg<D>;
+  constexpr int ST = C::kStages;
   extern __shared__ uint8_t dyn_raw[];
   uint8_t* const dyn = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* const q_sm = dyn;
-  uint8_t* const ring = dyn + 2 * C::kTileBytes;
-  __shared__ __align__(8) uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
-  __shared__ __align__(8) uint64_t full[C::kSlots], empty[C::kSlots], seen[4], drained;
+  uint8_t* const k_ring = dyn + 2 * C::kTileBytes;
+  uint8_t* const v_ring = k_ring + ST * C::kTileBytes;
+  // Who completes each barrier: *_full the copy or product that fills, *_empty who has used it.
+  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2];
+  __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], seen[2], turn[2], drained[2];
   __shared__ uint32_t tmem_base;
-  __shared__ int bad;  // a non-finite value of this sequence was taken out of a V tile
+  // [n & 7] == n + 1: a non-finite value of its sequence was taken out of a V tile of the
+  // CTA's n-th item with keys (copies run at most 4 items ahead of the rows, so n's are done when n + 8 comes)
+  __shared__ int bad[8];
   unsigned int* const err = &g_prompt_error_word;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -153,17 +200,23 @@ __global__ void __launch_bounds__(320, 1)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(&q_full[i], 1);
+      ptx::mbar_init(&q_empty[i], 1);
       ptx::mbar_init(&s_full[i], 1);
-      ptx::mbar_init(&p_full[i], 128);
+      ptx::mbar_init(&p_half[i], 4);
+      ptx::mbar_init(&p_full[i], 4);
       ptx::mbar_init(&o_full[i], 1);
+      ptx::mbar_init(&o_empty[i], 4);
+      ptx::mbar_init(&seen[i], 1);
+      ptx::mbar_init(&turn[i], 1);
+      ptx::mbar_init(&drained[i], 1);
     }
-    for (int i = 0; i < C::kSlots; ++i) {
-      ptx::mbar_init(&full[i], 1);
-      ptx::mbar_init(&empty[i], 1);
+    for (int i = 0; i < ST; ++i) {
+      ptx::mbar_init(&k_full[i], 1);
+      ptx::mbar_init(&k_empty[i], 2);
+      ptx::mbar_init(&v_full[i], 1);
+      ptx::mbar_init(&v_empty[i], 3);
     }
-    for (int i = 0; i < 4; ++i) ptx::mbar_init(&seen[i], 1);
-    ptx::mbar_init(&drained, 1);
-    bad = 0;
+    for (int i = 0; i < 8; ++i) bad[i] = 0;
     ptx::fence_mbar_init();
   }
   if (warp == 9) ptx::tmem_alloc(&tmem_base, C::kCols);
@@ -172,7 +225,6 @@ __global__ void __launch_bounds__(320, 1)
     ptx::prefetch_tmap(&kmap);
     ptx::prefetch_tmap(&vmap);
   }
-  const Item it = find_item(tab, p);
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
@@ -180,267 +232,344 @@ __global__ void __launch_bounds__(320, 1)
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
 
-  const int nk = max(it.ke[0], it.ke[1]) - it.kb;  // key tiles of this CTA
-  if (warp == 8) {
-    const int k_row0 = tab.k_start[it.seq];
-    if (lane == 0 && nk > 0) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        if (it.ke[x] <= it.kb) continue;
-        ptx::mbar_arrive_expect_tx(&q_full[x], p.tokens * p.group * D * 2);
-        for (int h = 0; h < C::kHalves; ++h)
-          ptx::tma_load_3d(ptx::smem_addr(q_sm + x * C::kTileBytes + h * kTile * 128), &qmap, &q_full[x], h * 64,
-                           it.head * p.group, tab.q_start[it.seq] + it.t0[x]);
-      }
-    }
-    const int klen = tab.k_len[it.seq];
-    // Takes non-finite values out of V tile j (of this CTA) and announces it.
-    auto look_over = [&](int j) {
-      const int n = 2 * j + 1, s = n % C::kSlots;
-      if (!ptx::mbar_wait(&full[s], (n / C::kSlots) & 1, err, kErrTma, kWaitNs)) return false;
-      uint4* const v = reinterpret_cast<uint4*>(ring + s * C::kTileBytes);
-      const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
-      for (int i = lane; i < C::kTileBytes / 16; i += 32) {
-        uint4 u = v[i];
-        __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
-        __nv_bfloat162 a = zero;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a = __hfma2(h[e], zero, a);  // 0 unless a factor is NaN or infinite
-        if (__low2float(a) != 0.f || __high2float(a) != 0.f || __hisnan(a.x) || __hisnan(a.y)) {
-          __nv_bfloat16* b = reinterpret_cast<__nv_bfloat16*>(&u);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (!isfinite(__bfloat162float(b[e]))) b[e] = __float2bfloat16_rn(0.f);
-          v[i] = u;
-          if ((it.kb + j) * kTile + (i / 8) % kTile < klen) bad = 1;
-        }
-      }
-      ptx::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&seen[(it.kb + j - max(it.kb, it.clean)) & 3]);
-      return true;
-    };
+  // registers at launch: 384 x 168 = 64512; 256 x 208 + 128 x 80 = 63488
+  if (warp >= 8) {
+    ptx::reg_dec<80>();
+    Rounds rounds;
+    int i;
+    uint32_t tiles = 0;  // key tiles of the items so far: ring position
     bool ok = true;
-    int issued = 0;
-    for (int j = 0; j < nk && ok; ++j) {
+    if (warp == 8) {
+      // ---- copies
+      if (lane == 0) {
+        uint32_t qn[2] = {0, 0}, issued = 0;  // copies of each row tile, and of K and V tiles
+        while (ok && rounds.next(p.items, &i)) {
+          const Item it = find_item(tab, p, i);
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const int n = 2 * j + kv, s = n % C::kSlots;
-        if (lane == 0 && ok) {
-          ok = n < C::kSlots || ptx::mbar_wait(&empty[s], ((n / C::kSlots) & 1) ^ 1, err, kErrTma, kWaitNs);
-          if (ok) {
-            ptx::mbar_arrive_expect_tx(&full[s], C::kTileBytes);
+          for (int x = 0; x < 2; ++x) {
+            if (!ok || it.n[x] == 0) continue;
+            ok = qn[x] == 0 || ptx::mbar_wait(&q_empty[x], (qn[x] - 1) & 1, err, kErrTma, kWaitNs);
+            if (!ok) continue;
+            ++qn[x];
+            ptx::mbar_arrive_expect_tx(&q_full[x], p.tokens * p.group * D * 2);
             for (int h = 0; h < C::kHalves; ++h)
-              ptx::tma_load_3d(ptx::smem_addr(ring + s * C::kTileBytes + h * kTile * 128), kv ? &vmap : &kmap, &full[s],
-                               h * 64, it.head, k_row0 + (it.kb + j) * kTile);
-            ++issued;
+              ptx::tma_load_3d(ptx::smem_addr(q_sm + x * C::kTileBytes + h * kTile * 128), &qmap, &q_full[x], h * 64,
+                               it.head * p.group, tab.q_start[it.seq] + it.t0[x]);
           }
-        }
-      }
-      ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0);
-      if (ok && j > 0 && it.kb + j - 1 >= it.clean) ok = look_over(j - 1);
-      ok = __all_sync(0xffffffffu, ok);
-    }
-    if (ok && nk > 0 && it.kb + nk - 1 >= it.clean) ok = look_over(nk - 1);
-    if (!ok && lane == 0) {
-      // a wait gave up: the copies that were issued land before the CTA ends
-      for (int n = max(0, issued - C::kSlots); n < issued; ++n)
-        ptx::mbar_wait(&full[n % C::kSlots], (n / C::kSlots) & 1, err, kErrTma, kWaitNs);
-      for (int x = 0; x < 2; ++x)
-        if (it.ke[x] > it.kb) ptx::mbar_wait(&q_full[x], 0, err, kErrTma, kWaitNs);
-    }
-  } else if (warp == 9) {
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = ptx::idesc_bf16_f32(kTile, kTile);
-      constexpr uint32_t idesc_o = ptx::idesc_bf16_f32(kTile, D) | ptx::kIdescBMnMajor;
-      const int n[2] = {it.ke[0] - it.kb, it.ke[1] - it.kb};
-      bool ok = true;
-      auto scores = [&](int x, int j) {  // S_x = Q_x K_j^T
-        const uint32_t q = ptx::smem_addr(q_sm + x * C::kTileBytes);
-        const uint32_t k = ptx::smem_addr(ring + (2 * j) % C::kSlots * C::kTileBytes);
+          const int row0 = tab.k_start[it.seq] + it.kb * kTile;
+          for (int j = 0; j < it.nk && ok; ++j, ++tiles) {
+            const int s = tiles % ST;
+            const uint32_t ph = ((tiles / ST) & 1) ^ 1;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t o = (kk >> 2) * kTile * 128 + (kk & 3) * 32;
-          ptx::mma_bf16_ss(tmem + C::kS + x * kTile, ptx::sw128_kmajor_desc(q + o), ptx::sw128_kmajor_desc(k + o),
-                           idesc_s, kk > 0 ? 1u : 0u);
-        }
-        ptx::tc_commit(&s_full[x]);
-      };
-      auto wait_full = [&](int i) {
-        return ptx::mbar_wait(&full[i % C::kSlots], (i / C::kSlots) & 1, err, kErrMma, kWaitNs);
-      };
-      if (nk > 0) {
-        ok = wait_full(0);
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (ok && n[x] > 0) {
-            ok = ptx::mbar_wait(&q_full[x], 0, err, kErrMma, kWaitNs);
-            if (ok) {
-              ptx::tc_fence_after();
-              scores(x, 0);
+            for (int kv = 0; kv < 2; ++kv) {
+              uint64_t* const bar = kv ? &v_full[s] : &k_full[s];
+              ok = ok && (tiles < ST || ptx::mbar_wait(kv ? &v_empty[s] : &k_empty[s], ph, err, kErrTma, kWaitNs));
+              if (!ok) break;
+              ptx::mbar_arrive_expect_tx(bar, C::kTileBytes);
+              const uint32_t dst = ptx::smem_addr((kv ? v_ring : k_ring) + s * C::kTileBytes);
+              for (int h = 0; h < C::kHalves; ++h)
+                ptx::tma_load_3d(dst + h * kTile * 128, kv ? &vmap : &kmap, bar, h * 64, it.head, row0 + j * kTile);
+              ++issued;
             }
           }
-        ptx::tc_commit(&empty[0]);
+        }
+        if (!ok) {  // a wait gave up: the copies that were issued land before the CTA ends
+          for (uint32_t n = issued > 2 * ST ? issued - 2 * ST : 0; n < issued; ++n)
+            ptx::mbar_wait((n & 1) ? &v_full[n / 2 % ST] : &k_full[n / 2 % ST], (n / 2 / ST) & 1, err, kErrTma, kWaitNs);
+          for (int x = 0; x < 2; ++x)
+            if (qn[x]) ptx::mbar_wait(&q_full[x], (qn[x] - 1) & 1, err, kErrTma, kWaitNs);
+        }
       }
-      for (int j = 0; j < nk && ok; ++j) {
-        const int vs = (2 * j + 1) % C::kSlots;
-        ok = wait_full(2 * j + 1);
-        const int looked = it.kb + j - max(it.kb, it.clean);
-        if (ok && looked >= 0) ok = ptx::mbar_wait(&seen[looked & 3], (looked >> 2) & 1, err, kErrMma, kWaitNs);
-        if (ok && j + 1 < nk) ok = wait_full(2 * j + 2);
+    } else if (warp == 11) {
+      // ---- takes non-finite values out of the V tiles that some row sees only in part
+      uint32_t looked = 0;
+      int busy = 0;
+      while (ok && rounds.next(p.items, &i)) {
+        const Item it = find_item(tab, p, i);
+        if (it.nk == 0) continue;
+        const int klen = tab.k_len[it.seq];
+        for (int j = 0; j < it.nk && ok; ++j, ++tiles) {
+          // every tile's barrier is waited for and released, so that it never runs two phases ahead
+          ok = ptx::mbar_wait(&v_full[tiles % ST], (tiles / ST) & 1, err, kErrTma, kWaitNs);
+          __syncwarp();
+          if (ok && j < it.clean && lane == 0) ptx::mbar_arrive(&v_empty[tiles % ST]);
+          if (!ok || j < it.clean) continue;
+          uint4* const v = reinterpret_cast<uint4*>(v_ring + (tiles % ST) * C::kTileBytes);
+          const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
+#pragma unroll 1
+          for (int b = lane; b < C::kTileBytes / 16; b += 32 * 8) {
+            uint4 u[8];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if (!ok || j >= n[x]) continue;
-          ok = ptx::mbar_wait(&p_full[x], j & 1, err, kErrMma, kWaitNs);
+            for (int q = 0; q < 8; ++q) u[q] = v[b + 32 * q];
+            uint32_t odd = 0;  // bit q: u[q] holds a non-finite value
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u[q]);
+              __nv_bfloat162 a = zero;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) a = __hfma2(h[e], zero, a);  // NaN where a factor is not finite
+              if (!(__low2float(a) == 0.f) || !(__high2float(a) == 0.f)) odd |= 1u << q;
+            }
+            if (odd) {
+#pragma unroll 1
+              for (int q = 0; q < 8; ++q) {
+                if (!(odd >> q & 1u)) continue;
+                __nv_bfloat16* w = reinterpret_cast<__nv_bfloat16*>(v + b + 32 * q);
+                for (int e = 0; e < 8; ++e)
+                  if (!isfinite(__bfloat162float(w[e]))) w[e] = __float2bfloat16_rn(0.f);
+                if ((it.kb + j) * kTile + (b + 32 * q) / 8 % kTile < klen) bad[busy & 7] = busy + 1;
+              }
+            }
+          }
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            ptx::mbar_arrive(&seen[looked & 1]);
+            ptx::mbar_arrive(&v_empty[tiles % ST]);
+          }
+          ++looked;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        ++busy;
+      }
+    } else if (lane == 0) {
+      // ---- products of row tile x: each tile has its own issuing warp, so that one's waits
+      // pass while the other's products run
+      const int x = warp - 9;
+      constexpr uint32_t idesc_s = ptx::idesc_bf16_f32(kTile, kTile);
+      constexpr uint32_t idesc_o = ptx::idesc_bf16_f32(kTile, D) | ptx::kIdescBMnMajor;
+      const uint32_t ts = tmem + C::kS + x * kTile, to = tmem + C::kO + x * D;
+      const uint64_t qd = ptx::sw128_kmajor_desc(ptx::smem_addr(q_sm + x * C::kTileBytes));
+      const uint64_t kd = ptx::sw128_kmajor_desc(ptx::smem_addr(k_ring));
+      const uint64_t vd = ptx::sw128_mnmajor_desc(ptx::smem_addr(v_ring), kTile * 128);
+      uint32_t qn = 0, pn = 0, looked = 0;  // items and key tiles of this row tile; V tiles looked over
+      auto scores = [&](uint32_t tile) {    // S = Q K^T
+        const uint64_t k = kd + (tile % ST) * (C::kTileBytes >> 4);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t o = ((kk >> 2) * kTile * 128 + (kk & 3) * 32) >> 4;
+          ptx::mma_bf16_ss(ts, qd + o, k + o, idesc_s, kk > 0 ? 1u : 0u);
+        }
+        ptx::tc_commit(&s_full[x]);
+        ptx::tc_commit(&k_empty[tile % ST]);
+      };
+      while (ok && rounds.next(p.items, &i)) {
+        const Item it = find_item(tab, p, i);
+        const int n = it.n[x];
+        if (it.nk == 0) continue;
+        ok = ptx::mbar_wait(&k_full[tiles % ST], (tiles / ST) & 1, err, kErrMma, kWaitNs);
+        if (ok && n > 0) {
+          ok = ptx::mbar_wait(&q_full[x], qn & 1, err, kErrMma, kWaitNs);
           if (!ok) break;
           ptx::tc_fence_after();
-          const uint32_t v = ptx::smem_addr(ring + vs * C::kTileBytes);
+          scores(tiles);
+          if (n == 1) ptx::tc_commit(&q_empty[x]);
+        } else if (ok) {
+          ptx::mbar_arrive(&k_empty[tiles % ST]);
+        }
+        for (int j = 0; j < it.nk && ok; ++j, ++tiles) {
+          const int s = tiles % ST;
+          // everything this step needs is waited for, used or not, so that no barrier is ever two phases ahead
+          ok = ptx::mbar_wait(&v_full[s], (tiles / ST) & 1, err, kErrMma, kWaitNs);
+          if (ok && j >= it.clean) {
+            ok = ptx::mbar_wait(&seen[looked & 1], (looked >> 1) & 1, err, kErrMma, kWaitNs);
+            ++looked;
+          }
+          if (ok && j + 1 < it.nk)
+            ok = ptx::mbar_wait(&k_full[(tiles + 1) % ST], ((tiles + 1) / ST) & 1, err, kErrMma, kWaitNs);
+          if (ok && j < n) {
+            if (j == 0 && qn > 0) ok = ptx::mbar_wait(&o_empty[x], (qn - 1) & 1, err, kErrMma, kWaitNs);
+            ok = ok && ptx::mbar_wait(&p_half[x], pn & 1, err, kErrMma, kWaitNs);
+          }
+          // the two warps issue a step in turn: 0, 1, 0, 1, ..., so the row tiles stay half a step apart
+          // (in step, both would wait for their exponentials at once and leave the tensor cores idle)
+          if (ok && (x == 1 || tiles > 0)) ok = ptx::mbar_wait(&turn[x], (x == 1 ? tiles : tiles - 1) & 1, err, kErrMma, kWaitNs);
+          if (!ok) break;
+          if (j < n) {
+            const uint64_t v = vd + s * (C::kTileBytes >> 4);
 #pragma unroll
-          for (int kk = 0; kk < kTile / 16; ++kk)
-            ptx::mma_bf16_ts(tmem + C::kO + x * D, tmem + C::kS + x * kTile + kk * 8,
-                             ptx::sw128_mnmajor_desc(v + kk * 16 * 128, kTile * 128), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
-          if (j + 1 == n[x]) ptx::tc_commit(&o_full[x]);
-          if (j + 1 < n[x]) scores(x, j + 1);
+            for (int half = 0; half < 2; ++half) {
+              if (half) ok = ptx::mbar_wait(&p_full[x], pn & 1, err, kErrMma, kWaitNs);
+              if (!ok) break;
+              ptx::tc_fence_after();
+#pragma unroll
+              for (int kk = half * 4; kk < half * 4 + 4; ++kk)
+                ptx::mma_bf16_ts(to, ts + kk * 8, v + kk * (16 * 128 >> 4), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+            }
+            if (!ok) break;
+            ++pn;
+            ptx::tc_commit(&v_empty[s]);
+            if (j + 1 == n) {
+              ptx::tc_commit(&o_full[x]);
+            } else {
+              scores(tiles + 1);
+              if (j + 2 == n) ptx::tc_commit(&q_empty[x]);
+            }
+          } else {
+            ptx::mbar_arrive(&v_empty[s]);
+          }
+          if (j + 1 >= n && j + 1 < it.nk) ptx::mbar_arrive(&k_empty[(tiles + 1) % ST]);
+          ptx::mbar_arrive(&turn[x ^ 1]);
         }
-        if (ok) {
-          ptx::tc_commit(&empty[vs]);
-          if (j + 1 < nk) ptx::tc_commit(&empty[(2 * j + 2) % C::kSlots]);
-        }
+        if (n > 0) ++qn;
       }
       if (!ok) {  // a wait gave up: what was issued finishes before the tensor memory is freed
-        ptx::tc_commit(&drained);
-        ptx::mbar_wait(&drained, 0, err, kErrMma, kWaitNs);
+        ptx::tc_commit(&drained[x]);
+        ptx::mbar_wait(&drained[x], 0, err, kErrMma, kWaitNs);
       }
     }
     __syncwarp();
   } else {
-    const int x = warp >> 2;                 // tile
+    // ---- softmax and epilogue: a thread has one row
+    ptx::reg_inc<208>();
+    const int x = warp >> 2;                 // row tile
     const int r = (warp & 3) * 32 + lane;    // row of the tile = lane of the tensor memory
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + C::kS + x * kTile, to = tmem + lanes + C::kO + x * D;
-    const int n = it.ke[x] - it.kb, token = r / p.group;
-    const bool real = token < it.nt[x];
-    const int klen = tab.k_len[it.seq];
-    const int sees = real ? max(0, min(klen, it.first[x] + token)) : 0;  // keys 0 .. sees - 1
-    const int whole = max(0, it.first[x]) / kTile;  // tiles before this one need no mask
-    float m = -INFINITY, l = 0.f;  // reference (scaled, base 2) and sum of weights
+    const int token = r / p.group, head_in = r % p.group;
+    Rounds rounds;
+    int i, busy = 0;
+    uint32_t sn = 0, on = 0;  // key tiles and items of this row tile so far
     bool ok = true;
-    for (int j = 0; j < n; ++j) {
-      ok = ptx::mbar_wait(&s_full[x], j & 1, err, kErrSoftmax, kWaitNs);
-      if (!ok) break;
-      ptx::tc_fence_after();
-      uint32_t s[4][32];
+    while (ok && rounds.next(p.items, &i)) {
+      const Item it = find_item(tab, p, i);
+      const int n = it.n[x];
+      const bool real = token < it.nt[x];
+      const int sees = real ? max(0, min(tab.k_len[it.seq], it.first[x] + token)) : 0;  // keys 0 .. sees - 1
+      const int whole = max(0, it.first[x]) / kTile - it.kb;  // tiles before this one need no mask
+      float m = -INFINITY, l = 0.f;  // reference (scaled, base 2) and sum of weights
+      for (int j = 0; j < n; ++j, ++sn) {
+        ok = ptx::mbar_wait(&s_full[x], sn & 1, err, kErrSoftmax, kWaitNs);
+        if (!ok) break;
+        __syncwarp();
+        ptx::tc_fence_after();
+        uint32_t s[4][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(ts + c * 32, s[c]);
+        for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(ts + c * 32, s[c]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) ptx::tmem_wait_regs(s[c]);
-      if (it.kb + j >= whole) {
-        const int lim = sees - (it.kb + j) * kTile;
+        for (int c = 0; c < 4; ++c) ptx::tmem_wait_regs(s[c]);
+        if (j >= whole) {
+          const int lim = sees - (it.kb + j) * kTile;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c * 32 + i >= lim) s[c][i] = 0xff800000u;
-      }
-      float mx[4];
+            for (int e = 0; e < 32; ++e)
+              if (c * 32 + e >= lim) s[c][e] = 0xff800000u;
+        }
+        float mx[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        mx[c] = __uint_as_float(s[c][0]);
+        for (int c = 0; c < 4; ++c) mx[c] = fmaxf(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
 #pragma unroll
-        for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][i]));
-      }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-      if (__any_sync(0xffffffffu, top > m + kRescaleLog2)) {
-        const float mn = fmaxf(m, top);
-        const float f = m == mn ? 1.f : ex2(m - mn);
-        m = mn;
-        l *= f;
-        if (j > 0) {
+        for (int e = 2; e < 32; e += 2)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mx[c] = max3(mx[c], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+        const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * p.scale_log2;
+        if (__any_sync(0xffffffffu, top > m + kRescaleLog2)) {
+          const float mn = fmaxf(m, top);
+          const float f = m == mn ? 1.f : ex2(m - mn);
+          m = mn;
+          l *= f;
+          if (j > 0) {  // the product that wrote O is complete: S of this tile came after it
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            ptx::tmem_ld_32x32b_x32(to + c * 32, o);
-            ptx::tmem_wait_regs(o);
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              ptx::tmem_ld_32x32b_x32(to + c * 32, o);
+              ptx::tmem_wait_regs(o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            ptx::tmem_st_32x32b_x32(to + c * 32, o);
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              ptx::tmem_st_32x32b_x32(to + c * 32, o);
+            }
           }
         }
-      }
-      const float mm = m == -INFINITY ? 0.f : m;  // nothing seen yet: every weight is zero
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const float mm = m == -INFINITY ? 0.f : -m;  // nothing seen yet: every weight is zero
+        const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), m2 = make_float2(mm, mm);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t w[32];
+        for (int c = 0; c < 2; ++c) {
+          uint32_t w[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int cc = 2 * c + i / 16, ii = i % 16 * 2;
-          const float a = ex2(fmaf(__uint_as_float(s[cc][ii]), p.scale_log2, -mm));
-          const float b = ex2(fmaf(__uint_as_float(s[cc][ii + 1]), p.scale_log2, -mm));
-          sum[(i & 1) * 2] += a;
-          sum[(i & 1) * 2 + 1] += b;
-          w[i] = pack_bf16x2(a, b);
+          for (int q = 0; q < 32; ++q) {
+            const int cc = 2 * c + q / 16, ii = q % 16 * 2;
+            float2 e = fma2(make_float2(__uint_as_float(s[cc][ii]), __uint_as_float(s[cc][ii + 1])), scale2, m2);
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            sum[q & 1] = add2(sum[q & 1], e);
+            w[q] = pack_bf16x2(e.x, e.y);
+          }
+          ptx::tmem_st_32x32b_x32(ts + c * 32, w);
+          // the product of the first half of the keys starts while the second half is in work
+          ptx::tmem_wait_st();
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(c == 0 ? &p_half[x] : &p_full[x]);
         }
-        ptx::tmem_st_32x32b_x32(ts + c * 32, w);
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      ptx::tmem_wait_st();
-      ptx::tc_fence_before();
-      ptx::mbar_arrive(&p_full[x]);
-    }
-    // ---- epilogue: this thread's row
-    if (n > 0 && ok) {
-      ok = ptx::mbar_wait(&o_full[x], 0, err, kErrSoftmax, kWaitNs);
-      ptx::tc_fence_after();
-    }
-    const int64_t grow = tab.q_start[it.seq] + it.t0[x] + token;
-    const int head = it.head * p.group + r % p.group;
-    const bool fix = ok && n > 0 && *reinterpret_cast<volatile int*>(&bad);
-    const float inv = p.splits > 1 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
-    const int64_t rec = (grow * p.hq + head) * p.splits + it.split;
-    if (real && p.splits > 1) {
-      float* ml = p.part + p.part_rows * D + rec * 2;
-      ml[0] = n > 0 ? m : -INFINITY;
-      ml[1] = l;
-    }
-#pragma unroll 1
-    for (int c = 0; c < D / 32; ++c) {
-      uint32_t o[32];
+      if (!ok) break;
+      uint32_t o[D / 32][32];
+      bool fix = false;
       if (n > 0) {
-        ptx::tmem_ld_32x32b_x32(to + c * 32, o);
-        ptx::tmem_wait_regs(o);
+        ok = ptx::mbar_wait(&o_full[x], on & 1, err, kErrSoftmax, kWaitNs);
+        if (!ok) break;
+        ++on;
+        __syncwarp();
+        ptx::tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) ptx::tmem_ld_32x32b_x32(to + c * 32, o[c]);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) ptx::tmem_wait_regs(o[c]);
+        fix = *reinterpret_cast<volatile int*>(&bad[busy & 7]) == busy + 1;
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&o_empty[x]);
       } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = 0u;
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[c][e] = 0u;
       }
-      if (!real || !ok) continue;
+      if (it.nk > 0) ++busy;
+      if (!real) continue;
+      const int64_t grow = static_cast<int64_t>(tab.q_start[it.seq]) + it.t0[x] + token;
+      const int head = it.head * p.group + head_in;
       if (fix) {
         // non-finite values of V that this row does see
-        for (int key = max(it.kb, it.clean) * kTile; key < min(sees, it.ke[x] * kTile); ++key) {
-          const __nv_bfloat16* vr = p.v + (tab.k_start[it.seq] + static_cast<int64_t>(key)) * p.v_stride + it.head * D + c * 32;
+        for (int key = (it.kb + it.clean) * kTile; key < min(sees, (it.kb + n) * kTile); ++key) {
+          const __nv_bfloat16* vr = p.v + (tab.k_start[it.seq] + static_cast<int64_t>(key)) * p.v_stride + it.head * D;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float f = __bfloat162float(vr[i]);
-            if (!isfinite(f)) o[i] = __float_as_uint(__uint_as_float(o[i]) + f);
-          }
+          for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float f = __bfloat162float(vr[c * 32 + e]);
+              if (!isfinite(f)) o[c][e] = __float_as_uint(__uint_as_float(o[c][e]) + f);
+            }
         }
       }
       if (p.splits > 1) {
-        float4* dst = reinterpret_cast<float4*>(p.part + rec * D + c * 32);
+        const int64_t rec = (grow * p.hq + head) * p.splits + it.split;
+        float* ml = p.part + p.part_rows * D + rec * 2;
+        ml[0] = n > 0 ? m : -INFINITY;
+        ml[1] = l;
+        float4* dst = reinterpret_cast<float4*>(p.part + rec * D);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
-                               __uint_as_float(o[4 * i + 3]));
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            dst[c * 8 + e] = make_float4(__uint_as_float(o[c][4 * e]), __uint_as_float(o[c][4 * e + 1]),
+                                         __uint_as_float(o[c][4 * e + 2]), __uint_as_float(o[c][4 * e + 3]));
       } else {
-        uint4* dst = reinterpret_cast<uint4*>(p.out + grow * p.out_stride + head * D + c * 32);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint4* dst = reinterpret_cast<uint4*>(p.out + grow * p.out_stride + head * D);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t w[4];
+        for (int c = 0; c < D / 32; ++c)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = pack_bf16x2(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-          dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+          for (int e = 0; e < 4; ++e) {
+            uint32_t w[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              w[q] = pack_bf16x2(__uint_as_float(o[c][8 * e + 2 * q]) * inv, __uint_as_float(o[c][8 * e + 2 * q + 1]) * inv);
+            dst[c * 4 + e] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
       }
     }
     ptx::tc_fence_before();
@@ -525,7 +654,9 @@ int launch_prompt(const Plan& pl, const PromptParams& p, const CUtensorMap& qm, 
     SWL_CUDA_TRY(cudaFuncSetAttribute(prompt_attention_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem));
     done.fetch_or(bit);
   }
-  SWL_CUDA_TRY(launch_kernel(prompt_attention_kernel<D>, dim3(static_cast<unsigned>(pl.items) * p.hkv * p.splits), dim3(320),
+  int sms = 0;
+  SWL_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  SWL_CUDA_TRY(launch_kernel(prompt_attention_kernel<D>, dim3(std::min(p.items, sms)), dim3(kThreads),
                              Cfg<D>::kSmem, st, 1, pl.t, p, qm, km, vm));
   if (p.splits > 1)
     SWL_CUDA_TRY(launch_kernel(prompt_combine_kernel<D>, dim3(static_cast<unsigned>(pl.total_q), p.hq), dim3(D), 0, st, 1, p));
@@ -574,6 +705,7 @@ SWL_EXPORT int swl_prompt_attention(int nseg, const int* q_lens, const int* k_le
   p.tokens = kTile / p.group;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.splits = pl.splits;
+  p.items = pl.items * hkv * pl.splits;
   p.part = part;
   p.part_rows = pl.total_q * hq * pl.splits;
   // without any key the maps of K and V are never used: they describe q's row instead
