@@ -79,7 +79,8 @@ struct Cfg {
   static constexpr int kHalves = D / 64;
   static constexpr int kStages = D == 128 ? 2 : 4;  // tiles of K, and of V
   static constexpr int kTileBytes = kTile * D * 2;
-  static constexpr int kSmem = (2 + 2 * kStages) * kTileBytes + 1024;
+  static constexpr int kOutBytes = 8 * 32 * 64;     // epilogue: 32 rows x 64 B for each softmax warp
+  static constexpr int kSmem = (2 + 2 * kStages) * kTileBytes + kOutBytes + 1024;
   static constexpr uint32_t kS = 0, kO = 2 * kTile, kCols = 512;  // tensor memory columns
 };
 
@@ -176,7 +177,7 @@ struct Rounds {
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
-    prompt_attention_kernel(const __grid_constant__ PromptTable tab, const __grid_constant__ PromptParams p,
+    prompt_attention_kernel(const __grid_constant__ PromptTable table, const __grid_constant__ PromptParams p,
                             const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                             const __grid_constant__ CUtensorMap vmap) {
   using C = Cfg<D>;
@@ -186,6 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* const q_sm = dyn;
   uint8_t* const k_ring = dyn + 2 * C::kTileBytes;
   uint8_t* const v_ring = k_ring + ST * C::kTileBytes;
+  uint8_t* const out_sm = v_ring + ST * C::kTileBytes;
   // Who completes each barrier: *_full the copy or product that fills, *_empty who has used it.
   __shared__ __align__(8) uint64_t q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2];
   __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], seen[2], turn[2], drained[2];
@@ -193,6 +195,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   // [n & 7] == n + 1: a non-finite value of its sequence was taken out of a V tile of the
   // CTA's n-th item with keys (copies run at most 4 items ahead of the rows, so n's are done when n + 8 comes)
   __shared__ int bad[8];
+  // the launch's table: reading it from the parameter space costs a miss an entry, for every item anew
+  __shared__ PromptTable tab;
   unsigned int* const err = &g_prompt_error_word;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -219,6 +223,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 8; ++i) bad[i] = 0;
     ptx::fence_mbar_init();
   }
+  for (int i = threadIdx.x; i < table.nseq; i += kThreads) {
+    tab.q_start[i] = table.q_start[i];
+    tab.q_len[i] = table.q_len[i];
+    tab.k_start[i] = table.k_start[i];
+    tab.k_len[i] = table.k_len[i];
+    tab.item_start[i + 1] = table.item_start[i + 1];
+  }
+  if (threadIdx.x == 0) {
+    tab.nseq = table.nseq;
+    tab.item_start[0] = 0;
+  }
   if (warp == 9) ptx::tmem_alloc(&tmem_base, C::kCols);
   if (warp == 8 && lane == 0) {
     ptx::prefetch_tmap(&qmap);
@@ -243,8 +258,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---- copies
       if (lane == 0) {
         uint32_t qn[2] = {0, 0}, issued = 0;  // copies of each row tile, and of K and V tiles
-        while (ok && rounds.next(p.items, &i)) {
-          const Item it = find_item(tab, p, i);
+        bool have = rounds.next(p.items, &i);
+        Item it;
+        if (have) it = find_item(tab, p, i);
+        while (ok && have) {
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             if (!ok || it.n[x] == 0) continue;
@@ -255,6 +272,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int h = 0; h < C::kHalves; ++h)
               ptx::tma_load_3d(ptx::smem_addr(q_sm + x * C::kTileBytes + h * kTile * 128), &qmap, &q_full[x], h * 64,
                                it.head * p.group, tab.q_start[it.seq] + it.t0[x]);
+          }
+          // the next item's rows of Q come from memory: they are asked for an item ahead
+          have = rounds.next(p.items, &i);
+          Item next = it;
+          if (have) {
+            next = find_item(tab, p, i);
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              if (next.n[x] > 0)
+                for (int h = 0; h < C::kHalves; ++h)
+                  ptx::tma_prefetch_3d(&qmap, h * 64, next.head * p.group, tab.q_start[next.seq] + next.t0[x]);
           }
           const int row0 = tab.k_start[it.seq] + it.kb * kTile;
           for (int j = 0; j < it.nk && ok; ++j, ++tiles) {
@@ -272,6 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               ++issued;
             }
           }
+          it = next;
         }
         if (!ok) {  // a wait gave up: the copies that were issued land before the CTA ends
           for (uint32_t n = issued > 2 * ST ? issued - 2 * ST : 0; n < issued; ++n)
@@ -301,23 +330,26 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint4 u[8];
 #pragma unroll
             for (int q = 0; q < 8; ++q) u[q] = v[b + 32 * q];
-            uint32_t odd = 0;  // bit q: u[q] holds a non-finite value
+            __nv_bfloat162 a[8];  // sums of 0 x: NaN where an x is not finite
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
               const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u[q]);
-              __nv_bfloat162 a = zero;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) a = __hfma2(h[e], zero, a);  // NaN where a factor is not finite
-              if (!(__low2float(a) == 0.f) || !(__high2float(a) == 0.f)) odd |= 1u << q;
+              a[q] = __hfma2(h[3], zero, __hfma2(h[2], zero, __hfma2(h[1], zero, __hmul2(h[0], zero))));
             }
-            if (odd) {
+#pragma unroll
+            for (int w = 4; w; w >>= 1)
+#pragma unroll
+              for (int q = 0; q < w; ++q) a[q] = __hadd2(a[q], a[q + w]);
+            if (!(__low2float(a[0]) == 0.f && __high2float(a[0]) == 0.f)) {
 #pragma unroll 1
               for (int q = 0; q < 8; ++q) {
-                if (!(odd >> q & 1u)) continue;
                 __nv_bfloat16* w = reinterpret_cast<__nv_bfloat16*>(v + b + 32 * q);
+#pragma unroll 1
                 for (int e = 0; e < 8; ++e)
-                  if (!isfinite(__bfloat162float(w[e]))) w[e] = __float2bfloat16_rn(0.f);
-                if ((it.kb + j) * kTile + (b + 32 * q) / 8 % kTile < klen) bad[busy & 7] = busy + 1;
+                  if (!isfinite(__bfloat162float(w[e]))) {
+                    w[e] = __float2bfloat16_rn(0.f);
+                    if ((it.kb + j) * kTile + (b + 32 * q) / 8 % kTile < klen) bad[busy & 7] = busy + 1;
+                  }
               }
             }
           }
@@ -343,10 +375,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t kd = ptx::sw128_kmajor_desc(ptx::smem_addr(k_ring));
       const uint64_t vd = ptx::sw128_mnmajor_desc(ptx::smem_addr(v_ring), kTile * 128);
       uint32_t qn = 0, pn = 0, looked = 0;  // items and key tiles of this row tile; V tiles looked over
-      auto scores = [&](uint32_t tile) {    // S = Q K^T
+      // S = Q K^T; the other warp's turn (hand) comes two products before the end, so that its
+      // wake-up passes while they run
+      auto scores = [&](uint32_t tile, bool hand) {
         const uint64_t k = kd + (tile % ST) * (C::kTileBytes >> 4);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
+          if (kk == D / 16 - 2 && hand) ptx::mbar_arrive(&turn[x ^ 1]);
           const uint32_t o = ((kk >> 2) * kTile * 128 + (kk & 3) * 32) >> 4;
           ptx::mma_bf16_ss(ts, qd + o, k + o, idesc_s, kk > 0 ? 1u : 0u);
         }
@@ -362,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = ptx::mbar_wait(&q_full[x], qn & 1, err, kErrMma, kWaitNs);
           if (!ok) break;
           ptx::tc_fence_after();
-          scores(tiles);
+          scores(tiles, false);
           if (n == 1) ptx::tc_commit(&q_empty[x]);
         } else if (ok) {
           ptx::mbar_arrive(&k_empty[tiles % ST]);
@@ -383,33 +418,35 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           // the two warps issue a step in turn: 0, 1, 0, 1, ..., so the row tiles stay half a step apart
           // (in step, both would wait for their exponentials at once and leave the tensor cores idle)
+          const bool both = ok && j < n && ptx::mbar_test(&p_full[x], pn & 1);
           if (ok && (x == 1 || tiles > 0)) ok = ptx::mbar_wait(&turn[x], (x == 1 ? tiles : tiles - 1) & 1, err, kErrMma, kWaitNs);
           if (!ok) break;
           if (j < n) {
             const uint64_t v = vd + s * (C::kTileBytes >> 4);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              if (half) ok = ptx::mbar_wait(&p_full[x], pn & 1, err, kErrMma, kWaitNs);
+              if (half && !both) ok = ptx::mbar_wait(&p_full[x], pn & 1, err, kErrMma, kWaitNs);
               if (!ok) break;
-              ptx::tc_fence_after();
+              if (!half || !both) ptx::tc_fence_after();
 #pragma unroll
               for (int kk = half * 4; kk < half * 4 + 4; ++kk)
                 ptx::mma_bf16_ts(to, ts + kk * 8, v + kk * (16 * 128 >> 4), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
             }
             if (!ok) break;
             ++pn;
-            ptx::tc_commit(&v_empty[s]);
+            // the score product follows at once; what only frees memory is announced after it
             if (j + 1 == n) {
               ptx::tc_commit(&o_full[x]);
             } else {
-              scores(tiles + 1);
+              scores(tiles + 1, true);
               if (j + 2 == n) ptx::tc_commit(&q_empty[x]);
             }
+            ptx::tc_commit(&v_empty[s]);
           } else {
             ptx::mbar_arrive(&v_empty[s]);
           }
           if (j + 1 >= n && j + 1 < it.nk) ptx::mbar_arrive(&k_empty[(tiles + 1) % ST]);
-          ptx::mbar_arrive(&turn[x ^ 1]);
+          if (j + 1 >= n) ptx::mbar_arrive(&turn[x ^ 1]);
         }
         if (n > 0) ++qn;
       }
@@ -427,6 +464,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + C::kS + x * kTile, to = tmem + lanes + C::kO + x * D;
     const int token = r / p.group, head_in = r % p.group;
+    uint8_t* const stage = out_sm + warp * 32 * 64;
+    // the rows that this thread writes 16 bytes of a pass: 8 q + lane / 4 of its warp
+    int w_token[4];
+    int64_t w_off[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int row = (warp & 3) * 32 + 8 * q + (lane >> 2);
+      w_token[q] = row / p.group;
+      w_off[q] = w_token[q] * p.out_stride + row % p.group * D + (lane & 3) * 8;
+    }
     Rounds rounds;
     int i, busy = 0;
     uint32_t sn = 0, on = 0;  // key tiles and items of this row tile so far
@@ -452,9 +499,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int lim = sees - (it.kb + j) * kTile;
 #pragma unroll
           for (int c = 0; c < 4; ++c)
+            if (__any_sync(0xffffffffu, lim < c * 32 + 32)) {  // columns 32 c .. that some row does not see
+              const int n_c = lim - c * 32;
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (c * 32 + e >= lim) s[c][e] = 0xff800000u;
+              for (int e = 0; e < 32; ++e)
+                if (e >= n_c) s[c][e] = 0xff800000u;
+            }
         }
         float mx[4];
 #pragma unroll
@@ -529,10 +579,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int e = 0; e < 32; ++e) o[c][e] = 0u;
       }
       if (it.nk > 0) ++busy;
-      if (!real) continue;
       const int64_t grow = static_cast<int64_t>(tab.q_start[it.seq]) + it.t0[x] + token;
       const int head = it.head * p.group + head_in;
-      if (fix) {
+      if (fix && real) {
         // non-finite values of V that this row does see
         for (int key = (it.kb + it.clean) * kTile; key < min(sees, (it.kb + n) * kTile); ++key) {
           const __nv_bfloat16* vr = p.v + (tab.k_start[it.seq] + static_cast<int64_t>(key)) * p.v_stride + it.head * D;
@@ -546,6 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (p.splits > 1) {
+        if (!real) continue;
         const int64_t rec = (grow * p.hq + head) * p.splits + it.split;
         float* ml = p.part + p.part_rows * D + rec * 2;
         ml[0] = n > 0 ? m : -INFINITY;
@@ -559,17 +609,29 @@ __global__ void __launch_bounds__(kThreads, 1)
                                          __uint_as_float(o[c][4 * e + 2]), __uint_as_float(o[c][4 * e + 3]));
       } else {
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        uint4* dst = reinterpret_cast<uint4*>(p.out + grow * p.out_stride + head * D);
+        // through shared memory, 32 dimensions a pass: a row straight from its thread would
+        // touch 32 lines with every store (4096 line accesses an item, now 1024)
+        __nv_bfloat16* const dst =
+            p.out + (static_cast<int64_t>(tab.q_start[it.seq]) + it.t0[x]) * p.out_stride + it.head * p.group * D;
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c)
+        for (int c = 0; c < D / 32; ++c) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             uint32_t w[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q)
               w[q] = pack_bf16x2(__uint_as_float(o[c][8 * e + 2 * q]) * inv, __uint_as_float(o[c][8 * e + 2 * q + 1]) * inv);
-            dst[c * 4 + e] = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((e ^ (lane >> 1 & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
           }
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int row = 8 * q + (lane >> 2);
+            const uint4 w = *reinterpret_cast<const uint4*>(stage + row * 64 + (((lane & 3) ^ (row >> 1 & 3)) << 4));
+            if (w_token[q] < it.nt[x]) *reinterpret_cast<uint4*>(dst + w_off[q] + c * 32) = w;
+          }
+          __syncwarp();
+        }
       }
     }
     ptx::tc_fence_before();
