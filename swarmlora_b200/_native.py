@@ -133,17 +133,16 @@ SIGNATURES: dict[str, tuple] = {
     "swl_paged_attention_noalloc": (_i32, [_i32, _pi32, _pp, _pp, _pp, _pp, _pp, _i64, _i32, _i32,
                                            _i32, _i32, _f32, _i32, _p, _p]),
     "swl_noalloc_forget_device": (_i32, []),
-    "swl_prompt_attention_part_floats": (_i64, [_i32, _pi32, _pi32, _i32, _i32, _i32]),
-    "swl_prompt_attention": (_i32, [_i32, _pi32, _pi32, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _i32, _i32, _f32,
-                                    _p, _p]),
+    # (host arrays by address: callers pass ctypes arrays or array.array buffers)
+    "swl_prompt_attention_part_floats": (_i64, [_i32, _p, _p, _i32, _i32, _i32]),
+    "swl_prompt_attention": (_i32, [_i32, _p, _p, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _i32, _i32, _f32, _p, _p]),
     "swl_attention_device_error": (_i32, [_pu32]),
     "swl_kv4_block_bytes": (_i64, [_i32]),
-    "swl_kv4_append": (_i32, [_i32, _pi32, _pp, _i64, _pp, _i32, _pp, _i64, _pp, _i32, _i32, _i32, _i32, _p, _i32, _p,
-                              _p, _p]),
-    "swl_kv4_gather": (_i32, [_i32, _pi32, _pi32, _pp, _i32, _pp, _i64, _i32, _i32, _i32, _p, _p, _p]),
-    "swl_kv4_part_floats": (_i64, [_i32, _pi32, _i32, _i32, _i32, _i32]),
-    "swl_paged_attention_kv4": (_i32, [_i32, _pi32, _pp, _i32, _pp, _i64, _pp, _pp, _i64, _i32, _i32, _i32, _i32, _f32,
-                                       _i32, _p, _p, _p]),
+    "swl_kv4_append": (_i32, [_i32, _p, _p, _i64, _p, _i32, _p, _i64, _p, _i32, _i32, _i32, _i32, _p, _i32, _p, _p, _p]),
+    "swl_kv4_gather": (_i32, [_i32, _p, _p, _p, _i32, _p, _i64, _i32, _i32, _i32, _p, _p, _p]),
+    "swl_kv4_part_floats": (_i64, [_i32, _p, _i32, _i32, _i32, _i32]),
+    "swl_paged_attention_kv4": (_i32, [_i32, _p, _p, _i32, _p, _i64, _p, _p, _i64, _i32, _i32, _i32, _i32, _f32, _i32, _p,
+                                       _p, _p]),
     "swl_rms_norm": (_i32, [_i32, _pi32, _pp, _i64, _pp, _i64, _p, _i64, _f32, _p]),
     "swl_copy_rows": (_i32, [_i32, _pp, _pp, _pi64, _p]),
     "swl_paged_attention_shrink": (_i32, [_i32, _pi32, _pp, _pp, _pp, _pp, _pp, _i64, _i32, _i32, _i32,

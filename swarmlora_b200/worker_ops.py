@@ -10,7 +10,10 @@ matrices are pre-scaled by alpha/r in bf16, O / Down scale after the expand
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
+import itertools
+from array import array
 from dataclasses import dataclass
 
 import torch
@@ -203,20 +206,49 @@ NOALLOC_ATTN_SCRATCH_FLOATS = 1 << 20
 
 
 # ---- whole prompts, and the key/value cache held in 4 bits --------------------------------------
-def _bf16_rows(name: str, t: torch.Tensor, heads: int | None, head_dim: int | None, device=None) -> None:
-    """A bf16 CUDA tensor [rows, heads, head_dim] whose heads are contiguous."""
-    if t.dtype != torch.bfloat16 or not t.is_cuda or (device is not None and t.device != device):
+# A decode step makes these calls once a layer with kernels of a few microseconds, so their
+# host side is kept short: tables go through array.array, contexts are entered only where needed.
+def _elsewhere(device: torch.device, stream) -> bool:
+    """Whether a call has to switch to its tensors' device or to a stream of its own."""
+    return stream is not None or device.index != torch.cuda.current_device()
+
+
+def _there(device: torch.device, stream):
+    if device.type != "cuda":
+        raise ValueError("CUDA tensors are needed")
+    ctx = contextlib.ExitStack()
+    ctx.enter_context(torch.cuda.device(device))
+    ctx.enter_context(torch.cuda.stream(stream))
+    return ctx
+
+
+def _ints(values) -> array:
+    return array("i", values)
+
+
+def _addr(table: array) -> int:
+    return table.buffer_info()[0]
+
+
+def _bf16_rows(name: str, t: torch.Tensor, device, heads=None, head_dim=None) -> None:
+    """A bf16 tensor [rows, heads, head_dim] on `device` whose heads are contiguous."""
+    if t.dtype is not torch.bfloat16 or t.device != device:
         raise ValueError(f"{name}: a bf16 tensor on the call's CUDA device is needed")
-    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or (head_dim is not None and t.shape[2] != head_dim):
-        raise ValueError(f"{name}: shape {tuple(t.shape)} does not fit")
-    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2])):
-        raise ValueError(f"{name}: heads must be contiguous")
+    shape = t.shape
+    if len(shape) != 3 or (heads is not None and shape[1] != heads) or (head_dim is not None and shape[2] != head_dim):
+        raise ValueError(f"{name}: shape {tuple(shape)} does not fit")
+    st = t.stride()
+    if st[2] != 1 or (shape[1] > 1 and st[1] != shape[2]):
+        if t.numel():
+            raise ValueError(f"{name}: heads must be contiguous")
 
 
 def _row_stride(t: torch.Tensor) -> int:
     """Elements between rows; a single row's stride is never used (torch leaves it arbitrary)."""
-    width = t.shape[-1] * (t.shape[-2] if t.dim() == 3 else 1)
-    return int(t.stride(0)) if t.shape[0] > 1 else -(-width // 8) * 8
+    shape = t.shape
+    if shape[0] > 1:
+        return t.stride(0)
+    return -(-shape[-1] * (shape[-2] if len(shape) == 3 else 1) // 8) * 8
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_lens, k_lens=None, scale: float | None = None,
@@ -226,33 +258,37 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_lens, 
     r of a sequence sees its keys 0 .. r + k_len - q_len (k_lens defaults to
     q_lens; longer ones hold a prefix); a row without keys gives zeros.
     Returns out [rows of q, hq, D] (rows behind the last sequence are left as they are)."""
-    _bf16_rows("q", q, None, None)
-    hq, D = int(q.shape[1]), int(q.shape[2])
-    _bf16_rows("k", k, None, D, q.device)
-    hkv = int(k.shape[1])
-    _bf16_rows("v", v, hkv, D, q.device)
-    q_lens = [int(x) for x in q_lens]
-    k_lens = q_lens if k_lens is None else [int(x) for x in k_lens]
-    if len(k_lens) != len(q_lens):
+    dev = q.device
+    if dev.type != "cuda" or _elsewhere(dev, stream):
+        with _there(dev, stream):
+            return prompt_attention(q, k, v, q_lens, k_lens, scale, out)
+    _bf16_rows("q", q, dev)
+    hq, D = q.shape[1], q.shape[2]
+    _bf16_rows("k", k, dev, None, D)
+    hkv = k.shape[1]
+    _bf16_rows("v", v, dev, hkv, D)
+    if k_lens is None:
+        k_lens = q_lens
+    n, total = len(q_lens), sum(q_lens)
+    if len(k_lens) != n:
         raise ValueError("prompt_attention: one key length per sequence")
-    if sum(q_lens) > q.shape[0] or sum(k_lens) > min(k.shape[0], v.shape[0]):
+    if total > q.shape[0] or sum(k_lens) > min(k.shape[0], v.shape[0]):
         raise ValueError("prompt_attention: the lengths add up to more rows than there are")
-    n, ql, kl = len(q_lens), i32_array(q_lens), i32_array(k_lens)
-    with torch.cuda.device(q.device):
-        s = stream if stream is not None else torch.cuda.current_stream()
-        with torch.cuda.stream(s):  # the scratch belongs to the stream that uses it
-            if out is None:
-                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            else:
-                _bf16_rows("out", out, hq, D, q.device)
-                if sum(q_lens) > out.shape[0]:
-                    raise ValueError("prompt_attention: out has fewer rows than q_lens")
-            need = int(lib().swl_prompt_attention_part_floats(n, ql, kl, hq, hkv, D))
-            part = torch.empty(need, dtype=torch.float32, device=q.device) if need > 0 else None
-            check(lib().swl_prompt_attention(n, ql, kl, q.data_ptr(), _row_stride(q), k.data_ptr(), _row_stride(k),
-                                             v.data_ptr(), _row_stride(v), out.data_ptr(), _row_stride(out), hq, hkv, D,
-                                             float(scale) if scale is not None else D ** -0.5,
-                                             part.data_ptr() if part is not None else None, s.cuda_stream))
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    else:
+        _bf16_rows("out", out, dev, hq, D)
+        if total > out.shape[0]:
+            raise ValueError("prompt_attention: out has fewer rows than q_lens")
+    ql, kl = _ints(q_lens), _ints(k_lens)
+    pq, pk = _addr(ql), _addr(kl)
+    L = lib()
+    need = L.swl_prompt_attention_part_floats(n, pq, pk, hq, hkv, D)
+    part = torch.empty(need, dtype=torch.float32, device=dev) if need > 0 else None
+    check(L.swl_prompt_attention(n, pq, pk, q.data_ptr(), _row_stride(q), k.data_ptr(), _row_stride(k), v.data_ptr(),
+                                 _row_stride(v), out.data_ptr(), _row_stride(out), hq, hkv, D,
+                                 float(scale) if scale is not None else D ** -0.5,
+                                 part.data_ptr() if part is not None else None, torch.cuda.current_stream().cuda_stream))
     return out
 
 
@@ -272,55 +308,67 @@ def kv4_cache(num_pages: int, hkv: int, head_dim: int = 128, page: int = 16, dev
                        device=device if device is not None else "cuda")
 
 
-def _rows_of(ts, n: int, what: str, dtype, device, step=None) -> list:
+def _slot_rows(ts, n: int, what: str, dtype, device, first=None) -> array:
     """Addresses of each slot's rows: a list of tensors, or one tensor with a
-    row per slot (step: the first row of each slot)."""
+    row per slot (first: the first row of each slot)."""
     if isinstance(ts, torch.Tensor):
-        if ts.dtype != dtype or ts.device != device:
+        if ts.dtype is not dtype or ts.device != device:
             raise ValueError(f"{what}: {dtype} on {device} is needed")
-        if (ts.dim() > 1 and ts.stride(-1) != 1) or (step is None and ts.shape[0] != n):
+        if (ts.dim() > 1 and ts.stride(-1) != 1) or (first is None and ts.shape[0] != n):
             raise ValueError(f"{what}: one row per slot, contiguous inside")
-        base, by = ts.data_ptr(), ts.element_size() * int(ts.stride(0))
-        return [base + i * by for i in (step if step is not None else range(n))]
-    if len(ts) != n or any(t.dtype != dtype or t.device != device or (t.dim() and t.numel() > 1 and t.stride(-1) != 1)
-                           for t in ts):
+        base, by = ts.data_ptr(), ts.element_size() * ts.stride(0)
+        if first is not None:
+            return array("Q", [base + i * by for i in first])
+        return array("Q", range(base, base + n * by, by)) if by > 0 else array("Q", [base]) * n
+    if len(ts) != n or any(t.dtype is not dtype or t.device != device or
+                           (t.dim() and t.numel() > 1 and t.stride(-1) != 1) for t in ts):
         raise ValueError(f"{what}: one {dtype} tensor per slot on {device}, contiguous inside")
-    return [t.data_ptr() for t in ts]
+    return array("Q", [t.data_ptr() for t in ts])
 
 
 def _kv4_slots(block_tables, caches, n: int, hkv: int, head_dim: int, page: int, device):
     """Block tables, their length, caches and their pages of a call over slots."""
-    block = kv4_block_bytes(head_dim)
     if isinstance(block_tables, torch.Tensor):
         if block_tables.dim() != 2:
             raise ValueError("block tables: [slots, pages] or one tensor per slot")
-        table_len = int(block_tables.shape[1])
+        table_len = block_tables.shape[1]
     else:
-        table_len = min((int(t.shape[0]) for t in block_tables), default=1)
-    tables = _rows_of(block_tables, n, "block tables", torch.int32, device)
-    each = [caches] if isinstance(caches, torch.Tensor) else list(caches)
+        table_len = min((t.shape[0] for t in block_tables), default=1)
+    tables = _slot_rows(block_tables, n, "block tables", torch.int32, device)
+    each = (caches,) if isinstance(caches, torch.Tensor) else caches
+    want = (page // 16, hkv, kv4_block_bytes(head_dim))
     for c in each:
-        if c.dtype != torch.uint8 or c.device != device or not c.is_contiguous() or \
-                tuple(c.shape[1:]) != (page // 16, hkv, block):
-            raise ValueError(f"4-bit cache: contiguous uint8 [pages, {page // 16}, {hkv}, {block}] on {device} is needed")
-    ptrs = [caches.data_ptr()] * n if isinstance(caches, torch.Tensor) else [c.data_ptr() for c in each]
-    if len(ptrs) != n:
+        if c.dtype is not torch.uint8 or c.device != device or not c.is_contiguous() or c.shape[1:] != want:
+            raise ValueError(f"4-bit cache: contiguous uint8 [pages, {want[0]}, {want[1]}, {want[2]}] on {device} is needed")
+    if isinstance(caches, torch.Tensor):
+        return tables, table_len, array("Q", [caches.data_ptr()]) * n, caches.shape[0]
+    if len(each) != n:
         raise ValueError("4-bit cache: one for all slots, or one per slot")
-    return ptr_array(tables), table_len, ptr_array(ptrs), min((int(c.shape[0]) for c in each), default=1)
+    return tables, table_len, array("Q", [c.data_ptr() for c in each]), min((c.shape[0] for c in each), default=1)
 
 
 def _first_rows(rows) -> list:
-    out, at = [], 0
-    for r in rows:
-        out.append(at)
-        at += r
-    return out
+    return [0, *itertools.accumulate(rows)][:len(rows)]
 
 
 def _packed(name: str, t: torch.Tensor, rows: int, width: int, device) -> None:
-    if t.dtype != torch.bfloat16 or t.device != device or not t.is_contiguous() or t.shape[0] < rows or \
+    if t.dtype is not torch.bfloat16 or t.device != device or not t.is_contiguous() or t.shape[0] < rows or \
             t.numel() != t.shape[0] * width:
         raise ValueError(f"{name}: contiguous bf16 with at least {rows} rows of {width} on {device} is needed")
+
+
+def _slots_of_rows(name: str, ts, rows, total: int, width: int) -> int:
+    """Checks rows packed in one tensor or given per slot; returns their stride."""
+    if isinstance(ts, torch.Tensor):
+        if ts.dim() != 2 or ts.shape[1] < width or ts.shape[0] < total:
+            raise ValueError(f"{name}: {tuple(ts.shape)} holds fewer than {total} rows of {width}")
+        return _row_stride(ts)
+    if len(ts) != len(rows) or any(t.dim() != 2 or t.shape[1] < width or t.shape[0] < r for t, r in zip(ts, rows)):
+        raise ValueError(f"{name}: each slot must hold its rows of {width}")
+    strides = {t.stride(0) for t in ts if t.shape[0] > 1}
+    if len(strides) > 1:
+        raise ValueError(f"{name}: the slots' rows must have one stride")
+    return strides.pop() if strides else -(-width // 8) * 8
 
 
 def kv4_append(qkvs, block_tables, caches, seqlens, q_rot, cos_sin, hq: int, hkv: int, head_dim: int = 128,
@@ -328,40 +376,32 @@ def kv4_append(qkvs, block_tables, caches, seqlens, q_rot, cos_sin, hq: int, hkv
     """rope_append into a 4-bit cache: rotates the new rows' q and k (rotated q
     to q_rot [rows, hq * D], k to k_rot [rows, hkv * D] when given) and appends k
     and v quantised. qkvs: one tensor of rows per slot, or all rows packed
-    in one tensor (then `rows` counts them per slot); block_tables: int32, one per slot or [slots, pages];
-    caches: kv4_cache, one or one per slot; seqlens: int32, tokens cached before."""
+    in one tensor (then `rows` counts them per slot); block_tables: int32, one per
+    slot or [slots, pages]; caches: kv4_cache, one or one per slot; seqlens: int32,
+    tokens cached before."""
+    dev = q_rot.device
+    if dev.type != "cuda" or _elsewhere(dev, stream):
+        with _there(dev, stream):
+            return kv4_append(qkvs, block_tables, caches, seqlens, q_rot, cos_sin, hq, hkv, head_dim, page, rows, k_rot)
     packed = isinstance(qkvs, torch.Tensor)
     if rows is None:
         if packed:
             raise ValueError("kv4_append: packed rows need their counts")
-        rows = [int(t.shape[0]) for t in qkvs]
-    rows = [int(r) for r in rows]
-    n, total, dev = len(rows), sum(rows), q_rot.device
-    width = (hq + 2 * hkv) * head_dim
-    if dev.type != "cuda":
-        raise ValueError("kv4_append: CUDA tensors are needed")
-    if packed:
-        if qkvs.dim() != 2 or qkvs.shape[1] < width or qkvs.shape[0] < total:
-            raise ValueError(f"kv4_append: qkv {tuple(qkvs.shape)} holds fewer than {total} rows of {width}")
-        stride = _row_stride(qkvs)
-    else:
-        if any(t.dim() != 2 or t.shape[1] < width or t.shape[0] < r for t, r in zip(qkvs, rows)):
-            raise ValueError(f"kv4_append: each slot's qkv must hold its rows of {width}")
-        strides = {_row_stride(t) for t in qkvs if t.shape[0] > 1} or {-(-width // 8) * 8}
-        if len(strides) > 1:
-            raise ValueError("kv4_append: the slots' rows must have one stride")
-        stride = strides.pop()
+        rows = [t.shape[0] for t in qkvs]
+    n, total = len(rows), sum(rows)
+    stride = _slots_of_rows("kv4_append: qkv", qkvs, rows, total, (hq + 2 * hkv) * head_dim)
     _packed("kv4_append: q_rot", q_rot, total, hq * head_dim, dev)
     if k_rot is not None:
         _packed("kv4_append: k_rot", k_rot, total, hkv * head_dim, dev)
     _packed("kv4_append: cos_sin", cos_sin, 1, head_dim, dev)
-    src = _rows_of(qkvs, n, "kv4_append: qkv", torch.bfloat16, dev, _first_rows(rows) if packed else None)
+    src = _slot_rows(qkvs, n, "kv4_append: qkv", torch.bfloat16, dev, _first_rows(rows) if packed else None)
     tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, dev)
-    lens = _rows_of(seqlens, n, "kv4_append: seqlens", torch.int32, dev)
-    with torch.cuda.device(dev):
-        check(lib().swl_kv4_append(n, i32_array(rows), ptr_array(src), stride, tables, table_len, cache, pages,
-                                   ptr_array(lens), hq, hkv, head_dim, page, cos_sin.data_ptr(), int(cos_sin.shape[0]),
-                                   q_rot.data_ptr(), k_rot.data_ptr() if k_rot is not None else None, _stream(stream)))
+    lens = _slot_rows(seqlens, n, "kv4_append: seqlens", torch.int32, dev)
+    counts = _ints(rows)
+    check(lib().swl_kv4_append(n, _addr(counts), _addr(src), stride, _addr(tables), table_len, _addr(cache), pages,
+                               _addr(lens), hq, hkv, head_dim, page, cos_sin.data_ptr(), cos_sin.shape[0],
+                               q_rot.data_ptr(), k_rot.data_ptr() if k_rot is not None else None,
+                               torch.cuda.current_stream().cuda_stream))
 
 
 def kv4_gather(block_tables, caches, starts, lens, k_out, v_out, hkv: int, head_dim: int = 128, page: int = 16,
@@ -369,20 +409,25 @@ def kv4_gather(block_tables, caches, starts, lens, k_out, v_out, hkv: int, head_
     """Tokens starts[i] .. starts[i] + lens[i] - 1 of each slot's 4-bit cache as
     packed bf16 rows of K and V (k_out, v_out [sum lens, hkv, D]): the keys
     that prompt_attention reads for a chunk behind a cached prefix."""
-    lens = [int(x) for x in lens]
-    n, dev = len(lens), k_out.device
-    if dev.type != "cuda" or len(starts) != n:
-        raise ValueError("kv4_gather: CUDA tensors and one start per slot are needed")
-    for name, t in (("k_out", k_out), ("v_out", v_out)):
-        _packed(f"kv4_gather: {name}", t, sum(lens), hkv * head_dim, dev)
+    dev = k_out.device
+    if dev.type != "cuda" or _elsewhere(dev, stream):
+        with _there(dev, stream):
+            return kv4_gather(block_tables, caches, starts, lens, k_out, v_out, hkv, head_dim, page)
+    n, total = len(lens), sum(lens)
+    if len(starts) != n:
+        raise ValueError("kv4_gather: one start per slot is needed")
+    _packed("kv4_gather: k_out", k_out, total, hkv * head_dim, dev)
+    _packed("kv4_gather: v_out", v_out, total, hkv * head_dim, dev)
     tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, dev)
-    with torch.cuda.device(dev):
-        check(lib().swl_kv4_gather(n, i32_array(starts), i32_array(lens), tables, table_len, cache, pages, hkv, head_dim,
-                                   page, k_out.data_ptr(), v_out.data_ptr(), _stream(stream)))
+    begin, count = _ints(starts), _ints(lens)
+    check(lib().swl_kv4_gather(n, _addr(begin), _addr(count), _addr(tables), table_len, _addr(cache), pages, hkv, head_dim,
+                               page, k_out.data_ptr(), v_out.data_ptr(), torch.cuda.current_stream().cuda_stream))
 
 
 def kv4_part_floats(rows, hq: int, hkv: int, max_len: int, head_dim: int = 128) -> int:
-    return int(lib().swl_kv4_part_floats(len(rows), i32_array(rows), hq, hkv, head_dim, max_len))
+    """fp32 scratch values that paged_attention_kv4 needs for such a call."""
+    counts = _ints(rows)
+    return int(lib().swl_kv4_part_floats(len(rows), _addr(counts), hq, hkv, head_dim, max_len))
 
 
 def paged_attention_kv4(rows, block_tables, caches, seqlens, outs, q_rot, hq: int, hkv: int, max_len: int, scale: float,
@@ -391,36 +436,30 @@ def paged_attention_kv4(rows, block_tables, caches, seqlens, outs, q_rot, hq: in
     appended) at positions seqlens[i] + t. outs: one tensor of rows per slot,
     or all rows packed in one [rows, hq * D]. part: kv4_part_floats fp32 of scratch for
     this call alone (allocated here when None)."""
-    rows = [int(r) for r in rows]
-    n, total, dev = len(rows), sum(rows), q_rot.device
-    if dev.type != "cuda":
-        raise ValueError("paged_attention_kv4: CUDA tensors are needed")
-    _packed("paged_attention_kv4: q_rot", q_rot, total, hq * head_dim, dev)
-    width = hq * head_dim
-    packed = isinstance(outs, torch.Tensor)
-    for t, r in [(outs, total)] if packed else zip(outs, rows):
-        if t.dim() != 2 or t.shape[1] < width or t.shape[0] < r:
-            raise ValueError(f"paged_attention_kv4: an output holds fewer than {r} rows of {width}")
-    strides = {_row_stride(t) for t in ([outs] if packed else outs) if t.shape[0] > 1} or {-(-width // 8) * 8}
-    if len(strides) > 1:
-        raise ValueError("paged_attention_kv4: the slots' rows must have one stride")
-    dst = _rows_of(outs, n, "paged_attention_kv4: out", torch.bfloat16, dev, _first_rows(rows) if packed else None)
+    dev = q_rot.device
+    if dev.type != "cuda" or _elsewhere(dev, stream):
+        with _there(dev, stream):
+            return paged_attention_kv4(rows, block_tables, caches, seqlens, outs, q_rot, hq, hkv, max_len, scale, head_dim,
+                                       page, part)
+    n, total, width = len(rows), sum(rows), hq * head_dim
+    _packed("paged_attention_kv4: q_rot", q_rot, total, width, dev)
+    stride = _slots_of_rows("paged_attention_kv4: out", outs, rows, total, width)
+    first = _first_rows(rows) if isinstance(outs, torch.Tensor) else None
+    dst = _slot_rows(outs, n, "paged_attention_kv4: out", torch.bfloat16, dev, first)
     tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, dev)
-    lens = _rows_of(seqlens, n, "paged_attention_kv4: seqlens", torch.int32, dev)
-    c_rows = i32_array(rows)
-    need = int(lib().swl_kv4_part_floats(n, c_rows, hq, hkv, head_dim, max_len))
-    with torch.cuda.device(dev):
-        s = stream if stream is not None else torch.cuda.current_stream()
-        if part is None and need > 0:
-            with torch.cuda.stream(s):  # the scratch belongs to the stream that uses it
-                part = torch.empty(need, dtype=torch.float32, device=dev)
-        elif part is not None and (part.dtype != torch.float32 or part.device != dev or not part.is_contiguous() or
-                                   part.numel() < need):
-            raise ValueError(f"paged_attention_kv4: part needs {need} contiguous fp32 values on {dev}")
-        check(lib().swl_paged_attention_kv4(n, c_rows, tables, table_len, cache, pages, ptr_array(lens), ptr_array(dst),
-                                            strides.pop(), hq, hkv, head_dim, page, float(scale), max_len,
-                                            q_rot.data_ptr(), part.data_ptr() if part is not None else None,
-                                            s.cuda_stream))
+    lens = _slot_rows(seqlens, n, "paged_attention_kv4: seqlens", torch.int32, dev)
+    counts = _ints(rows)
+    L = lib()
+    need = L.swl_kv4_part_floats(n, _addr(counts), hq, hkv, head_dim, max_len)
+    if part is None:
+        if need > 0:
+            part = torch.empty(need, dtype=torch.float32, device=dev)
+    elif part.dtype is not torch.float32 or part.device != dev or not part.is_contiguous() or part.numel() < need:
+        raise ValueError(f"paged_attention_kv4: part needs {need} contiguous fp32 values on {dev}")
+    check(L.swl_paged_attention_kv4(n, _addr(counts), _addr(tables), table_len, _addr(cache), pages, _addr(lens),
+                                    _addr(dst), stride, hq, hkv, head_dim, page, float(scale), max_len, q_rot.data_ptr(),
+                                    part.data_ptr() if part is not None else None,
+                                    torch.cuda.current_stream().cuda_stream))
 
 
 def rms_norm(xs, outs, w: torch.Tensor, eps: float, rows=None, x_stride: int | None = None,
