@@ -31,6 +31,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "common.h"
 #include "kv4.cuh"
@@ -56,7 +57,7 @@ struct AttnTable4 {
 struct AttnParams4 {
   int hq, group;           // query heads, query heads per kv head
   int64_t out_stride;
-  float scale_log2;
+  float scale_log2, inv_scale;
   int max_len;
   const __nv_bfloat16* q;  // [total_rows, hq * D]
   int whole;               // 1: CTAs take whole pairs; 0: equal ranges
@@ -85,6 +86,13 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_c(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                           uint32_t b1, float c0, float c1) {  // C: (c0, c1) in both halves of the rows
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 // Two nibbles (bits 0-3 of each half) as bf16 128 + v.
 __device__ __forceinline__ uint32_t codes2(uint32_t w) {
@@ -257,9 +265,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
   Piece lp;
   bool more = lw.next(sh, nseg, &lp);
   int lb = more ? lp.b0 + warp : 0;       // next block of the load piece that is not in the batch
-  const uint8_t* addr = nullptr;          // lane i: the batch's i-th block (nullptr: no such page)
+  const uint8_t* addr = nullptr;          // lane i: the batch's i-th block (nullptr: no such page), which it fetches
   int batch = 0, taken = 0, issued = 0;
-  uint32_t ring_ok = 0;                   // bit per stage: the block exists
+  uint32_t batch_ok = 0, ring_ok = 0;     // bit per batch entry and per stage: the block exists
   auto issue = [&]() {
     while (more && taken == batch) {      // the next up to 32 blocks of this warp
       const int left = lp.b1 > lb ? (lp.b1 - lb + kWarps - 1) / kWarps : 0;
@@ -271,17 +279,19 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
       batch = min(left, 32);
       taken = 0;
       addr = lane < batch ? block_of<D>(tab.c, lp.slot, lb + lane * kWarps, lp.head) : nullptr;
+      batch_ok = __ballot_sync(0xffffffffu, addr != nullptr);
       lb += batch * kWarps;
     }
     if (!more) return;
-    const uint64_t a = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(addr), taken);
     const int st = issued % ST;
-    ring_ok = a ? ring_ok | 1u << st : ring_ok & ~(1u << st);
-    if (lane == 0 && a) {
-      ptx::mbar_arrive_expect_tx(&bars[warp][st], C::kBlock);
-      ptx::bulk_load(ring + st * C::kBlock, reinterpret_cast<const void*>(a), C::kBlock, &bars[warp][st]);
-    } else if (lane == 0) {
-      ptx::mbar_arrive(&bars[warp][st]);
+    ring_ok = (ring_ok & ~(1u << st)) | (batch_ok >> taken & 1u) << st;
+    if (lane == taken) {
+      if (addr) {
+        ptx::mbar_arrive_expect_tx(&bars[warp][st], C::kBlock);
+        ptx::bulk_load(ring + st * C::kBlock, addr, C::kBlock, &bars[warp][st]);
+      } else {
+        ptx::mbar_arrive(&bars[warp][st]);
+      }
     }
     ++taken;
     ++issued;
@@ -299,7 +309,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
     const int64_t len0 = *tab.c.seqlen[x.slot];
     // ---- this piece's query columns: B fragments, sums per group, visible lengths ----
     uint32_t qb[NT][2 * W][2];
-    float qs[NT][NG][2];
+    float qs[NT][NG][2], qo[NT][NG][2];  // sum q, and -128 sum q
     int seen[NT][2], seen_g[NT];  // tokens that columns 2c, 2c + 1 and column g see
     int all_see = 0x7fffffff;     // tokens that every column sees
     auto sees = [&](int col) {
@@ -332,13 +342,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
         part[i] += __shfl_xor_sync(0xffffffffu, part[i], 2);
         qs[nt][i][0] = __shfl_sync(0xffffffffu, part[i], 8 * c);
         qs[nt][i][1] = __shfl_sync(0xffffffffu, part[i], 8 * c + 4);
+        qo[nt][i][0] = -128.f * qs[nt][i][0];
+        qo[nt][i][1] = -128.f * qs[nt][i][1];
       }
       seen[nt][0] = sees(col0 + nt * 8 + 2 * c);
       seen[nt][1] = sees(col0 + nt * 8 + 2 * c + 1);
       seen_g[nt] = sees(col);
     }
     all_see = sees(col0);  // the pass's first column belongs to its first row
-    float o[NT][2 * W][4], ps[NT][NG][4], corr[NT][NG], m[NT][2], l[NT][2];
+    // m: reference (scaled, base 2), nm: -m, bar_: the raw score that moves it
+    float o[NT][2 * W][4], ps[NT][NG][4], corr[NT][NG], m[NT][2], nm[NT][2], bar_[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -348,31 +361,20 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
         ps[nt][i][0] = ps[nt][i][1] = ps[nt][i][2] = ps[nt][i][3] = 0.f;
         corr[nt][i] = 0.f;
       }
-      m[nt][0] = m[nt][1] = -INFINITY;
+      m[nt][0] = m[nt][1] = bar_[nt][0] = bar_[nt][1] = -INFINITY;
+      nm[nt][0] = nm[nt][1] = 0.f;
       l[nt][0] = l[nt][1] = 0.f;
     }
-#pragma unroll 1
-    for (int b = x.b0 + warp; b < x.b1; b += kWarps) {
-      const int st = used % ST;
-      const uint8_t* const blk = ring + st * C::kBlock;
-      const bool there = ring_ok >> st & 1u;
-      if (!ptx::mbar_wait(&bars[warp][st], (used / ST) & 1, &g_kv4_error_word, kErrBlock, limit)) limit = 1000000;
-      ++used;
-      issue();  // into the stage that the previous block left
-      if (!there) continue;
-      const int tok0 = b * kBlockTok;
-      const bool edge = tok0 + kBlockTok > all_see;  // some column ends in this block
+    // One block: tokens tok0 ..; edge: some column does not see all of them.
+    auto block = [&](const uint8_t* blk, int tok0, auto edge_) {
+      constexpr bool edge = decltype(edge_)::value;
       uint32_t kw[2][W], kp[2][NG];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         lds<W>(blk + (h * 32 + lane) * W * 4, kw[h]);
         lds<NG>(blk + k_pair_off(D) + (h * 8 + g) * NG * 4, kp[h]);
       }
-      float acc[NT][NG][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < NG; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
+      float acc[NT][NG][4];  // sum q v: the accumulator starts at -128 sum q
 #pragma unroll
       for (int j = 0; j < W; ++j)
 #pragma unroll
@@ -380,35 +382,30 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
           const uint32_t a0 = codes2(kw[0][j] >> (8 * e)), a1 = codes2(kw[1][j] >> (8 * e));
           const uint32_t a2 = codes2(kw[0][j] >> (8 * e + 4)), a3 = codes2(kw[1][j] >> (8 * e + 4));
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            mma16816(acc[nt][j / 2], a0, a1, a2, a3, qb[nt][2 * j + e][0], qb[nt][2 * j + e][1]);
+          for (int nt = 0; nt < NT; ++nt) {
+            if (j % 2 == 0 && e == 0)
+              mma16816_c(acc[nt][j / 2], a0, a1, a2, a3, qb[nt][2 * j][0], qb[nt][2 * j][1], qo[nt][j / 2][0], qo[nt][j / 2][1]);
+            else
+              mma16816(acc[nt][j / 2], a0, a1, a2, a3, qb[nt][2 * j + e][0], qb[nt][2 * j + e][1]);
+          }
         }
-      // scores of tokens g, g + 8 and columns 2c, 2c + 1, in units of log2
+      // raw scores of tokens g, g + 8 and columns 2c, 2c + 1
       float sc[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sc[nt][i] = 0.f;
+      bool grow = false;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < NG; ++i) {
-          const float s = scale_of(kp[h][i]), mp = fmaf(-128.f, s, min_of(kp[h][i]));
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int k = 0; k < 2; ++k) {
+            float v = fmaf(min_of(kp[h][0]), qs[nt][0][k], scale_of(kp[h][0]) * acc[nt][0][2 * h + k]);
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-              sc[nt][2 * h + k] += fmaf(s, acc[nt][i][2 * h + k], mp * qs[nt][i][k]);
-        }
-      bool grow = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sc[nt][i] *= p.scale_log2;
-          if (edge && tok0 + g + 8 * (i >> 1) >= seen[nt][i & 1]) sc[nt][i] = -INFINITY;
-          grow |= sc[nt][i] > m[nt][i & 1] + kRescaleLog2;
-        }
+            for (int i = 1; i < NG; ++i)
+              v = fmaf(min_of(kp[h][i]), qs[nt][i][k], fmaf(scale_of(kp[h][i]), acc[nt][i][2 * h + k], v));
+            if (edge && tok0 + g + 8 * h >= seen[nt][k]) v = -INFINITY;
+            sc[nt][2 * h + k] = v;
+            grow |= v > bar_[nt][k];
+          }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -418,9 +415,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
             float mx = fmaxf(sc[nt][k], sc[nt][2 + k]);
 #pragma unroll
             for (int q = 4; q < 32; q <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, q));
-            const float mn = fmaxf(m[nt][k], mx);
+            const float mn = fmaxf(m[nt][k], mx * p.scale_log2);
             f[k] = m[nt][k] == mn ? 1.f : ex2(m[nt][k] - mn);
             m[nt][k] = mn;
+            nm[nt][k] = mn == -INFINITY ? 0.f : -mn;  // nothing seen yet: every weight is zero
+            bar_[nt][k] = (mn + kRescaleLog2) * p.inv_scale;
             l[nt][k] *= f[k];
           }
 #pragma unroll
@@ -448,20 +447,22 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
       uint32_t pb[NT][NG][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float pe = ex2(sc[nt][2 * h] - m0), po = ex2(sc[nt][2 * h + 1] - m1);
+          const float pe = ex2(fmaf(sc[nt][2 * h], p.scale_log2, nm[nt][0]));
+          const float po = ex2(fmaf(sc[nt][2 * h + 1], p.scale_log2, nm[nt][1]));
           l[nt][0] += pe;
           l[nt][1] += po;
           const __half2 hp = __floats2half2_rn(pe, po);
           const uint32_t tr = transpose8x8(*reinterpret_cast<const uint32_t*>(&hp));
           const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&tr));  // column g, tokens 2c, 2c + 1 (+ 8 h)
-          const bool hide0 = edge && tok0 + 8 * h + 2 * c >= seen_g[nt], hide1 = edge && tok0 + 8 * h + 2 * c + 1 >= seen_g[nt];
 #pragma unroll
           for (int i = 0; i < NG; ++i) {
-            // a hidden token's pair may be anything, a NaN too: its weight of 0 does not meet it
-            const uint32_t w0 = hide0 ? 0u : vp[h][i], w1 = hide1 ? 0u : vp[h][NG + i];
+            uint32_t w0 = vp[h][i], w1 = vp[h][NG + i];
+            if (edge) {  // a hidden token's pair may be anything, a NaN too: its weight of 0 does not meet it
+              if (tok0 + 8 * h + 2 * c >= seen_g[nt]) w0 = 0u;
+              if (tok0 + 8 * h + 2 * c + 1 >= seen_g[nt]) w1 = 0u;
+            }
             pb[nt][i][h] = pack_bf16x2(w.x * scale_of(w0), w.y * scale_of(w1));
             corr[nt][i] = fmaf(w.x, min_of(w0), fmaf(w.y, min_of(w1), corr[nt][i]));
           }
@@ -479,6 +480,19 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][2 * u + e], a0, a1, a2, a3, pb[nt][u / 2][0], pb[nt][u / 2][1]);
         }
+    };
+#pragma unroll 1
+    for (int b = x.b0 + warp; b < x.b1; b += kWarps) {
+      const int st = used % ST;
+      const uint8_t* const blk = ring + st * C::kBlock;
+      const bool there = ring_ok >> st & 1u;
+      if (!ptx::mbar_wait(&bars[warp][st], (used / ST) & 1, &g_kv4_error_word, kErrBlock, limit)) limit = 1000000;
+      ++used;
+      issue();  // into the stage that the previous block left
+      if (there) {
+        if ((b + 1) * kBlockTok > all_see) block(blk, b * kBlockTok, std::true_type{});  // some column ends in this block
+        else block(blk, 0, std::false_type{});
+      }
       __syncwarp();  // every lane has read the stage before it is filled again
     }
     // ---- the warps' results joined ----
@@ -706,6 +720,7 @@ SWL_EXPORT int swl_paged_attention_kv4(int nseg, const int* rows, const void* co
   p.group = hq / hkv;
   p.out_stride = out_stride;
   p.scale_log2 = scale * 1.4426950408889634f;
+  p.inv_scale = 1.f / p.scale_log2;
   p.max_len = max_len;
   p.q = static_cast<const __nv_bfloat16*>(q_rot);
   p.whole = pl.whole;
