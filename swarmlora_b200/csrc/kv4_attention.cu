@@ -67,10 +67,10 @@ struct AttnParams4 {
 template <int D, int NT>
 struct Cfg4 {
   static constexpr int W = D / 32, NG = D / kGroup, kBlock = block_bytes(D);
-  static constexpr int kStages = (NT == 1 ? 4 : 6) * (128 / D);
+  static constexpr int kStages = (NT == 1 ? 2 : 3) * (128 / D);  // of two blocks
   static constexpr int kCols = 8 * NT;
   static constexpr int kLd = D + 4;  // floats between columns of the merge buffer: no bank twice in a quarter warp
-  static constexpr int kRing = kWarps * kStages * kBlock;
+  static constexpr int kRing = kWarps * kStages * 2 * kBlock;
   static constexpr int kMerge = kWarps * 8 * kLd * 4;
   static constexpr int kSmem = kRing + kMerge;
 };
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
   __shared__ float ml_sm[kWarps][8][2], corr_sm[kWarps][8][NG];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
-  uint8_t* const ring = dyn + warp * ST * C::kBlock;
+  uint8_t* const ring = dyn + warp * ST * 2 * C::kBlock;
   float* const merge = reinterpret_cast<float*>(dyn + C::kRing);
   if (lane == 0) {
     for (int i = 0; i < ST; ++i) ptx::mbar_init(&bars[warp][i], 1);
@@ -260,38 +260,39 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
   share_out<D, NT>(tab, p, &sh, gridDim.x);
   const int nseg = tab.seg.nseg;
 
-  // ---- loads: this warp's blocks in the order in which it will use them ----
+  // ---- loads: this warp's pairs of blocks in the order in which it will use them ----
   Walk lw(sh, nseg, p.whole);
   Piece lp;
   bool more = lw.next(sh, nseg, &lp);
-  int lb = more ? lp.b0 + warp : 0;       // next block of the load piece that is not in the batch
-  const uint8_t* addr = nullptr;          // lane i: the batch's i-th block (nullptr: no such page), which it fetches
+  int lb = more ? lp.b0 + 2 * warp : 0;   // next block of the load piece that is not in the batch
+  const uint8_t *addr0 = nullptr, *addr1 = nullptr;  // lane i: the batch's i-th pair (nullptr: no such block), which it fetches
   int batch = 0, taken = 0, issued = 0;
-  uint32_t batch_ok = 0, ring_ok = 0;     // bit per batch entry and per stage: the block exists
+  uint32_t ok0 = 0, ok1 = 0, ring_ok = 0;  // a bit per batch entry; two bits per stage: the blocks exist
   auto issue = [&]() {
-    while (more && taken == batch) {      // the next up to 32 blocks of this warp
-      const int left = lp.b1 > lb ? (lp.b1 - lb + kWarps - 1) / kWarps : 0;
+    while (more && taken == batch) {      // the next up to 32 pairs of this warp
+      const int left = lp.b1 > lb ? (lp.b1 - lb + 2 * kWarps - 1) / (2 * kWarps) : 0;
       if (left == 0) {
         more = lw.next(sh, nseg, &lp);
-        lb = lp.b0 + warp;
+        lb = lp.b0 + 2 * warp;
         continue;
       }
       batch = min(left, 32);
       taken = 0;
-      addr = lane < batch ? block_of<D>(tab.c, lp.slot, lb + lane * kWarps, lp.head) : nullptr;
-      batch_ok = __ballot_sync(0xffffffffu, addr != nullptr);
-      lb += batch * kWarps;
+      const int b = lb + lane * 2 * kWarps;
+      addr0 = lane < batch ? block_of<D>(tab.c, lp.slot, b, lp.head) : nullptr;
+      addr1 = lane < batch && b + 1 < lp.b1 ? block_of<D>(tab.c, lp.slot, b + 1, lp.head) : nullptr;
+      ok0 = __ballot_sync(0xffffffffu, addr0 != nullptr);
+      ok1 = __ballot_sync(0xffffffffu, addr1 != nullptr);
+      lb += batch * 2 * kWarps;
     }
     if (!more) return;
     const int st = issued % ST;
-    ring_ok = (ring_ok & ~(1u << st)) | (batch_ok >> taken & 1u) << st;
+    ring_ok = (ring_ok & ~(3u << 2 * st)) | ((ok0 >> taken & 1u) | (ok1 >> taken & 1u) << 1) << 2 * st;
     if (lane == taken) {
-      if (addr) {
-        ptx::mbar_arrive_expect_tx(&bars[warp][st], C::kBlock);
-        ptx::bulk_load(ring + st * C::kBlock, addr, C::kBlock, &bars[warp][st]);
-      } else {
-        ptx::mbar_arrive(&bars[warp][st]);
-      }
+      uint64_t* const bar = &bars[warp][st];
+      ptx::mbar_arrive_expect_tx(bar, (addr0 ? C::kBlock : 0) + (addr1 ? C::kBlock : 0));
+      if (addr0) ptx::bulk_load(ring + st * 2 * C::kBlock, addr0, C::kBlock, bar);
+      if (addr1) ptx::bulk_load(ring + (st * 2 + 1) * C::kBlock, addr1, C::kBlock, bar);
     }
     ++taken;
     ++issued;
@@ -365,8 +366,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
       nm[nt][0] = nm[nt][1] = 0.f;
       l[nt][0] = l[nt][1] = 0.f;
     }
-    // One block: tokens tok0 ..; edge: some column does not see all of them.
-    auto block = [&](const uint8_t* blk, int tok0, auto edge_) {
+    // Raw scores of one block (tokens tok0 ..): tokens g, g + 8 and columns 2c, 2c + 1.
+    // edge: some column does not see all of the tokens.
+    auto scores = [&](const uint8_t* blk, int tok0, float (&sc)[NT][4], auto edge_) {
       constexpr bool edge = decltype(edge_)::value;
       uint32_t kw[2][W], kp[2][NG];
 #pragma unroll
@@ -389,9 +391,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
               mma16816(acc[nt][j / 2], a0, a1, a2, a3, qb[nt][2 * j + e][0], qb[nt][2 * j + e][1]);
           }
         }
-      // raw scores of tokens g, g + 8 and columns 2c, 2c + 1
-      float sc[NT][4];
-      bool grow = false;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -404,15 +403,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
               v = fmaf(min_of(kp[h][i]), qs[nt][i][k], fmaf(scale_of(kp[h][i]), acc[nt][i][2 * h + k], v));
             if (edge && tok0 + g + 8 * h >= seen[nt][k]) v = -INFINITY;
             sc[nt][2 * h + k] = v;
-            grow |= v > bar_[nt][k];
           }
-      if (__any_sync(0xffffffffu, grow)) {
+    };
+    // Moves the references to the largest scores of two blocks, and what is summed with them.
+    auto rescale = [&](const float (&s0)[NT][4], const float (&s1)[NT][4]) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float f[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            float mx = fmaxf(sc[nt][k], sc[nt][2 + k]);
+            float mx = fmaxf(fmaxf(s0[nt][k], s0[nt][2 + k]), fmaxf(s1[nt][k], s1[nt][2 + k]));
 #pragma unroll
             for (int q = 4; q < 32; q <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, q));
             const float mn = fmaxf(m[nt][k], mx * p.scale_log2);
@@ -437,7 +437,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
             corr[nt][i] *= (g & 1) ? fo : fe;
           }
         }
-      }
+    };
+    // Adds one block's values with the weights of its scores.
+    auto values = [&](const uint8_t* blk, int tok0, const float (&sc)[NT][4], auto edge_) {
+      constexpr bool edge = decltype(edge_)::value;
       uint32_t vw[2][W], vp[2][2 * NG];  // vp[h]: tokens 2c, 2c + 1 (+ 8 h)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -481,18 +484,38 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
           for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][2 * u + e], a0, a1, a2, a3, pb[nt][u / 2][0], pb[nt][u / 2][1]);
         }
     };
+    // Two blocks: their scores first, one vote on the references, then their values.
+    auto two = [&](const uint8_t* blk, int tok0, uint32_t there, auto edge) {
+      float sc[2][NT][4];
+      bool grow = false;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (there >> i & 1u) {
+          scores(blk + i * C::kBlock, tok0 + i * kBlockTok, sc[i], edge);
+        } else {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) sc[i][nt][0] = sc[i][nt][1] = sc[i][nt][2] = sc[i][nt][3] = -INFINITY;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) grow |= sc[i][nt][k] > bar_[nt][k & 1];
+      }
+      if (__any_sync(0xffffffffu, grow)) rescale(sc[0], sc[1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (there >> i & 1u) values(blk + i * C::kBlock, tok0 + i * kBlockTok, sc[i], edge);
+    };
 #pragma unroll 1
-    for (int b = x.b0 + warp; b < x.b1; b += kWarps) {
+    for (int b = x.b0 + 2 * warp; b < x.b1; b += 2 * kWarps) {
       const int st = used % ST;
-      const uint8_t* const blk = ring + st * C::kBlock;
-      const bool there = ring_ok >> st & 1u;
+      const uint8_t* const blk = ring + st * 2 * C::kBlock;
+      const uint32_t there = ring_ok >> 2 * st & 3u;
       if (!ptx::mbar_wait(&bars[warp][st], (used / ST) & 1, &g_kv4_error_word, kErrBlock, limit)) limit = 1000000;
       ++used;
-      issue();  // into the stage that the previous block left
-      if (there) {
-        if ((b + 1) * kBlockTok > all_see) block(blk, b * kBlockTok, std::true_type{});  // some column ends in this block
-        else block(blk, 0, std::false_type{});
-      }
+      issue();  // into the stage that the previous pair left
+      if ((b + 2) * kBlockTok > all_see) two(blk, b * kBlockTok, there, std::true_type{});  // some column ends here
+      else two(blk, b * kBlockTok, there, std::false_type{});
       __syncwarp();  // every lane has read the stage before it is filled again
     }
     // ---- the warps' results joined ----
