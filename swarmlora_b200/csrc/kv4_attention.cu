@@ -47,7 +47,7 @@ __device__ unsigned int g_kv4_error_word = 0;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr unsigned kErrBlock = 111;
 constexpr float kRescaleLog2 = 8.f;
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 
 struct AttnTable4 {
   RowSegments seg;
@@ -178,7 +178,7 @@ __device__ __forceinline__ void share_out(const AttnTable4& tab, const AttnParam
     if (threadIdx.x == 0) {
       sh->unit[tab.seg.nseg] = u;
       sh->pair[tab.seg.nseg] = pr;
-      sh->per_cta = max((u + ctas - 1) / ctas, int64_t{kWarps});
+      sh->per_cta = max((u + ctas - 1) / ctas, int64_t{2 * kWarps});
     }
   }
   __syncthreads();
@@ -238,8 +238,12 @@ struct Walk {
   }
 };
 
-template <int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
+// kDual (columns up to 4, NT = 1): columns 4 .. 7 repeat the queries of 0 .. 3; the first
+// four go with the first block of a pair and the other four with its second, so that
+// scores, exponentials and weights of two blocks are computed at once (columns
+// that would otherwise be empty). The two sets keep their own references and meet at the merge.
+template <int D, int NT, bool kDual>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
     kv4_attention_kernel(const __grid_constant__ AttnTable4 tab, const __grid_constant__ AttnParams4 p) {
   using C = Cfg4<D, NT>;
   constexpr int W = C::W, NG = C::NG, ST = C::kStages;
@@ -319,7 +323,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
     };
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int col = col0 + nt * 8 + g;
+      const int col = col0 + (kDual ? g & 3 : nt * 8 + g);
       const __nv_bfloat16* src =
           p.q + (static_cast<int64_t>(row0 + col / p.group) * p.hq + x.head * p.group + col % p.group) * D;
       float part[NG];
@@ -346,8 +350,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
         qo[nt][i][0] = -128.f * qs[nt][i][0];
         qo[nt][i][1] = -128.f * qs[nt][i][1];
       }
-      seen[nt][0] = sees(col0 + nt * 8 + 2 * c);
-      seen[nt][1] = sees(col0 + nt * 8 + 2 * c + 1);
+      const int c2 = kDual ? 2 * c & 3 : nt * 8 + 2 * c;
+      seen[nt][0] = sees(col0 + c2);
+      seen[nt][1] = sees(col0 + c2 + 1);
       seen_g[nt] = sees(col);
     }
     all_see = sees(col0);  // the pass's first column belongs to its first row
@@ -366,17 +371,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
       nm[nt][0] = nm[nt][1] = 0.f;
       l[nt][0] = l[nt][1] = 0.f;
     }
-    // Raw scores of one block (tokens tok0 ..): tokens g, g + 8 and columns 2c, 2c + 1.
-    // edge: some column does not see all of the tokens.
-    auto scores = [&](const uint8_t* blk, int tok0, float (&sc)[NT][4], auto edge_) {
-      constexpr bool edge = decltype(edge_)::value;
-      uint32_t kw[2][W], kp[2][NG];
+    // Sums q v of one block and each group: tokens g, g + 8 and columns 2c, 2c + 1.
+    auto product = [&](const uint8_t* blk, float (&acc)[NT][NG][4]) {
+      uint32_t kw[2][W];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        lds<W>(blk + (h * 32 + lane) * W * 4, kw[h]);
-        lds<NG>(blk + k_pair_off(D) + (h * 8 + g) * NG * 4, kp[h]);
-      }
-      float acc[NT][NG][4];  // sum q v: the accumulator starts at -128 sum q
+      for (int h = 0; h < 2; ++h) lds<W>(blk + (h * 32 + lane) * W * 4, kw[h]);
+      // the accumulator starts at -128 sum q
 #pragma unroll
       for (int j = 0; j < W; ++j)
 #pragma unroll
@@ -391,6 +391,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
               mma16816(acc[nt][j / 2], a0, a1, a2, a3, qb[nt][2 * j + e][0], qb[nt][2 * j + e][1]);
           }
         }
+    };
+    // Their raw scores. edge: some column does not see all of the tokens (from tok0 on); a block
+    // that is not there is seen by none.
+    auto scores = [&](const uint8_t* blk, int tok0, bool there, const float (&acc)[NT][NG][4], float (&sc)[NT][4], auto edge_) {
+      constexpr bool edge = decltype(edge_)::value;
+      uint32_t kp[2][NG];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) lds<NG>(blk + k_pair_off(D) + (h * 8 + g) * NG * 4, kp[h]);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -401,18 +409,19 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
 #pragma unroll
             for (int i = 1; i < NG; ++i)
               v = fmaf(min_of(kp[h][i]), qs[nt][i][k], fmaf(scale_of(kp[h][i]), acc[nt][i][2 * h + k], v));
-            if (edge && tok0 + g + 8 * h >= seen[nt][k]) v = -INFINITY;
+            if (edge && (!there || tok0 + g + 8 * h >= seen[nt][k])) v = -INFINITY;
             sc[nt][2 * h + k] = v;
           }
     };
-    // Moves the references to the largest scores of two blocks, and what is summed with them.
-    auto rescale = [&](const float (&s0)[NT][4], const float (&s1)[NT][4]) {
+    // Moves the references to the largest of n scores a thread, and what is summed with them.
+    auto rescale = [&](const float (&sc)[2][NT][4], int n) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float f[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            float mx = fmaxf(fmaxf(s0[nt][k], s0[nt][2 + k]), fmaxf(s1[nt][k], s1[nt][2 + k]));
+            float mx = fmaxf(sc[0][nt][k], sc[0][nt][2 + k]);
+            if (n > 1) mx = fmaxf(mx, fmaxf(sc[1][nt][k], sc[1][nt][2 + k]));
 #pragma unroll
             for (int q = 4; q < 32; q <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, q));
             const float mn = fmaxf(m[nt][k], mx * p.scale_log2);
@@ -438,16 +447,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
           }
         }
     };
-    // Adds one block's values with the weights of its scores.
-    auto values = [&](const uint8_t* blk, int tok0, const float (&sc)[NT][4], auto edge_) {
+    // The weights p s of one block's scores as the second operand of the value product: column g,
+    // tokens 2c, 2c + 1 (+ 8 h). blk, tok0, there: the block of this lane's column g.
+    auto weights = [&](const uint8_t* blk, int tok0, bool there, const float (&sc)[NT][4], uint32_t (&pb)[NT][NG][2],
+                       auto edge_) {
       constexpr bool edge = decltype(edge_)::value;
-      uint32_t vw[2][W], vp[2][2 * NG];  // vp[h]: tokens 2c, 2c + 1 (+ 8 h)
+      uint32_t vp[2][2 * NG];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        lds<W>(blk + v_code_off(D) + (h * 32 + lane) * W * 4, vw[h]);
-        lds<2 * NG>(blk + v_pair_off(D) + (h * 8 + 2 * c) * NG * 4, vp[h]);
-      }
-      uint32_t pb[NT][NG][2];
+      for (int h = 0; h < 2; ++h) lds<2 * NG>(blk + v_pair_off(D) + (h * 8 + 2 * c) * NG * 4, vp[h]);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -463,8 +470,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
           for (int i = 0; i < NG; ++i) {
             uint32_t w0 = vp[h][i], w1 = vp[h][NG + i];
             if (edge) {  // a hidden token's pair may be anything, a NaN too: its weight of 0 does not meet it
-              if (tok0 + 8 * h + 2 * c >= seen_g[nt]) w0 = 0u;
-              if (tok0 + 8 * h + 2 * c + 1 >= seen_g[nt]) w1 = 0u;
+              if (!there || tok0 + 8 * h + 2 * c >= seen_g[nt]) w0 = 0u;
+              if (!there || tok0 + 8 * h + 2 * c + 1 >= seen_g[nt]) w1 = 0u;
             }
             pb[nt][i][h] = pack_bf16x2(w.x * scale_of(w0), w.y * scale_of(w1));
             corr[nt][i] = fmaf(w.x, min_of(w0), fmaf(w.y, min_of(w1), corr[nt][i]));
@@ -474,6 +481,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
         for (int i = 0; i < NG; ++i)
           mma16816(ps[nt][i], 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, pb[nt][i][0], pb[nt][i][1]);
       }
+    };
+    // Adds one block's values with these weights.
+    auto values = [&](const uint8_t* blk, const uint32_t (&pb)[NT][NG][2]) {
+      uint32_t vw[2][W];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) lds<W>(blk + v_code_off(D) + (h * 32 + lane) * W * 4, vw[h]);
 #pragma unroll
       for (int u = 0; u < W; ++u)
 #pragma unroll
@@ -488,23 +501,57 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
     auto two = [&](const uint8_t* blk, int tok0, uint32_t there, auto edge) {
       float sc[2][NT][4];
       bool grow = false;
+      if constexpr (kDual) {
+        float a0[NT][NG][4], a1[NT][NG][4];
+        product(blk, a0);
+        product(blk + C::kBlock, a1);
+        const int mine = c >> 1, mine_g = g >> 2;  // the block of columns 2c, 2c + 1, and of column g
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (there >> i & 1u) {
-          scores(blk + i * C::kBlock, tok0 + i * kBlockTok, sc[i], edge);
-        } else {
+        for (int i = 0; i < NG; ++i)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) sc[i][nt][0] = sc[i][nt][1] = sc[i][nt][2] = sc[i][nt][3] = -INFINITY;
+          for (int k = 0; k < 4; ++k)
+            if (mine) a0[0][i][k] = a1[0][i][k];
+        scores(blk + mine * C::kBlock, tok0 + mine * kBlockTok, there >> mine & 1u, a0, sc[0], edge);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) grow |= sc[0][0][k] > bar_[0][k & 1];
+        if (__any_sync(0xffffffffu, grow)) rescale(sc, 1);
+        uint32_t pb[NT][NG][2];
+        weights(blk + mine_g * C::kBlock, tok0 + mine_g * kBlockTok, there >> mine_g & 1u, sc[0], pb, edge);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t only[NT][NG][2];  // this block's columns
+#pragma unroll
+          for (int i = 0; i < NG; ++i) {
+            only[0][i][0] = mine_g == j ? pb[0][i][0] : 0u;
+            only[0][i][1] = mine_g == j ? pb[0][i][1] : 0u;
+          }
+          values(blk + j * C::kBlock, only);
         }
+      } else {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int i = 0; i < 2; ++i) {
+          if (there >> i & 1u) {
+            float acc[NT][NG][4];
+            product(blk + i * C::kBlock, acc);
+            scores(blk + i * C::kBlock, tok0 + i * kBlockTok, true, acc, sc[i], edge);
+          } else {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) grow |= sc[i][nt][k] > bar_[nt][k & 1];
+            for (int nt = 0; nt < NT; ++nt) sc[i][nt][0] = sc[i][nt][1] = sc[i][nt][2] = sc[i][nt][3] = -INFINITY;
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) grow |= sc[i][nt][k] > bar_[nt][k & 1];
+        }
+        if (__any_sync(0xffffffffu, grow)) rescale(sc, 2);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (there >> i & 1u) {
+            uint32_t pb[NT][NG][2];
+            weights(blk + i * C::kBlock, tok0 + i * kBlockTok, true, sc[i], pb, edge);
+            values(blk + i * C::kBlock, pb);
+          }
       }
-      if (__any_sync(0xffffffffu, grow)) rescale(sc[0], sc[1]);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (there >> i & 1u) values(blk + i * C::kBlock, tok0 + i * kBlockTok, sc[i], edge);
     };
 #pragma unroll 1
     for (int b = x.b0 + 2 * warp; b < x.b1; b += 2 * kWarps) {
@@ -514,7 +561,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
       if (!ptx::mbar_wait(&bars[warp][st], (used / ST) & 1, &g_kv4_error_word, kErrBlock, limit)) limit = 1000000;
       ++used;
       issue();  // into the stage that the previous pair left
-      if ((b + 2) * kBlockTok > all_see) two(blk, b * kBlockTok, there, std::true_type{});  // some column ends here
+      // some column ends here, or a block is missing
+      if ((b + 2) * kBlockTok > all_see || there != 3u) two(blk, b * kBlockTok, there, std::true_type{});
       else two(blk, b * kBlockTok, there, std::false_type{});
       __syncwarp();  // every lane has read the stage before it is filled again
     }
@@ -550,22 +598,26 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
         if (c == 0) corr_sm[warp][g][i] = s;
       }
       __syncthreads();
-      const int mc = threadIdx.x / (D / 4), d4 = threadIdx.x % (D / 4) * 4;  // column of the 8, dimensions
-      const int col = col0 + nt * 8 + mc;
-      if (mc < 8 && col < ncols) {
+      constexpr int kMerged = kDual ? 4 : 8;  // columns of the pass, and sets of results for each
+      constexpr int kSets = kDual ? 2 * kWarps : kWarps;
+      for (int at = threadIdx.x; at < kMerged * (D / 4); at += kWarps * 32) {
+        const int mc = at / (D / 4), d4 = at % (D / 4) * 4;  // column, dimensions
+        const int col = col0 + nt * 8 + mc;
+        if (col >= ncols) continue;
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml_sm[w][mc][0]);
+        for (int e = 0; e < kSets; ++e) top = fmaxf(top, ml_sm[e % kWarps][mc + e / kWarps * 4][0]);
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
         float sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float mw = ml_sm[w][mc][0], lw_ = ml_sm[w][mc][1];
+        for (int e = 0; e < kSets; ++e) {
+          const int w = e % kWarps, mw_c = mc + e / kWarps * 4;
+          const float mw = ml_sm[w][mw_c][0], lw_ = ml_sm[w][mw_c][1];
           // no reference: nothing seen (no sum), or nothing but NaN, which stays
           const float f = mw == -INFINITY ? (lw_ == 0.f ? 0.f : 1.f) : ex2(mw - top);
           if (f == 0.f) continue;
-          const float4 v = *reinterpret_cast<const float4*>(merge + (w * 8 + mc) * C::kLd + d4);
-          const float z = corr_sm[w][mc][d4 / kGroup];
+          const float4 v = *reinterpret_cast<const float4*>(merge + (w * 8 + mw_c) * C::kLd + d4);
+          const float z = corr_sm[w][mw_c][d4 / kGroup];
           sum += f * lw_;
           a.x += f * (v.x + z);
           a.y += f * (v.y + z);
@@ -645,6 +697,7 @@ __global__ void __launch_bounds__(kWarps * 32)
 
 struct Plan4 {
   int nt, ctas, whole;
+  bool dual;
   int64_t pairs;
 };
 
@@ -661,29 +714,30 @@ Plan4 make_plan4(int nseg, const int* rows, int hq, int hkv, int max_len) {
   int most = 0;
   for (int i = 0; i < nseg; ++i) most = std::max(most, rows[i]);
   pl.nt = static_cast<int64_t>(most) * group > 8 ? 2 : 1;
+  pl.dual = static_cast<int64_t>(most) * group <= 4;
   pl.pairs = 0;
   for (int i = 0; i < nseg; ++i) pl.pairs += (static_cast<int64_t>(rows[i]) * group + 8 * pl.nt - 1) / (8 * pl.nt) * hkv;
   const int64_t blocks = (max_len + kBlockTok - 1) / kBlockTok;
-  const int64_t slots = static_cast<int64_t>(sm_count4()) * (pl.nt == 1 ? 2 : 1);  // CTAs at a time
+  const int64_t slots = static_cast<int64_t>(sm_count4()) * (pl.nt == 1 ? 3 : 2);  // CTAs at a time
   // whole pairs where cutting them would at most halve what a CTA has to do
-  pl.whole = blocks <= 2 * std::max<int64_t>((pl.pairs * blocks + slots - 1) / slots, kWarps) ? 1 : 0;
+  pl.whole = blocks <= 2 * std::max<int64_t>((pl.pairs * blocks + slots - 1) / slots, 2 * kWarps) ? 1 : 0;
   pl.ctas = static_cast<int>(std::max<int64_t>(
-      1, std::min<int64_t>(slots, pl.whole ? pl.pairs : (pl.pairs * blocks + kWarps - 1) / kWarps)));
+      1, std::min<int64_t>(slots, pl.whole ? pl.pairs : (pl.pairs * blocks + 2 * kWarps - 1) / (2 * kWarps))));
   return pl;
 }
 
-template <int D, int NT>
+template <int D, int NT, bool kDual>
 int launch_kv4(const AttnTable4& t, const AttnParams4& p, const Plan4& pl, cudaStream_t st) {
   int dev = 0;
   SWL_CUDA_TRY(cudaGetDevice(&dev));
   static std::atomic<uint64_t> done{0};  // devices whose kernel has its shared memory limit raised
   const uint64_t bit = uint64_t{1} << (dev & 63);
   if (!(done.load(std::memory_order_relaxed) & bit)) {
-    SWL_CUDA_TRY(cudaFuncSetAttribute(kv4_attention_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    SWL_CUDA_TRY(cudaFuncSetAttribute(kv4_attention_kernel<D, NT, kDual>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       Cfg4<D, NT>::kSmem));
     done.fetch_or(bit);
   }
-  SWL_CUDA_TRY(launch_kernel(kv4_attention_kernel<D, NT>, dim3(pl.ctas), dim3(kWarps * 32), Cfg4<D, NT>::kSmem, st, 1, t, p));
+  SWL_CUDA_TRY(launch_kernel(kv4_attention_kernel<D, NT, kDual>, dim3(pl.ctas), dim3(kWarps * 32), Cfg4<D, NT>::kSmem, st, 1, t, p));
   if (!pl.whole)
     SWL_CUDA_TRY(launch_kernel(kv4_join_kernel<D, NT>, dim3(static_cast<unsigned>(pl.pairs)), dim3(kWarps * 32), 0, st, 1, t, p,
                                pl.ctas));
@@ -749,6 +803,11 @@ SWL_EXPORT int swl_paged_attention_kv4(int nseg, const int* rows, const void* co
   p.whole = pl.whole;
   p.part = part;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (head_dim == 128) return pl.nt == 1 ? kv4::launch_kv4<128, 1>(t, p, pl, st) : kv4::launch_kv4<128, 2>(t, p, pl, st);
-  return pl.nt == 1 ? kv4::launch_kv4<64, 1>(t, p, pl, st) : kv4::launch_kv4<64, 2>(t, p, pl, st);
+  if (head_dim == 128)
+    return pl.dual      ? kv4::launch_kv4<128, 1, true>(t, p, pl, st)
+           : pl.nt == 1 ? kv4::launch_kv4<128, 1, false>(t, p, pl, st)
+                        : kv4::launch_kv4<128, 2, false>(t, p, pl, st);
+  return pl.dual      ? kv4::launch_kv4<64, 1, true>(t, p, pl, st)
+         : pl.nt == 1 ? kv4::launch_kv4<64, 1, false>(t, p, pl, st)
+                      : kv4::launch_kv4<64, 2, false>(t, p, pl, st);
 }
