@@ -297,9 +297,12 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_lens, 
     return out
 
 
+_KV4_BLOCK = {64: 1152, 128: 2304}  # swl_kv4_block_bytes
+
+
 def kv4_block_bytes(head_dim: int = 128) -> int:
     """Bytes of one cache block: 16 tokens of one kv head, K and V."""
-    n = int(lib().swl_kv4_block_bytes(head_dim))
+    n = _KV4_BLOCK.get(head_dim)
     if not n:
         raise ValueError(f"kv4 cache: head_dim must be 64 or 128 (got {head_dim})")
     return n
@@ -313,18 +316,18 @@ def kv4_cache(num_pages: int, hkv: int, head_dim: int = 128, page: int = 16, dev
                        device=device if device is not None else "cuda")
 
 
-def _slot_rows(ts, n: int, what: str, dtype, device, first=None) -> array:
-    """Addresses of each slot's rows: a list of tensors, or one tensor with a
-    row per slot (first: the first row of each slot)."""
+def _slot_rows(ts, n: int, what: str, dtype, size: int, device, first=None) -> array:
+    """Addresses of each slot's rows (elements of `size` bytes): a list of tensors,
+    or one tensor with a row per slot (first: the first row of each slot)."""
     if isinstance(ts, torch.Tensor):
-        if ts.dtype is not dtype or ts.device != device:
-            raise ValueError(f"{what}: {dtype} on {device} is needed")
-        if (ts.dim() > 1 and ts.stride(-1) != 1) or (first is None and ts.shape[0] != n):
-            raise ValueError(f"{what}: one row per slot, contiguous inside")
-        base, by = ts.data_ptr(), ts.element_size() * ts.stride(0)
-        if first is not None:
-            return array("Q", [base + i * by for i in first])
-        return array("Q", range(base, base + n * by, by)) if by > 0 else array("Q", [base]) * n
+        st = ts.stride()
+        if ts.dtype is not dtype or ts.device != device or (len(st) > 1 and st[-1] != 1) or \
+                (first is None and ts.size(0) != n):
+            raise ValueError(f"{what}: {dtype} on {device}, one row per slot, contiguous inside")
+        base, by = ts.data_ptr(), size * st[0]
+        if first is None:
+            return array("Q", range(base, base + n * by, by)) if by > 0 else array("Q", (base,)) * n
+        return array("Q", [base + i * by for i in first])
     if len(ts) != n or any(t.dtype is not dtype or t.device != device or
                            (t.dim() and t.numel() > 1 and t.stride(-1) != 1) for t in ts):
         raise ValueError(f"{what}: one {dtype} tensor per slot on {device}, contiguous inside")
@@ -336,20 +339,24 @@ def _kv4_slots(block_tables, caches, n: int, hkv: int, head_dim: int, page: int,
     if isinstance(block_tables, torch.Tensor):
         if block_tables.dim() != 2:
             raise ValueError("block tables: [slots, pages] or one tensor per slot")
-        table_len = block_tables.shape[1]
+        table_len = block_tables.size(1)
     else:
         table_len = min((t.shape[0] for t in block_tables), default=1)
-    tables = _slot_rows(block_tables, n, "block tables", torch.int32, device)
-    each = (caches,) if isinstance(caches, torch.Tensor) else caches
+    tables = _slot_rows(block_tables, n, "block tables", torch.int32, 4, device)
     want = (page // 16, hkv, kv4_block_bytes(head_dim))
-    for c in each:
-        if c.dtype is not torch.uint8 or c.device != device or not c.is_contiguous() or c.shape[1:] != want:
-            raise ValueError(f"4-bit cache: contiguous uint8 [pages, {want[0]}, {want[1]}, {want[2]}] on {device} is needed")
     if isinstance(caches, torch.Tensor):
-        return tables, table_len, array("Q", [caches.data_ptr()]) * n, caches.shape[0]
-    if len(each) != n:
+        _kv4_check(caches, want, device)
+        return tables, table_len, array("Q", (caches.data_ptr(),)) * n, caches.size(0)
+    for c in caches:
+        _kv4_check(c, want, device)
+    if len(caches) != n:
         raise ValueError("4-bit cache: one for all slots, or one per slot")
-    return tables, table_len, array("Q", [c.data_ptr() for c in each]), min((c.shape[0] for c in each), default=1)
+    return tables, table_len, array("Q", [c.data_ptr() for c in caches]), min((c.size(0) for c in caches), default=1)
+
+
+def _kv4_check(cache: torch.Tensor, want: tuple, device) -> None:
+    if cache.dtype is not torch.uint8 or cache.device != device or not cache.is_contiguous() or cache.shape[1:] != want:
+        raise ValueError(f"4-bit cache: contiguous uint8 [pages, {want[0]}, {want[1]}, {want[2]}] on {device} is needed")
 
 
 def _first_rows(rows) -> list:
@@ -357,8 +364,9 @@ def _first_rows(rows) -> list:
 
 
 def _packed(name: str, t: torch.Tensor, rows: int, width: int, device) -> None:
-    if t.dtype is not torch.bfloat16 or t.device != device or not t.is_contiguous() or t.shape[0] < rows or \
-            t.numel() != t.shape[0] * width:
+    have = t.size(0)
+    if t.dtype is not torch.bfloat16 or t.device != device or not t.is_contiguous() or have < rows or \
+            t.numel() != have * width:
         raise ValueError(f"{name}: contiguous bf16 with at least {rows} rows of {width} on {device} is needed")
 
 
@@ -399,9 +407,9 @@ def kv4_append(qkvs, block_tables, caches, seqlens, q_rot, cos_sin, hq: int, hkv
     if k_rot is not None:
         _packed("kv4_append: k_rot", k_rot, total, hkv * head_dim, dev)
     _packed("kv4_append: cos_sin", cos_sin, 1, head_dim, dev)
-    src = _slot_rows(qkvs, n, "kv4_append: qkv", torch.bfloat16, dev, _first_rows(rows) if packed else None)
+    src = _slot_rows(qkvs, n, "kv4_append: qkv", torch.bfloat16, 2, dev, _first_rows(rows) if packed else None)
     tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, dev)
-    lens = _slot_rows(seqlens, n, "kv4_append: seqlens", torch.int32, dev)
+    lens = _slot_rows(seqlens, n, "kv4_append: seqlens", torch.int32, 4, dev)
     counts = _ints(rows)
     check(lib().swl_kv4_append(n, _addr(counts), _addr(src), stride, _addr(tables), table_len, _addr(cache), pages,
                                _addr(lens), hq, hkv, head_dim, page, cos_sin.data_ptr(), cos_sin.shape[0],
@@ -450,9 +458,9 @@ def paged_attention_kv4(rows, block_tables, caches, seqlens, outs, q_rot, hq: in
     _packed("paged_attention_kv4: q_rot", q_rot, total, width, dev)
     stride = _slots_of_rows("paged_attention_kv4: out", outs, rows, total, width)
     first = _first_rows(rows) if isinstance(outs, torch.Tensor) else None
-    dst = _slot_rows(outs, n, "paged_attention_kv4: out", torch.bfloat16, dev, first)
+    dst = _slot_rows(outs, n, "paged_attention_kv4: out", torch.bfloat16, 2, dev, first)
     tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, dev)
-    lens = _slot_rows(seqlens, n, "paged_attention_kv4: seqlens", torch.int32, dev)
+    lens = _slot_rows(seqlens, n, "paged_attention_kv4: seqlens", torch.int32, 4, dev)
     counts = _ints(rows)
     L = lib()
     need = L.swl_kv4_part_floats(n, _addr(counts), hq, hkv, head_dim, max_len)

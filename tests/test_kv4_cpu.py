@@ -90,7 +90,9 @@ def test_kv4_calls_of_nothing_are_done(native, call):
 
 
 def test_block_bytes(native):
+    from swarmlora_b200 import worker_ops as wo
     assert [native.lib().swl_kv4_block_bytes(d) for d in (64, 128, 96)] == [1152, 2304, 0]
+    assert [wo.kv4_block_bytes(d) for d in (64, 128)] == [1152, 2304]
 
 
 def test_python_entry_points_refuse_host_tensors(native):
