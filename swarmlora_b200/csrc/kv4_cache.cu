@@ -88,24 +88,40 @@ __device__ __forceinline__ uint32_t group_pair(float lo, float hi) {
 __device__ __forceinline__ float pair_scale(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float pair_min(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
+// The codes of 8 numbers: (x - m) / s rounded as IEEE division rounds it, then to
+// the nearest integer, ties to even, within 0 .. 15. In the range where nothing under- or
+// overflows the quotient comes from the correctly rounded reciprocal r of s by Markstein's
+// theorem (q = a r, then q + r (a - q s) is the correctly rounded a / s); elsewhere from a
+// division. NaN (a group without a finite scale) ends as code 0.
 __device__ __forceinline__ uint32_t codes8(const float (&x)[8], uint32_t pair) {
   const float s = pair_scale(pair), m = pair_min(pair);
+  float q[8];
+  if (s >= 0x1p-60f && s <= 0x1p60f) {
+    const float r = __frcp_rn(s);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float a = __fsub_rn(x[e], m), q0 = __fmul_rn(a, r);
+      q[e] = __fmaf_rn(r, __fmaf_rn(-q0, s, a), q0);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = s > 0.f ? __fdiv_rn(__fsub_rn(x[e], m), s) : 0.f;
+  }
   uint32_t w = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    // NaN (a group that holds no finite scale) ends as code 0
-    const float c = s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[e], m), s)), 0.f), 15.f) : 0.f;
-    w |= static_cast<uint32_t>(c) << (4 * e);
-  }
+  for (int e = 0; e < 8; ++e)  // adding 1.5 * 2^23 rounds and leaves the code in the low bits
+    w |= (__float_as_uint(__fadd_rn(fminf(fmaxf(q[e], 0.f), 15.f), 12582912.f)) & 15u) << (4 * e);
   return w;
 }
 
 // CTA = (one block's 16 positions of a slot, heads_per_cta heads of q | k | v).
 // TPH = D / 16 threads share a head: each holds 8 dimensions of the lower half
 // and the 8 they are rotated with, which are one code word of K each; a warp
-// holds 32 / TPH tokens, so the reductions over a group stay inside it.
+// holds 32 / TPH tokens, so the reductions over a group stay inside it. Memory bounds
+// it (rows in, rotated rows and codes out): 6499 rows of 32 + 2 * 8 heads of 128 in 36.6 us,
+// 154 MB at 4.2 TB/s; four CTAs an SM rather than three 39.2 -> 36.6.
 template <int D>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ AppendTable tab,
+__global__ void __launch_bounds__(256, 4) kv4_append_kernel(const __grid_constant__ AppendTable tab,
                                                          const AppendParams p) {
   constexpr int TPH = D / 16, TPW = 32 / TPH, TG = kBlockTok / TPW, HW = 8 / TG;  // HW heads side by side
   ptx::grid_dep_wait();
@@ -137,15 +153,19 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__
   const __nv_bfloat16* src = tab.qkv[s] + local * p.qkv_stride;
   const int hkv = tab.c.hkv;
   const int h0 = blockIdx.y * p.heads_per_cta, h1 = min(h0 + p.heads_per_cta, p.hq + 2 * hkv);
-  for (int h = h0 + warp / TG; h < h1; h += HW) {
-    uint4 u = make_uint4(0, 0, 0, 0), w = u;
-    if (known) {
+  uint4 u = make_uint4(0, 0, 0, 0), w = u;
+  auto load = [&](int h) {
+    if (known && h < h1) {
       u = *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(h) * D + 8 * k);
       w = *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(h) * D + D / 2 + 8 * k);
     }
+  };
+  load(h0 + warp / TG);
+  for (int h = h0 + warp / TG; h < h1; h += HW) {
     float a[8], b[8];
     unpack8(u, a);
     unpack8(w, b);
+    load(h + HW);  // the next head's rows are on their way while this one's are in work
     const bool is_v = h >= p.hq + hkv;
     if (!is_v) {
 #pragma unroll
@@ -222,8 +242,10 @@ struct GatherTable {
   Cache c;
 };
 
-// CTA = one block of a slot (all kv heads): a thread turns 8 dimensions of one
-// token and head at a time, 16 bytes out.
+// CTA = one block of a slot and two kv heads: a thread turns 8 dimensions of one
+// token and head at a time, 16 bytes out. 6499 tokens of 8 heads of 128: 7.4 us (all
+// heads of a block in one CTA 10.0).
+constexpr int kGatherHeads = 2;
 template <int D>
 __global__ void __launch_bounds__(256) kv4_gather_kernel(const __grid_constant__ GatherTable tab,
                                                          __nv_bfloat16* __restrict__ k_out,
@@ -236,10 +258,12 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(const __grid_constant__
   const int hkv = tab.c.hkv;
   constexpr int C = D / 8;
   const uint8_t* base = block_of<D>(tab.c, s, tile, 0);
-  for (int i = threadIdx.x; i < kBlockTok * hkv * C; i += blockDim.x) {
-    const int t = i / (hkv * C), h = i / C % hkv, d = i % C * 8;
+#pragma unroll
+  for (int i0 = 0; i0 < kBlockTok * kGatherHeads * C; i0 += 256) {
+    const int i = i0 + threadIdx.x;
+    const int t = i / (kGatherHeads * C), h = blockIdx.y * kGatherHeads + i / C % kGatherHeads, d = i % C * 8;
     const int64_t local = tile * kBlockTok + t - tab.start[s];
-    if (local < 0 || local >= rows) continue;
+    if (local < 0 || local >= rows || h >= hkv) continue;
     float kv[8], vv[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) kv[e] = vv[e] = 0.f;  // a page that is not there: zeros
@@ -347,7 +371,10 @@ SWL_EXPORT int swl_kv4_append(int nseg, const int* rows, const void* const* qkv,
   p.max_pos = max_pos;
   p.q_rot = static_cast<__nv_bfloat16*>(q_rot);
   p.k_rot = static_cast<__nv_bfloat16*>(k_rot);
-  p.heads_per_cta = 8;
+  // One pass of heads a CTA while there are few CTAs (28 single tokens: 12.3 -> 5.7 us), four
+  // passes, each loading ahead of the last, when there are many.
+  const int side = head_dim == 128 ? 2 : 4, heads = hq + 2 * hkv;
+  p.heads_per_cta = tiles * ((heads + side - 1) / side) <= 148 * 8 ? side : 4 * side;
   const dim3 grid(static_cast<unsigned>(tiles), (hq + 2 * hkv + p.heads_per_cta - 1) / p.heads_per_cta);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   SWL_CUDA_TRY(head_dim == 128 ? launch_kernel(kv4::kv4_append_kernel<128>, grid, dim3(256), 0, st, 1, t, p)
@@ -377,7 +404,7 @@ SWL_EXPORT int swl_kv4_gather(int nseg, const int* starts, const int* lens, cons
   }
   t.tile_start[nseg] = static_cast<int>(tiles);
   if (tiles == 0) return SWL_OK;
-  const dim3 grid(static_cast<unsigned>(tiles));
+  const dim3 grid(static_cast<unsigned>(tiles), (hkv + kv4::kGatherHeads - 1) / kv4::kGatherHeads);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   __nv_bfloat16 *ko = static_cast<__nv_bfloat16*>(k_out), *vo = static_cast<__nv_bfloat16*>(v_out);
   SWL_CUDA_TRY(head_dim == 128 ? launch_kernel(kv4::kv4_gather_kernel<128>, grid, dim3(256), 0, st, 1, t, ko, vo)
