@@ -483,6 +483,20 @@ int swl_paged_attention_kv4(int nseg, const int* rows, const void* const* block_
                             const void* const* caches, int64_t num_pages, const void* const* seqlens,
                             void* const* out, int64_t out_stride, int hq, int hkv, int head_dim, int page,
                             float scale, int max_len, const void* q_rot, float* part, void* stream);
+/* The same three calls for slots whose rows are packed one behind the other
+ * (qkv, out), whose block tables are rows of one array (table_stride entries
+ * apart), whose context lengths are one array and which share one cache. */
+int swl_kv4_append_packed(int nseg, const int* rows, const void* qkv, int64_t qkv_stride, const int* block_tables,
+                          int64_t table_stride, int table_len, void* cache, int64_t num_pages, const int* seqlens,
+                          int hq, int hkv, int head_dim, int page, const void* cos_sin, int max_pos, void* q_rot,
+                          void* k_rot, void* stream);
+int swl_kv4_gather_packed(int nseg, const int* starts, const int* lens, const int* block_tables,
+                          int64_t table_stride, int table_len, const void* cache, int64_t num_pages, int hkv,
+                          int head_dim, int page, void* k_out, void* v_out, void* stream);
+int swl_paged_attention_kv4_packed(int nseg, const int* rows, const int* block_tables, int64_t table_stride,
+                                   int table_len, const void* cache, int64_t num_pages, const int* seqlens,
+                                   void* out, int64_t out_stride, int hq, int hkv, int head_dim, int page,
+                                   float scale, int max_len, const void* q_rot, float* part, void* stream);
 /* LlamaRMSNorm (HF modeling_llama; worker_sync.py:1346, 1380, 1416). */
 int swl_rms_norm(int nseg, const int* rows, const void* const* x, int64_t x_stride,
                  void* const* out, int64_t out_stride, const void* w, int64_t hidden, float eps,

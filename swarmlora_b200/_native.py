@@ -143,6 +143,11 @@ SIGNATURES: dict[str, tuple] = {
     "swl_kv4_part_floats": (_i64, [_i32, _p, _i32, _i32, _i32, _i32]),
     "swl_paged_attention_kv4": (_i32, [_i32, _p, _p, _i32, _p, _i64, _p, _p, _i64, _i32, _i32, _i32, _i32, _f32, _i32, _p,
                                        _p, _p]),
+    "swl_kv4_append_packed": (_i32, [_i32, _p, _p, _i64, _p, _i64, _i32, _p, _i64, _p, _i32, _i32, _i32, _i32, _p, _i32, _p,
+                                     _p, _p]),
+    "swl_kv4_gather_packed": (_i32, [_i32, _p, _p, _p, _i64, _i32, _p, _i64, _i32, _i32, _i32, _p, _p, _p]),
+    "swl_paged_attention_kv4_packed": (_i32, [_i32, _p, _p, _i64, _i32, _p, _i64, _p, _p, _i64, _i32, _i32, _i32, _i32, _f32,
+                                              _i32, _p, _p, _p]),
     "swl_rms_norm": (_i32, [_i32, _pi32, _pp, _i64, _pp, _i64, _p, _i64, _f32, _p]),
     "swl_copy_rows": (_i32, [_i32, _pp, _pp, _pi64, _p]),
     "swl_paged_attention_shrink": (_i32, [_i32, _pi32, _pp, _pp, _pp, _pp, _pp, _i64, _i32, _i32, _i32,

@@ -74,6 +74,16 @@ int fill_cache(Cache* c, const char* what, int nseg, const void* const* block_ta
                void* const* caches, int64_t num_pages, const void* const* seqlens, int hkv, int head_dim, int page);
 // Row counts to row starts; the total is bounded so that row indices stay in 31 bits.
 int fill_rows(RowSegments* s, const char* what, int nseg, const int* rows);
+// The pointer tables of a call whose slots' rows lie in one array each: slot i's
+// block table, cache and context length, and rows from the row starts on.
+struct Packed {
+  const void* tables[kMaxSlots];
+  void* caches[kMaxSlots];
+  const void* lens[kMaxSlots];
+  void* rows[kMaxSlots];
+};
+int fill_packed(Packed* p, const char* what, int nseg, const int* rows, const void* base, int64_t row_stride,
+                const int* block_tables, int64_t table_stride, void* cache, const int* seqlens);
 // The attention kernel's bounded-wait status on the current device; synchronous.
 int read_and_clear_error(unsigned int* code);
 

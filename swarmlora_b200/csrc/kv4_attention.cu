@@ -811,3 +811,14 @@ SWL_EXPORT int swl_paged_attention_kv4(int nseg, const int* rows, const void* co
          : pl.nt == 1 ? kv4::launch_kv4<64, 1, false>(t, p, pl, st)
                       : kv4::launch_kv4<64, 2, false>(t, p, pl, st);
 }
+
+SWL_EXPORT int swl_paged_attention_kv4_packed(int nseg, const int* rows, const int* block_tables, int64_t table_stride,
+                                              int table_len, const void* cache, int64_t num_pages, const int* seqlens,
+                                              void* out, int64_t out_stride, int hq, int hkv, int head_dim, int page,
+                                              float scale, int max_len, const void* q_rot, float* part, void* stream) {
+  kv4::Packed t;
+  SWL_TRY(kv4::fill_packed(&t, "attention_kv4", nseg, rows, out, out_stride, block_tables, table_stride,
+                           const_cast<void*>(cache), seqlens));
+  return swl_paged_attention_kv4(nseg, rows, t.tables, table_len, t.caches, num_pages, t.lens, t.rows, out_stride, hq, hkv,
+                                 head_dim, page, scale, max_len, q_rot, part, stream);
+}

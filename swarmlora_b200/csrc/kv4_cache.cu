@@ -329,6 +329,21 @@ int fill_cache(Cache* c, const char* what, int nseg, const void* const* block_ta
   return SWL_OK;
 }
 
+int fill_packed(Packed* p, const char* what, int nseg, const int* rows, const void* base, int64_t row_stride,
+                const int* block_tables, int64_t table_stride, void* cache, const int* seqlens) {
+  if (nseg < 0 || nseg > kMaxSlots) return set_error(SWL_ERR_ARG, "%s: segment count %d outside 0..%d", what, nseg, kMaxSlots);
+  if (nseg > 0 && (!rows || !block_tables || !cache)) return set_error(SWL_ERR_ARG, "%s: null row counts, block tables or cache", what);
+  int64_t at = 0;
+  for (int i = 0; i < nseg; ++i) {
+    p->tables[i] = block_tables + i * table_stride;
+    p->caches[i] = cache;
+    p->lens[i] = seqlens ? seqlens + i : nullptr;
+    p->rows[i] = base ? const_cast<char*>(static_cast<const char*>(base)) + 2 * at * row_stride : nullptr;
+    at += std::max(rows[i], 0);
+  }
+  return SWL_OK;
+}
+
 }  // namespace kv4
 }  // namespace swl
 
@@ -410,4 +425,23 @@ SWL_EXPORT int swl_kv4_gather(int nseg, const int* starts, const int* lens, cons
   SWL_CUDA_TRY(head_dim == 128 ? launch_kernel(kv4::kv4_gather_kernel<128>, grid, dim3(256), 0, st, 1, t, ko, vo)
                                : launch_kernel(kv4::kv4_gather_kernel<64>, grid, dim3(256), 0, st, 1, t, ko, vo));
   return SWL_OK;
+}
+
+SWL_EXPORT int swl_kv4_append_packed(int nseg, const int* rows, const void* qkv, int64_t qkv_stride, const int* block_tables,
+                                     int64_t table_stride, int table_len, void* cache, int64_t num_pages, const int* seqlens,
+                                     int hq, int hkv, int head_dim, int page, const void* cos_sin, int max_pos, void* q_rot,
+                                     void* k_rot, void* stream) {
+  kv4::Packed t;
+  SWL_TRY(kv4::fill_packed(&t, "kv4_append", nseg, rows, qkv, qkv_stride, block_tables, table_stride, cache, seqlens));
+  return swl_kv4_append(nseg, rows, t.rows, qkv_stride, t.tables, table_len, t.caches, num_pages, t.lens, hq, hkv, head_dim,
+                        page, cos_sin, max_pos, q_rot, k_rot, stream);
+}
+
+SWL_EXPORT int swl_kv4_gather_packed(int nseg, const int* starts, const int* lens, const int* block_tables,
+                                     int64_t table_stride, int table_len, const void* cache, int64_t num_pages, int hkv,
+                                     int head_dim, int page, void* k_out, void* v_out, void* stream) {
+  kv4::Packed t;
+  SWL_TRY(kv4::fill_packed(&t, "kv4_gather", nseg, lens, nullptr, 0, block_tables, table_stride, const_cast<void*>(cache),
+                           nullptr));
+  return swl_kv4_gather(nseg, starts, lens, t.tables, table_len, t.caches, num_pages, hkv, head_dim, page, k_out, v_out, stream);
 }

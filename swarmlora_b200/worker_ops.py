@@ -280,7 +280,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_lens, 
     if total > q.shape[0] or sum(k_lens) > min(k.shape[0], v.shape[0]):
         raise ValueError("prompt_attention: the lengths add up to more rows than there are")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _bf16_rows("out", out, dev, hq, D)
         if total > out.shape[0]:
@@ -316,22 +316,37 @@ def kv4_cache(num_pages: int, hkv: int, head_dim: int = 128, page: int = 16, dev
                        device=device if device is not None else "cuda")
 
 
+def _check_slots(what: str, t: torch.Tensor, n: int, dtype, device, dims: int) -> int:
+    """One row per slot, contiguous inside; returns the rows' stride."""
+    st = t.stride()
+    if t.dtype is not dtype or t.device != device or len(st) != dims or t.size(0) != n or st[-1] != 1:
+        raise ValueError(f"{what}: {dtype} on {device}, one row per slot, contiguous inside")
+    return st[0]
+
+
 def _slot_rows(ts, n: int, what: str, dtype, size: int, device, first=None) -> array:
     """Addresses of each slot's rows (elements of `size` bytes): a list of tensors,
     or one tensor with a row per slot (first: the first row of each slot)."""
     if isinstance(ts, torch.Tensor):
-        st = ts.stride()
-        if ts.dtype is not dtype or ts.device != device or (len(st) > 1 and st[-1] != 1) or \
-                (first is None and ts.size(0) != n):
-            raise ValueError(f"{what}: {dtype} on {device}, one row per slot, contiguous inside")
-        base, by = ts.data_ptr(), size * st[0]
         if first is None:
-            return array("Q", range(base, base + n * by, by)) if by > 0 else array("Q", (base,)) * n
+            by = size * _check_slots(what, ts, n, dtype, device, ts.dim())
+            first = range(n)
+        else:
+            by = size * ts.stride(0)
+            if ts.dtype is not dtype or ts.device != device:
+                raise ValueError(f"{what}: {dtype} on {device} is needed")
+        base = ts.data_ptr()
         return array("Q", [base + i * by for i in first])
     if len(ts) != n or any(t.dtype is not dtype or t.device != device or
                            (t.dim() and t.numel() > 1 and t.stride(-1) != 1) for t in ts):
         raise ValueError(f"{what}: one {dtype} tensor per slot on {device}, contiguous inside")
     return array("Q", [t.data_ptr() for t in ts])
+
+
+def _kv4_check(cache: torch.Tensor, hkv: int, head_dim: int, page: int, device) -> None:
+    want = (page // 16, hkv, kv4_block_bytes(head_dim))
+    if cache.dtype is not torch.uint8 or cache.device != device or not cache.is_contiguous() or cache.shape[1:] != want:
+        raise ValueError(f"4-bit cache: contiguous uint8 [pages, {want[0]}, {want[1]}, {want[2]}] on {device} is needed")
 
 
 def _kv4_slots(block_tables, caches, n: int, hkv: int, head_dim: int, page: int, device):
@@ -343,20 +358,17 @@ def _kv4_slots(block_tables, caches, n: int, hkv: int, head_dim: int, page: int,
     else:
         table_len = min((t.shape[0] for t in block_tables), default=1)
     tables = _slot_rows(block_tables, n, "block tables", torch.int32, 4, device)
-    want = (page // 16, hkv, kv4_block_bytes(head_dim))
     if isinstance(caches, torch.Tensor):
-        _kv4_check(caches, want, device)
-        return tables, table_len, array("Q", (caches.data_ptr(),)) * n, caches.size(0)
-    for c in caches:
-        _kv4_check(c, want, device)
+        caches = [caches] * n
+    for c in {id(c): c for c in caches}.values():
+        _kv4_check(c, hkv, head_dim, page, device)
     if len(caches) != n:
         raise ValueError("4-bit cache: one for all slots, or one per slot")
     return tables, table_len, array("Q", [c.data_ptr() for c in caches]), min((c.size(0) for c in caches), default=1)
 
 
-def _kv4_check(cache: torch.Tensor, want: tuple, device) -> None:
-    if cache.dtype is not torch.uint8 or cache.device != device or not cache.is_contiguous() or cache.shape[1:] != want:
-        raise ValueError(f"4-bit cache: contiguous uint8 [pages, {want[0]}, {want[1]}, {want[2]}] on {device} is needed")
+def _all_packed(*tensors) -> bool:
+    return all(isinstance(t, torch.Tensor) for t in tensors)
 
 
 def _first_rows(rows) -> list:
@@ -407,14 +419,23 @@ def kv4_append(qkvs, block_tables, caches, seqlens, q_rot, cos_sin, hq: int, hkv
     if k_rot is not None:
         _packed("kv4_append: k_rot", k_rot, total, hkv * head_dim, dev)
     _packed("kv4_append: cos_sin", cos_sin, 1, head_dim, dev)
+    counts = _ints(rows)
+    tail = (hq, hkv, head_dim, page, cos_sin.data_ptr(), cos_sin.size(0), q_rot.data_ptr(),
+            k_rot.data_ptr() if k_rot is not None else None, _current(dev))
+    if n and _all_packed(qkvs, block_tables, caches, seqlens):  # no tables of addresses to make
+        if qkvs.dtype is not torch.bfloat16 or qkvs.device != dev or qkvs.stride(1) != 1:
+            raise ValueError(f"kv4_append: qkv: bf16 rows on {dev} are needed")
+        by = _check_slots("block tables", block_tables, n, torch.int32, dev, 2)
+        _check_slots("kv4_append: seqlens", seqlens, n, torch.int32, dev, 1)
+        _kv4_check(caches, hkv, head_dim, page, dev)
+        check(lib().swl_kv4_append_packed(n, _addr(counts), qkvs.data_ptr(), stride, block_tables.data_ptr(), by,
+                                          block_tables.size(1), caches.data_ptr(), caches.size(0), seqlens.data_ptr(), *tail))
+        return
     src = _slot_rows(qkvs, n, "kv4_append: qkv", torch.bfloat16, 2, dev, _first_rows(rows) if packed else None)
     tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, dev)
     lens = _slot_rows(seqlens, n, "kv4_append: seqlens", torch.int32, 4, dev)
-    counts = _ints(rows)
     check(lib().swl_kv4_append(n, _addr(counts), _addr(src), stride, _addr(tables), table_len, _addr(cache), pages,
-                               _addr(lens), hq, hkv, head_dim, page, cos_sin.data_ptr(), cos_sin.shape[0],
-                               q_rot.data_ptr(), k_rot.data_ptr() if k_rot is not None else None,
-                               _current(dev)))
+                               _addr(lens), *tail))
 
 
 def kv4_gather(block_tables, caches, starts, lens, k_out, v_out, hkv: int, head_dim: int = 128, page: int = 16,
@@ -431,10 +452,16 @@ def kv4_gather(block_tables, caches, starts, lens, k_out, v_out, hkv: int, head_
         raise ValueError("kv4_gather: one start per slot is needed")
     _packed("kv4_gather: k_out", k_out, total, hkv * head_dim, dev)
     _packed("kv4_gather: v_out", v_out, total, hkv * head_dim, dev)
-    tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, dev)
     begin, count = _ints(starts), _ints(lens)
-    check(lib().swl_kv4_gather(n, _addr(begin), _addr(count), _addr(tables), table_len, _addr(cache), pages, hkv, head_dim,
-                               page, k_out.data_ptr(), v_out.data_ptr(), _current(dev)))
+    tail = (hkv, head_dim, page, k_out.data_ptr(), v_out.data_ptr(), _current(dev))
+    if n and _all_packed(block_tables, caches):
+        by = _check_slots("block tables", block_tables, n, torch.int32, dev, 2)
+        _kv4_check(caches, hkv, head_dim, page, dev)
+        check(lib().swl_kv4_gather_packed(n, _addr(begin), _addr(count), block_tables.data_ptr(), by, block_tables.size(1),
+                                          caches.data_ptr(), caches.size(0), *tail))
+        return
+    tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, dev)
+    check(lib().swl_kv4_gather(n, _addr(begin), _addr(count), _addr(tables), table_len, _addr(cache), pages, *tail))
 
 
 def kv4_part_floats(rows, hq: int, hkv: int, max_len: int, head_dim: int = 128) -> int:
@@ -457,10 +484,6 @@ def paged_attention_kv4(rows, block_tables, caches, seqlens, outs, q_rot, hq: in
     n, total, width = len(rows), sum(rows), hq * head_dim
     _packed("paged_attention_kv4: q_rot", q_rot, total, width, dev)
     stride = _slots_of_rows("paged_attention_kv4: out", outs, rows, total, width)
-    first = _first_rows(rows) if isinstance(outs, torch.Tensor) else None
-    dst = _slot_rows(outs, n, "paged_attention_kv4: out", torch.bfloat16, 2, dev, first)
-    tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, dev)
-    lens = _slot_rows(seqlens, n, "paged_attention_kv4: seqlens", torch.int32, 4, dev)
     counts = _ints(rows)
     L = lib()
     need = L.swl_kv4_part_floats(n, _addr(counts), hq, hkv, head_dim, max_len)
@@ -469,10 +492,23 @@ def paged_attention_kv4(rows, block_tables, caches, seqlens, outs, q_rot, hq: in
             part = torch.empty(need, dtype=torch.float32, device=dev)
     elif part.dtype is not torch.float32 or part.device != dev or not part.is_contiguous() or part.numel() < need:
         raise ValueError(f"paged_attention_kv4: part needs {need} contiguous fp32 values on {dev}")
+    tail = (stride, hq, hkv, head_dim, page, float(scale), max_len, q_rot.data_ptr(),
+            part.data_ptr() if part is not None else None, _current(dev))
+    if n and _all_packed(block_tables, caches, seqlens, outs):
+        if outs.dtype is not torch.bfloat16 or outs.device != dev or outs.stride(1) != 1:
+            raise ValueError(f"paged_attention_kv4: out: bf16 rows on {dev} are needed")
+        by = _check_slots("block tables", block_tables, n, torch.int32, dev, 2)
+        _check_slots("paged_attention_kv4: seqlens", seqlens, n, torch.int32, dev, 1)
+        _kv4_check(caches, hkv, head_dim, page, dev)
+        check(L.swl_paged_attention_kv4_packed(n, _addr(counts), block_tables.data_ptr(), by, block_tables.size(1),
+                                               caches.data_ptr(), caches.size(0), seqlens.data_ptr(), outs.data_ptr(), *tail))
+        return
+    first = _first_rows(rows) if isinstance(outs, torch.Tensor) else None
+    dst = _slot_rows(outs, n, "paged_attention_kv4: out", torch.bfloat16, 2, dev, first)
+    tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, dev)
+    lens = _slot_rows(seqlens, n, "paged_attention_kv4: seqlens", torch.int32, 4, dev)
     check(L.swl_paged_attention_kv4(n, _addr(counts), _addr(tables), table_len, _addr(cache), pages, _addr(lens),
-                                    _addr(dst), stride, hq, hkv, head_dim, page, float(scale), max_len, q_rot.data_ptr(),
-                                    part.data_ptr() if part is not None else None,
-                                    _current(dev)))
+                                    _addr(dst), *tail))
 
 
 def rms_norm(xs, outs, w: torch.Tensor, eps: float, rows=None, x_stride: int | None = None,
