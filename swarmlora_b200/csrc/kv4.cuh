@@ -47,7 +47,15 @@ __device__ __forceinline__ int v_piece(int t, int d) {
 
 // What a launch over slots reads: slot i's block table (page ids), cache and
 // cached length. table_len entries per table and num_pages pages per cache bound every access.
+// Packed slots go by base and step: an entry of a table in the parameter space is
+// a cache miss of its own, several of them one behind the other at the start of every CTA.
 struct Cache {
+  int packed;                    // 1: table0, cache0, len0; 0: the tables
+  int rows_each;                 // new rows of every slot where all have as many, else 0
+  const int* table0;
+  int64_t table_step;
+  uint8_t* cache0;
+  const int* len0;
   const int* block_table[kMaxSlots];
   uint8_t* cache[kMaxSlots];
   const int* seqlen[kMaxSlots];  // device int: tokens cached before this step
@@ -57,33 +65,47 @@ struct Cache {
   int hkv;
 };
 
+__device__ __forceinline__ const int* table_of(const Cache& c, int s) {
+  return c.packed ? c.table0 + s * c.table_step : c.block_table[s];
+}
+__device__ __forceinline__ uint8_t* cache_of(const Cache& c, int s) { return c.packed ? c.cache0 : c.cache[s]; }
+__device__ __forceinline__ const int* len_of(const Cache& c, int s) { return c.packed ? c.len0 + s : c.seqlen[s]; }
+// First row of slot s.
+__device__ __forceinline__ int row_of(const Cache& c, const RowSegments& seg, int s) {
+  return c.rows_each ? s * c.rows_each : seg.row_start[s];
+}
+
 // The block of tile `tile` (tokens 16 tile ..) of head h, or nullptr where the
 // table has no such entry or names no page of the cache.
-template <int D>
+// kEither: the cache may be a packed one (the appending and gathering kernels always get tables:
+// the choice costs them registers that they are short of).
+template <int D, bool kEither = false>
 __device__ __forceinline__ uint8_t* block_of(const Cache& c, int s, int64_t tile, int h) {
   const int64_t pi = tile >> c.page_shift;
   if (tile < 0 || pi >= c.table_len) return nullptr;
-  const int64_t page = c.block_table[s][pi];
+  const int64_t page = (kEither ? table_of(c, s) : c.block_table[s])[pi];
   if (page < 0 || page >= c.num_pages) return nullptr;
   const int64_t sub = tile & ((int64_t{1} << c.page_shift) - 1);
-  return c.cache[s] + (((page << c.page_shift) + sub) * c.hkv + h) * block_bytes(D);
+  return (kEither ? cache_of(c, s) : c.cache[s]) + (((page << c.page_shift) + sub) * c.hkv + h) * block_bytes(D);
 }
 
-// Checks and fills the parts every entry point shares.
-int fill_cache(Cache* c, const char* what, int nseg, const void* const* block_tables, int table_len,
-               void* const* caches, int64_t num_pages, const void* const* seqlens, int hkv, int head_dim, int page);
+// The slots of a call as its caller gives them: tables of pointers, or packed (base and step).
+struct Slots {
+  const void* const* block_tables = nullptr;
+  void* const* caches = nullptr;
+  const void* const* seqlens = nullptr;
+  bool packed = false;
+  const int* table0 = nullptr;
+  int64_t table_step = 0;
+  void* cache0 = nullptr;
+  const int* len0 = nullptr;
+};
+// Checks and fills the parts every entry point shares. lens: whether the call reads context
+// lengths; keep: whether packed slots stay so (else they become tables).
+int fill_cache(Cache* c, const char* what, int nseg, const int* rows, const Slots& s, bool lens, bool keep, int table_len,
+               int64_t num_pages, int hkv, int head_dim, int page);
 // Row counts to row starts; the total is bounded so that row indices stay in 31 bits.
 int fill_rows(RowSegments* s, const char* what, int nseg, const int* rows);
-// The pointer tables of a call whose slots' rows lie in one array each: slot i's
-// block table, cache and context length, and rows from the row starts on.
-struct Packed {
-  const void* tables[kMaxSlots];
-  void* caches[kMaxSlots];
-  const void* lens[kMaxSlots];
-  void* rows[kMaxSlots];
-};
-int fill_packed(Packed* p, const char* what, int nseg, const int* rows, const void* base, int64_t row_stride,
-                const int* block_tables, int64_t table_stride, void* cache, const int* seqlens);
 // The attention kernel's bounded-wait status on the current device; synchronous.
 int read_and_clear_error(unsigned int* code);
 

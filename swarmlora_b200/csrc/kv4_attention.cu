@@ -51,6 +51,8 @@ constexpr int kWarps = 4;
 
 struct AttnTable4 {
   RowSegments seg;
+  int passes_each;               // column passes of every slot where all have as many rows
+  __nv_bfloat16* out0;           // packed rows, or nullptr
   __nv_bfloat16* out[kMaxSlots];
   Cache c;
 };
@@ -61,6 +63,7 @@ struct AttnParams4 {
   int max_len;
   const __nv_bfloat16* q;  // [total_rows, hq * D]
   int whole;               // 1: CTAs take whole pairs; 0: equal ranges
+  int pairs;               // (slot, kv head, pass)es in all
   float* part;             // equal ranges: O [record][column][D], then (m, l) [record][column][2]
 };
 
@@ -82,14 +85,14 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma16816_c(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                            uint32_t b1, float c0, float c1) {  // C: (c0, c1) in both halves of the rows
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
@@ -137,6 +140,12 @@ struct Piece {
   int slot, head, pass, b0, b1, blocks;
 };
 
+// Cache blocks of a slot's context with its new rows.
+__device__ __forceinline__ int blocks_of(const AttnTable4& tab, const AttnParams4& p, int s, int rows) {
+  const int64_t len = min(static_cast<int64_t>(*len_of(tab.c, s)) + rows, static_cast<int64_t>(p.max_len));
+  return static_cast<int>((max(len, int64_t{1}) + kBlockTok - 1) / kBlockTok);
+}
+
 template <int D, int NT>
 __device__ __forceinline__ void share_out(const AttnTable4& tab, const AttnParams4& p, Shares* sh, int ctas) {
   if (threadIdx.x < 32) {
@@ -146,10 +155,9 @@ __device__ __forceinline__ void share_out(const AttnTable4& tab, const AttnParam
       const int s = s0 + threadIdx.x;
       int nb = 0, np = 0;
       if (s < tab.seg.nseg) {
-        const int rows = tab.seg.row_start[s + 1] - tab.seg.row_start[s];
+        const int rows = row_of(tab.c, tab.seg, s + 1) - row_of(tab.c, tab.seg, s);
         if (rows > 0) {
-          const int64_t len = min(static_cast<int64_t>(*tab.c.seqlen[s]) + rows, static_cast<int64_t>(p.max_len));
-          nb = static_cast<int>((max(len, int64_t{1}) + kBlockTok - 1) / kBlockTok);
+          nb = blocks_of(tab, p, s, rows);
           np = (rows * p.group + 8 * NT - 1) / (8 * NT) * tab.c.hkv;
         }
         sh->blocks[s] = nb;
@@ -197,26 +205,36 @@ __device__ __forceinline__ int find_pair(const Shares& sh, int n, int pair) {
 // Walks the pieces of this CTA.
 struct Walk {
   int64_t u, end;  // equal ranges: next unit; whole pairs: next pair
-  int whole, step;
-  __device__ __forceinline__ Walk(const Shares& sh, int n, int whole_) : whole(whole_), step(gridDim.x) {
-    if (whole) {
+  __device__ __forceinline__ Walk(const Shares& sh, const AttnTable4& tab, const AttnParams4& p) {
+    if (p.whole) {
       u = blockIdx.x;
-      end = sh.pair[n];
+      end = p.pairs;
     } else {
-      u = min(blockIdx.x * sh.per_cta, sh.unit[n]);
-      end = min(u + sh.per_cta, sh.unit[n]);
+      u = min(blockIdx.x * sh.per_cta, sh.unit[tab.seg.nseg]);
+      end = min(u + sh.per_cta, sh.unit[tab.seg.nseg]);
     }
   }
-  __device__ __forceinline__ bool next(const Shares& sh, int n, Piece* x) {
+  __device__ __forceinline__ bool next(const Shares& sh, const AttnTable4& tab, const AttnParams4& p, Piece* x) {
     if (u >= end) return false;
-    if (whole) {
-      const int s = find_pair(sh, n, static_cast<int>(u)), i = static_cast<int>(u) - sh.pair[s];
-      x->slot = s;
-      x->head = i / sh.passes[s];
-      x->pass = i % sh.passes[s];
-      x->blocks = x->b1 = sh.blocks[s];
+    const int n = tab.seg.nseg;
+    if (p.whole) {
+      int i = static_cast<int>(u), passes;
+      if (tab.c.rows_each) {  // nothing to look up
+        passes = tab.passes_each;
+        x->slot = i / (passes * tab.c.hkv);
+        i -= x->slot * passes * tab.c.hkv;
+        x->blocks = blocks_of(tab, p, x->slot, tab.c.rows_each);
+      } else {
+        x->slot = find_pair(sh, n, i);
+        i -= sh.pair[x->slot];
+        passes = sh.passes[x->slot];
+        x->blocks = sh.blocks[x->slot];
+      }
+      x->head = i / passes;
+      x->pass = i % passes;
       x->b0 = 0;
-      u += step;
+      x->b1 = x->blocks;
+      u += gridDim.x;
       return true;
     }
     int lo = 0, hi = n - 1;
@@ -259,15 +277,35 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
     for (int i = 0; i < ST; ++i) ptx::mbar_init(&bars[warp][i], 1);
     ptx::fence_mbar_init();
   }
+  __syncwarp();  // a warp's barriers are its own
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
-  share_out<D, NT>(tab, p, &sh, gridDim.x);
-  const int nseg = tab.seg.nseg;
+  if (!p.whole || !tab.c.rows_each) share_out<D, NT>(tab, p, &sh, gridDim.x);
+
+  // A piece's queries are asked for before anything else of it: column g's dimensions 8 c .. of each 32.
+  uint4 uq[NT][W];
+  auto load_q = [&](const Piece& x) {
+    const int row0 = row_of(tab.c, tab.seg, x.slot), ncols = (row_of(tab.c, tab.seg, x.slot + 1) - row0) * p.group;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int col = x.pass * C::kCols + (kDual ? g & 3 : nt * 8 + g);
+      const __nv_bfloat16* src =
+          p.q + (static_cast<int64_t>(row0 + col / p.group) * p.hq + x.head * p.group + col % p.group) * D;
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        uq[nt][j] = col < ncols ? *reinterpret_cast<const uint4*>(src + 32 * j + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  Walk cw(sh, tab, p);
+  Piece x;
+  constexpr bool kAhead = NT == 1;  // two tiles of columns have no registers to spare for it
+  bool have = cw.next(sh, tab, p, &x);
+  if (have && kAhead) load_q(x);
 
   // ---- loads: this warp's pairs of blocks in the order in which it will use them ----
-  Walk lw(sh, nseg, p.whole);
+  Walk lw(sh, tab, p);
   Piece lp;
-  bool more = lw.next(sh, nseg, &lp);
+  bool more = lw.next(sh, tab, p, &lp);
   int lb = more ? lp.b0 + 2 * warp : 0;   // next block of the load piece that is not in the batch
   const uint8_t *addr0 = nullptr, *addr1 = nullptr;  // lane i: the batch's i-th pair (nullptr: no such block), which it fetches
   int batch = 0, taken = 0, issued = 0;
@@ -276,15 +314,15 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
     while (more && taken == batch) {      // the next up to 32 pairs of this warp
       const int left = lp.b1 > lb ? (lp.b1 - lb + 2 * kWarps - 1) / (2 * kWarps) : 0;
       if (left == 0) {
-        more = lw.next(sh, nseg, &lp);
+        more = lw.next(sh, tab, p, &lp);
         lb = lp.b0 + 2 * warp;
         continue;
       }
       batch = min(left, 32);
       taken = 0;
       const int b = lb + lane * 2 * kWarps;
-      addr0 = lane < batch ? block_of<D>(tab.c, lp.slot, b, lp.head) : nullptr;
-      addr1 = lane < batch && b + 1 < lp.b1 ? block_of<D>(tab.c, lp.slot, b + 1, lp.head) : nullptr;
+      addr0 = lane < batch ? block_of<D, true>(tab.c, lp.slot, b, lp.head) : nullptr;
+      addr1 = lane < batch && b + 1 < lp.b1 ? block_of<D, true>(tab.c, lp.slot, b + 1, lp.head) : nullptr;
       ok0 = __ballot_sync(0xffffffffu, addr0 != nullptr);
       ok1 = __ballot_sync(0xffffffffu, addr1 != nullptr);
       lb += batch * 2 * kWarps;
@@ -306,12 +344,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
 
   int used = 0;
   uint64_t limit = kWaitNs;  // after a wait that gave up the others give up soon
-  Walk cw(sh, nseg, p.whole);
-  Piece x;
-  while (cw.next(sh, nseg, &x)) {
-    const int row0 = tab.seg.row_start[x.slot], rows = tab.seg.row_start[x.slot + 1] - row0;
+  while (have) {
+    if (!kAhead) load_q(x);
+    const int row0 = row_of(tab.c, tab.seg, x.slot), rows = row_of(tab.c, tab.seg, x.slot + 1) - row0;
     const int ncols = rows * p.group, col0 = x.pass * C::kCols;
-    const int64_t len0 = *tab.c.seqlen[x.slot];
+    const int64_t len0 = *len_of(tab.c, x.slot);
     // ---- this piece's query columns: B fragments, sums per group, visible lengths ----
     uint32_t qb[NT][2 * W][2];
     float qs[NT][NG][2], qo[NT][NG][2];  // sum q, and -128 sum q
@@ -324,14 +361,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int col = col0 + (kDual ? g & 3 : nt * 8 + g);
-      const __nv_bfloat16* src =
-          p.q + (static_cast<int64_t>(row0 + col / p.group) * p.hq + x.head * p.group + col % p.group) * D;
       float part[NG];
 #pragma unroll
       for (int i = 0; i < NG; ++i) part[i] = 0.f;
 #pragma unroll
       for (int j = 0; j < W; ++j) {
-        const uint4 u = col < ncols ? *reinterpret_cast<const uint4*>(src + 32 * j + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
+        const uint4 u = uq[nt][j];
         qb[nt][2 * j][0] = __byte_perm(u.x, u.z, 0x5410);
         qb[nt][2 * j][1] = __byte_perm(u.x, u.z, 0x7632);
         qb[nt][2 * j + 1][0] = __byte_perm(u.y, u.w, 0x5410);
@@ -371,26 +406,32 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
       nm[nt][0] = nm[nt][1] = 0.f;
       l[nt][0] = l[nt][1] = 0.f;
     }
-    // Sums q v of one block and each group: tokens g, g + 8 and columns 2c, 2c + 1.
-    auto product = [&](const uint8_t* blk, float (&acc)[NT][NG][4]) {
-      uint32_t kw[2][W];
+    // Sums q v of N blocks (from blk on) and each group: tokens g, g + 8 and columns 2c, 2c + 1. The
+    // chains of dependent products (a group of a block each) take turns.
+    auto product = [&](const uint8_t* blk, auto& acc) {
+      constexpr int N = sizeof(acc) / sizeof(acc[0]);
+      uint32_t kw[N][2][W];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) lds<W>(blk + (h * 32 + lane) * W * 4, kw[h]);
-      // the accumulator starts at -128 sum q
+      for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int j = 0; j < W; ++j)
+        for (int h = 0; h < 2; ++h) lds<W>(blk + i * C::kBlock + (h * 32 + lane) * W * 4, kw[i][h]);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint32_t a0 = codes2(kw[0][j] >> (8 * e)), a1 = codes2(kw[1][j] >> (8 * e));
-          const uint32_t a2 = codes2(kw[0][j] >> (8 * e + 4)), a3 = codes2(kw[1][j] >> (8 * e + 4));
+      for (int step = 0; step < 4; ++step)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            if (j % 2 == 0 && e == 0)
-              mma16816_c(acc[nt][j / 2], a0, a1, a2, a3, qb[nt][2 * j][0], qb[nt][2 * j][1], qo[nt][j / 2][0], qo[nt][j / 2][1]);
-            else
-              mma16816(acc[nt][j / 2], a0, a1, a2, a3, qb[nt][2 * j + e][0], qb[nt][2 * j + e][1]);
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr) {
+            const int j = 2 * gr + step / 2, e = step & 1;
+            const uint32_t a0 = codes2(kw[i][0][j] >> (8 * e)), a1 = codes2(kw[i][1][j] >> (8 * e));
+            const uint32_t a2 = codes2(kw[i][0][j] >> (8 * e + 4)), a3 = codes2(kw[i][1][j] >> (8 * e + 4));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if (step == 0)  // the accumulator starts at -128 sum q
+                mma16816_c(acc[i][nt][gr], a0, a1, a2, a3, qb[nt][2 * j][0], qb[nt][2 * j][1], qo[nt][gr][0], qo[nt][gr][1]);
+              else
+                mma16816(acc[i][nt][gr], a0, a1, a2, a3, qb[nt][2 * j + e][0], qb[nt][2 * j + e][1]);
+            }
           }
-        }
     };
     // Their raw scores. edge: some column does not see all of the tokens (from tok0 on); a block
     // that is not there is seen by none.
@@ -502,16 +543,15 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
       float sc[2][NT][4];
       bool grow = false;
       if constexpr (kDual) {
-        float a0[NT][NG][4], a1[NT][NG][4];
-        product(blk, a0);
-        product(blk + C::kBlock, a1);
+        float acc[2][NT][NG][4];
+        product(blk, acc);
         const int mine = c >> 1, mine_g = g >> 2;  // the block of columns 2c, 2c + 1, and of column g
 #pragma unroll
         for (int i = 0; i < NG; ++i)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (mine) a0[0][i][k] = a1[0][i][k];
-        scores(blk + mine * C::kBlock, tok0 + mine * kBlockTok, there >> mine & 1u, a0, sc[0], edge);
+            if (mine) acc[0][0][i][k] = acc[1][0][i][k];
+        scores(blk + mine * C::kBlock, tok0 + mine * kBlockTok, there >> mine & 1u, acc[0], sc[0], edge);
 #pragma unroll
         for (int k = 0; k < 4; ++k) grow |= sc[0][0][k] > bar_[0][k & 1];
         if (__any_sync(0xffffffffu, grow)) rescale(sc, 1);
@@ -531,9 +571,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (there >> i & 1u) {
-            float acc[NT][NG][4];
+            float acc[1][NT][NG][4];
             product(blk + i * C::kBlock, acc);
-            scores(blk + i * C::kBlock, tok0 + i * kBlockTok, true, acc, sc[i], edge);
+            scores(blk + i * C::kBlock, tok0 + i * kBlockTok, true, acc[0], sc[i], edge);
           } else {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) sc[i][nt][0] = sc[i][nt][1] = sc[i][nt][2] = sc[i][nt][3] = -INFINITY;
@@ -629,7 +669,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
           uint2 w2;
           w2.x = pack_bf16x2(a.x * inv, a.y * inv);
           w2.y = pack_bf16x2(a.z * inv, a.w * inv);
-          *reinterpret_cast<uint2*>(tab.out[x.slot] + static_cast<int64_t>(col / p.group) * p.out_stride +
+          __nv_bfloat16* const out = tab.out0 ? tab.out0 + row0 * p.out_stride : tab.out[x.slot];
+          *reinterpret_cast<uint2*>(out + static_cast<int64_t>(col / p.group) * p.out_stride +
                                     (x.head * p.group + col % p.group) * D + d4) = w2;
         } else {
           const int64_t r = static_cast<int64_t>(rec) * C::kCols + nt * 8 + mc;
@@ -643,6 +684,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
       }
       __syncthreads();
     }
+    have = cw.next(sh, tab, p, &x);
+    if (have && kAhead) load_q(x);
   }
 }
 
@@ -652,9 +695,10 @@ __global__ void __launch_bounds__(kWarps * 32)
     kv4_join_kernel(const __grid_constant__ AttnTable4 tab, const __grid_constant__ AttnParams4 p, int ctas) {
   using C = Cfg4<D, NT>;
   __shared__ Shares sh;
+  // the context lengths were complete before the attention launch, which started this one only then
+  share_out<D, NT>(tab, p, &sh, ctas);
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
-  share_out<D, NT>(tab, p, &sh, ctas);
   const int pair = blockIdx.x, n = tab.seg.nseg;
   if (pair >= sh.pair[n]) return;
   const int s = find_pair(sh, n, pair), i = pair - sh.pair[s];
@@ -662,7 +706,8 @@ __global__ void __launch_bounds__(kWarps * 32)
   const int c0 = static_cast<int>(u0 / sh.per_cta), c1 = static_cast<int>((u1 - 1) / sh.per_cta);
   if (c0 == c1) return;  // written whole
   const int head = i / sh.passes[s], pass = i % sh.passes[s];
-  const int ncols = (tab.seg.row_start[s + 1] - tab.seg.row_start[s]) * p.group;
+  const int row0 = row_of(tab.c, tab.seg, s), ncols = (row_of(tab.c, tab.seg, s + 1) - row0) * p.group;
+  __nv_bfloat16* const out = tab.out0 ? tab.out0 + row0 * p.out_stride : tab.out[s];
   const float* mls = p.part + static_cast<int64_t>(2 * ctas) * C::kCols * D;
   for (int k = threadIdx.x; k < C::kCols * (D / 4); k += blockDim.x) {
     const int mc = k / (D / 4), d4 = k % (D / 4) * 4, col = pass * C::kCols + mc;
@@ -690,7 +735,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     uint2 w2;
     w2.x = pack_bf16x2(a.x * inv, a.y * inv);
     w2.y = pack_bf16x2(a.z * inv, a.w * inv);
-    *reinterpret_cast<uint2*>(tab.out[s] + static_cast<int64_t>(col / p.group) * p.out_stride +
+    *reinterpret_cast<uint2*>(out + static_cast<int64_t>(col / p.group) * p.out_stride +
                               (head * p.group + col % p.group) * D + d4) = w2;
   }
 }
@@ -766,30 +811,32 @@ SWL_EXPORT int64_t swl_kv4_part_floats(int nseg, const int* rows, int hq, int hk
   return pl.whole ? 0 : static_cast<int64_t>(2 * pl.ctas) * 8 * pl.nt * (head_dim + 2);
 }
 
-SWL_EXPORT int swl_paged_attention_kv4(int nseg, const int* rows, const void* const* block_tables, int table_len,
-                                       const void* const* caches, int64_t num_pages, const void* const* seqlens,
-                                       void* const* out, int64_t out_stride, int hq, int hkv, int head_dim, int page,
-                                       float scale, int max_len, const void* q_rot, float* part, void* stream) {
+namespace {
+
+// swl_paged_attention_kv4: out0 for packed rows, else a pointer per slot.
+int attention(int nseg, const int* rows, const kv4::Slots& slots, int table_len, int64_t num_pages, void* out0,
+              void* const* out, int64_t out_stride, int hq, int hkv, int head_dim, int page, float scale, int max_len,
+              const void* q_rot, float* part, void* stream) {
   kv4::AttnTable4 t;
   SWL_TRY(kv4::fill_rows(&t.seg, "attention_kv4", nseg, rows));
-  if (!seqlens && nseg > 0) return set_error(SWL_ERR_ARG, "attention_kv4: null context lengths");
-  SWL_TRY(kv4::fill_cache(&t.c, "attention_kv4", nseg, block_tables, table_len, const_cast<void* const*>(caches), num_pages,
-                          seqlens, hkv, head_dim, page));
+  SWL_TRY(kv4::fill_cache(&t.c, "attention_kv4", nseg, rows, slots, true, true, table_len, num_pages, hkv, head_dim, page));
   if (hq < 1 || hq > 4096 || hq % hkv) return set_error(SWL_ERR_ARG, "attention_kv4: query heads must be a multiple of kv heads");
   if (!(scale > 0.f) || !std::isfinite(scale)) return set_error(SWL_ERR_ARG, "attention_kv4: scale must be positive and finite");
   if (max_len < 1) return set_error(SWL_ERR_ARG, "attention_kv4: max_len must be positive");
   if (!q_rot || (reinterpret_cast<uintptr_t>(q_rot) & 15)) return set_error(SWL_ERR_ARG, "attention_kv4: q must be 16-byte aligned");
   if (out_stride < static_cast<int64_t>(hq) * head_dim || out_stride % 8)
     return set_error(SWL_ERR_ARG, "attention_kv4: output stride must hold all heads and be a multiple of 8");
-  if (nseg > 0 && !out) return set_error(SWL_ERR_ARG, "attention_kv4: null outputs");
-  for (int i = 0; i < nseg; ++i) {
+  if (nseg > 0 && !out && !out0) return set_error(SWL_ERR_ARG, "attention_kv4: null outputs");
+  t.out0 = static_cast<__nv_bfloat16*>(out0);
+  bool good = (reinterpret_cast<uintptr_t>(out0) & 15) == 0;
+  for (int i = 0; i < nseg && !out0; ++i) {
     t.out[i] = static_cast<__nv_bfloat16*>(out[i]);
-    if (!t.out[i] || (reinterpret_cast<uintptr_t>(t.out[i]) & 15))
-      return set_error(SWL_ERR_ARG, "attention_kv4: outputs must be 16-byte aligned");
+    good = good && t.out[i] && (reinterpret_cast<uintptr_t>(t.out[i]) & 15) == 0;
   }
+  if (!good) return set_error(SWL_ERR_ARG, "attention_kv4: outputs must be 16-byte aligned");
   if (t.seg.total_rows == 0) return SWL_OK;
-  const kv4::Plan4 pl = kv4::make_plan4(nseg, rows, hq, hkv, max_len);
   if (static_cast<int64_t>(t.seg.total_rows) * hq > (1 << 30)) return set_error(SWL_ERR_ARG, "attention_kv4: too many rows");
+  const kv4::Plan4 pl = kv4::make_plan4(nseg, rows, hq, hkv, max_len);
   if (!pl.whole && (!part || (reinterpret_cast<uintptr_t>(part) & 15)))
     return set_error(SWL_ERR_ARG, "attention_kv4: missing or unaligned scratch");
   kv4::AttnParams4 p;
@@ -801,7 +848,9 @@ SWL_EXPORT int swl_paged_attention_kv4(int nseg, const int* rows, const void* co
   p.max_len = max_len;
   p.q = static_cast<const __nv_bfloat16*>(q_rot);
   p.whole = pl.whole;
+  p.pairs = static_cast<int>(pl.pairs);
   p.part = part;
+  t.passes_each = (t.c.rows_each * p.group + 8 * pl.nt - 1) / (8 * pl.nt);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (head_dim == 128)
     return pl.dual      ? kv4::launch_kv4<128, 1, true>(t, p, pl, st)
@@ -812,13 +861,30 @@ SWL_EXPORT int swl_paged_attention_kv4(int nseg, const int* rows, const void* co
                       : kv4::launch_kv4<64, 2, false>(t, p, pl, st);
 }
 
+}  // namespace
+
+SWL_EXPORT int swl_paged_attention_kv4(int nseg, const int* rows, const void* const* block_tables, int table_len,
+                                       const void* const* caches, int64_t num_pages, const void* const* seqlens,
+                                       void* const* out, int64_t out_stride, int hq, int hkv, int head_dim, int page,
+                                       float scale, int max_len, const void* q_rot, float* part, void* stream) {
+  kv4::Slots s;
+  s.block_tables = block_tables;
+  s.caches = const_cast<void* const*>(caches);
+  s.seqlens = seqlens;
+  return attention(nseg, rows, s, table_len, num_pages, nullptr, out, out_stride, hq, hkv, head_dim, page, scale, max_len,
+                   q_rot, part, stream);
+}
+
 SWL_EXPORT int swl_paged_attention_kv4_packed(int nseg, const int* rows, const int* block_tables, int64_t table_stride,
                                               int table_len, const void* cache, int64_t num_pages, const int* seqlens,
                                               void* out, int64_t out_stride, int hq, int hkv, int head_dim, int page,
                                               float scale, int max_len, const void* q_rot, float* part, void* stream) {
-  kv4::Packed t;
-  SWL_TRY(kv4::fill_packed(&t, "attention_kv4", nseg, rows, out, out_stride, block_tables, table_stride,
-                           const_cast<void*>(cache), seqlens));
-  return swl_paged_attention_kv4(nseg, rows, t.tables, table_len, t.caches, num_pages, t.lens, t.rows, out_stride, hq, hkv,
-                                 head_dim, page, scale, max_len, q_rot, part, stream);
+  kv4::Slots s;
+  s.packed = true;
+  s.table0 = block_tables;
+  s.table_step = table_stride;
+  s.cache0 = const_cast<void*>(cache);
+  s.len0 = seqlens;
+  return attention(nseg, rows, s, table_len, num_pages, out, nullptr, out_stride, hq, hkv, head_dim, page, scale, max_len,
+                   q_rot, part, stream);
 }

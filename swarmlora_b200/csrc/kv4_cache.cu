@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(256, 4) kv4_append_kernel(const __grid_constan
       }
     const uint32_t pr[2] = {group_pair(lo[0], hi[0]), group_pair(lo[1], hi[1])};
     const uint32_t wa = codes8(a, pr[0]), wb = codes8(b, pr[1]);
-    uint8_t* blk = known ? block_of<D>(tab.c, s, tile, is_v ? h - p.hq - hkv : h - p.hq) : nullptr;
+    uint8_t* const blk = known ? block_of<D>(tab.c, s, tile, is_v ? h - p.hq - hkv : h - p.hq) : nullptr;
     if (!is_v) {
       if (blk) {
         *reinterpret_cast<uint32_t*>(blk + k_word<D>(t, 8 * k)) = wa;
@@ -304,73 +304,62 @@ int fill_rows(RowSegments* s, const char* what, int nseg, const int* rows) {
   return SWL_OK;
 }
 
-int fill_cache(Cache* c, const char* what, int nseg, const void* const* block_tables, int table_len,
-               void* const* caches, int64_t num_pages, const void* const* seqlens, int hkv, int head_dim, int page) {
+int fill_cache(Cache* c, const char* what, int nseg, const int* rows, const Slots& s, bool lens, bool keep, int table_len,
+               int64_t num_pages, int hkv, int head_dim, int page) {
   if (head_dim != 64 && head_dim != 128) return set_error(SWL_ERR_ARG, "%s: head_dim must be 64 or 128", what);
   if (hkv < 1 || hkv > 1024) return set_error(SWL_ERR_ARG, "%s: kv heads outside 1..1024", what);
   if (page < kBlockTok || page > 1024 || (page & (page - 1)))
     return set_error(SWL_ERR_ARG, "%s: page must be 16, 32, 64, .. 1024 tokens", what);
   if (table_len < 1 || num_pages < 1) return set_error(SWL_ERR_ARG, "%s: empty block table or cache", what);
-  if (nseg > 0 && (!block_tables || !caches)) return set_error(SWL_ERR_ARG, "%s: null block tables or caches", what);
   c->table_len = table_len;
   c->num_pages = num_pages;
   c->hkv = hkv;
   c->page_shift = 0;
   while ((kBlockTok << c->page_shift) < page) ++c->page_shift;
-  for (int i = 0; i < nseg; ++i) {
-    c->block_table[i] = static_cast<const int*>(block_tables[i]);
-    c->cache[i] = static_cast<uint8_t*>(caches[i]);
-    c->seqlen[i] = seqlens ? static_cast<const int*>(seqlens[i]) : nullptr;
-    if (!c->block_table[i] || !c->cache[i] || (seqlens && !c->seqlen[i]))
+  c->rows_each = nseg > 0 ? rows[0] : 0;
+  for (int i = 1; i < nseg; ++i)
+    if (rows[i] != rows[0]) c->rows_each = 0;
+  c->packed = s.packed && keep;
+  c->table0 = s.table0;
+  c->table_step = s.table_step;
+  c->cache0 = static_cast<uint8_t*>(s.cache0);
+  c->len0 = s.len0;
+  if (nseg == 0) return SWL_OK;
+  if (s.packed ? !s.table0 || !s.cache0 || (lens && !s.len0) : !s.block_tables || !s.caches || (lens && !s.seqlens))
+    return set_error(SWL_ERR_ARG, "%s: null block tables, caches or context lengths", what);
+  uintptr_t align = reinterpret_cast<uintptr_t>(s.cache0);
+  for (int i = 0; i < nseg && !c->packed; ++i) {
+    c->block_table[i] = s.packed ? s.table0 + i * s.table_step : static_cast<const int*>(s.block_tables[i]);
+    c->cache[i] = static_cast<uint8_t*>(s.packed ? s.cache0 : s.caches[i]);
+    c->seqlen[i] = !lens ? nullptr : s.packed ? s.len0 + i : static_cast<const int*>(s.seqlens[i]);
+    if (!c->block_table[i] || !c->cache[i] || (lens && !c->seqlen[i]))
       return set_error(SWL_ERR_ARG, "%s: null per-slot pointer", what);
-    if (reinterpret_cast<uintptr_t>(c->cache[i]) & 15)
-      return set_error(SWL_ERR_ARG, "%s: caches must be 16-byte aligned", what);
+    align |= reinterpret_cast<uintptr_t>(c->cache[i]);
   }
+  if (align & 15) return set_error(SWL_ERR_ARG, "%s: caches must be 16-byte aligned", what);
   return SWL_OK;
 }
 
-int fill_packed(Packed* p, const char* what, int nseg, const int* rows, const void* base, int64_t row_stride,
-                const int* block_tables, int64_t table_stride, void* cache, const int* seqlens) {
-  if (nseg < 0 || nseg > kMaxSlots) return set_error(SWL_ERR_ARG, "%s: segment count %d outside 0..%d", what, nseg, kMaxSlots);
-  if (nseg > 0 && (!rows || !block_tables || !cache)) return set_error(SWL_ERR_ARG, "%s: null row counts, block tables or cache", what);
-  int64_t at = 0;
-  for (int i = 0; i < nseg; ++i) {
-    p->tables[i] = block_tables + i * table_stride;
-    p->caches[i] = cache;
-    p->lens[i] = seqlens ? seqlens + i : nullptr;
-    p->rows[i] = base ? const_cast<char*>(static_cast<const char*>(base)) + 2 * at * row_stride : nullptr;
-    at += std::max(rows[i], 0);
-  }
-  return SWL_OK;
-}
+namespace {
 
-}  // namespace kv4
-}  // namespace swl
-
-using namespace swl;
-
-SWL_EXPORT int64_t swl_kv4_block_bytes(int head_dim) {
-  return head_dim == 64 || head_dim == 128 ? kv4::block_bytes(head_dim) : 0;
-}
-
-SWL_EXPORT int swl_kv4_append(int nseg, const int* rows, const void* const* qkv, int64_t qkv_stride,
-                              const void* const* block_tables, int table_len, void* const* caches,
-                              int64_t num_pages, const void* const* seqlens, int hq, int hkv, int head_dim,
-                              int page, const void* cos_sin, int max_pos, void* q_rot, void* k_rot,
-                              void* stream) {
-  kv4::AppendTable t;
-  SWL_TRY(kv4::fill_rows(&t.seg, "kv4_append", nseg, rows));
-  if (!seqlens && nseg > 0) return set_error(SWL_ERR_ARG, "kv4_append: null context lengths");
-  SWL_TRY(kv4::fill_cache(&t.c, "kv4_append", nseg, block_tables, table_len, caches, num_pages, seqlens, hkv, head_dim, page));
+// swl_kv4_append: qkv0 for packed rows, else a pointer per slot.
+int append(int nseg, const int* rows, const void* qkv0, const void* const* qkv, int64_t qkv_stride, const Slots& slots,
+           int table_len, int64_t num_pages, int hq, int hkv, int head_dim, int page, const void* cos_sin, int max_pos,
+           void* q_rot, void* k_rot, void* stream) {
+  AppendTable t;
+  SWL_TRY(fill_rows(&t.seg, "kv4_append", nseg, rows));
+  SWL_TRY(fill_cache(&t.c, "kv4_append", nseg, rows, slots, true, false, table_len, num_pages, hkv, head_dim, page));
   if (hq < 1 || hq > 4096) return set_error(SWL_ERR_ARG, "kv4_append: query heads outside 1..4096");
   if (max_pos < 1 || !cos_sin || !q_rot) return set_error(SWL_ERR_ARG, "kv4_append: null or empty cos/sin table, or null q_rot");
   if (qkv_stride < static_cast<int64_t>(hq + 2 * hkv) * head_dim || qkv_stride % 8)
     return set_error(SWL_ERR_ARG, "kv4_append: row stride must hold all heads and be a multiple of 8");
-  uintptr_t align = reinterpret_cast<uintptr_t>(cos_sin) | reinterpret_cast<uintptr_t>(q_rot) | reinterpret_cast<uintptr_t>(k_rot);
-  if (nseg > 0 && !qkv) return set_error(SWL_ERR_ARG, "kv4_append: null rows");
+  uintptr_t align = reinterpret_cast<uintptr_t>(cos_sin) | reinterpret_cast<uintptr_t>(q_rot) |
+                    reinterpret_cast<uintptr_t>(k_rot) | reinterpret_cast<uintptr_t>(qkv0);
+  if (nseg > 0 && !qkv && !qkv0) return set_error(SWL_ERR_ARG, "kv4_append: null rows");
   int64_t tiles = 0;
   for (int i = 0; i < nseg; ++i) {
-    t.qkv[i] = static_cast<const __nv_bfloat16*>(qkv[i]);
+    t.qkv[i] = qkv0 ? static_cast<const __nv_bfloat16*>(qkv0) + t.seg.row_start[i] * qkv_stride
+                    : static_cast<const __nv_bfloat16*>(qkv[i]);
     if (!t.qkv[i]) return set_error(SWL_ERR_ARG, "kv4_append: null per-slot pointer");
     align |= reinterpret_cast<uintptr_t>(t.qkv[i]);
     t.tile_start[i] = static_cast<int>(tiles);
@@ -379,7 +368,7 @@ SWL_EXPORT int swl_kv4_append(int nseg, const int* rows, const void* const* qkv,
   t.tile_start[nseg] = static_cast<int>(tiles);
   if (align & 15) return set_error(SWL_ERR_ARG, "kv4_append: rows, cos/sin table and outputs must be 16-byte aligned");
   if (tiles == 0) return SWL_OK;
-  kv4::AppendParams p;
+  AppendParams p;
   p.hq = hq;
   p.qkv_stride = qkv_stride;
   p.cos_sin = static_cast<const __nv_bfloat16*>(cos_sin);
@@ -390,20 +379,18 @@ SWL_EXPORT int swl_kv4_append(int nseg, const int* rows, const void* const* qkv,
   // passes, each loading ahead of the last, when there are many.
   const int side = head_dim == 128 ? 2 : 4, heads = hq + 2 * hkv;
   p.heads_per_cta = tiles * ((heads + side - 1) / side) <= 148 * 8 ? side : 4 * side;
-  const dim3 grid(static_cast<unsigned>(tiles), (hq + 2 * hkv + p.heads_per_cta - 1) / p.heads_per_cta);
+  const dim3 grid(static_cast<unsigned>(tiles), (heads + p.heads_per_cta - 1) / p.heads_per_cta);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  SWL_CUDA_TRY(head_dim == 128 ? launch_kernel(kv4::kv4_append_kernel<128>, grid, dim3(256), 0, st, 1, t, p)
-                               : launch_kernel(kv4::kv4_append_kernel<64>, grid, dim3(256), 0, st, 1, t, p));
+  SWL_CUDA_TRY(head_dim == 128 ? launch_kernel(kv4_append_kernel<128>, grid, dim3(256), 0, st, 1, t, p)
+                               : launch_kernel(kv4_append_kernel<64>, grid, dim3(256), 0, st, 1, t, p));
   return SWL_OK;
 }
 
-SWL_EXPORT int swl_kv4_gather(int nseg, const int* starts, const int* lens, const void* const* block_tables,
-                              int table_len, const void* const* caches, int64_t num_pages, int hkv,
-                              int head_dim, int page, void* k_out, void* v_out, void* stream) {
-  kv4::GatherTable t;
-  SWL_TRY(kv4::fill_rows(&t.seg, "kv4_gather", nseg, lens));
-  SWL_TRY(kv4::fill_cache(&t.c, "kv4_gather", nseg, block_tables, table_len, const_cast<void* const*>(caches), num_pages,
-                          nullptr, hkv, head_dim, page));
+int gather(int nseg, const int* starts, const int* lens, const Slots& slots, int table_len, int64_t num_pages, int hkv,
+           int head_dim, int page, void* k_out, void* v_out, void* stream) {
+  GatherTable t;
+  SWL_TRY(fill_rows(&t.seg, "kv4_gather", nseg, lens));
+  SWL_TRY(fill_cache(&t.c, "kv4_gather", nseg, lens, slots, false, false, table_len, num_pages, hkv, head_dim, page));
   if (nseg > 0 && !starts) return set_error(SWL_ERR_ARG, "kv4_gather: null starts");
   if (!k_out || !v_out || ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15))
     return set_error(SWL_ERR_ARG, "kv4_gather: outputs must be 16-byte aligned");
@@ -419,29 +406,67 @@ SWL_EXPORT int swl_kv4_gather(int nseg, const int* starts, const int* lens, cons
   }
   t.tile_start[nseg] = static_cast<int>(tiles);
   if (tiles == 0) return SWL_OK;
-  const dim3 grid(static_cast<unsigned>(tiles), (hkv + kv4::kGatherHeads - 1) / kv4::kGatherHeads);
+  const dim3 grid(static_cast<unsigned>(tiles), (hkv + kGatherHeads - 1) / kGatherHeads);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   __nv_bfloat16 *ko = static_cast<__nv_bfloat16*>(k_out), *vo = static_cast<__nv_bfloat16*>(v_out);
-  SWL_CUDA_TRY(head_dim == 128 ? launch_kernel(kv4::kv4_gather_kernel<128>, grid, dim3(256), 0, st, 1, t, ko, vo)
-                               : launch_kernel(kv4::kv4_gather_kernel<64>, grid, dim3(256), 0, st, 1, t, ko, vo));
+  SWL_CUDA_TRY(head_dim == 128 ? launch_kernel(kv4_gather_kernel<128>, grid, dim3(256), 0, st, 1, t, ko, vo)
+                               : launch_kernel(kv4_gather_kernel<64>, grid, dim3(256), 0, st, 1, t, ko, vo));
   return SWL_OK;
+}
+
+}  // namespace
+}  // namespace kv4
+}  // namespace swl
+
+using namespace swl;
+
+SWL_EXPORT int64_t swl_kv4_block_bytes(int head_dim) {
+  return head_dim == 64 || head_dim == 128 ? kv4::block_bytes(head_dim) : 0;
+}
+
+SWL_EXPORT int swl_kv4_append(int nseg, const int* rows, const void* const* qkv, int64_t qkv_stride,
+                              const void* const* block_tables, int table_len, void* const* caches,
+                              int64_t num_pages, const void* const* seqlens, int hq, int hkv, int head_dim,
+                              int page, const void* cos_sin, int max_pos, void* q_rot, void* k_rot,
+                              void* stream) {
+  kv4::Slots s;
+  s.block_tables = block_tables;
+  s.caches = caches;
+  s.seqlens = seqlens;
+  return kv4::append(nseg, rows, nullptr, qkv, qkv_stride, s, table_len, num_pages, hq, hkv, head_dim, page, cos_sin, max_pos,
+                     q_rot, k_rot, stream);
 }
 
 SWL_EXPORT int swl_kv4_append_packed(int nseg, const int* rows, const void* qkv, int64_t qkv_stride, const int* block_tables,
                                      int64_t table_stride, int table_len, void* cache, int64_t num_pages, const int* seqlens,
                                      int hq, int hkv, int head_dim, int page, const void* cos_sin, int max_pos, void* q_rot,
                                      void* k_rot, void* stream) {
-  kv4::Packed t;
-  SWL_TRY(kv4::fill_packed(&t, "kv4_append", nseg, rows, qkv, qkv_stride, block_tables, table_stride, cache, seqlens));
-  return swl_kv4_append(nseg, rows, t.rows, qkv_stride, t.tables, table_len, t.caches, num_pages, t.lens, hq, hkv, head_dim,
-                        page, cos_sin, max_pos, q_rot, k_rot, stream);
+  kv4::Slots s;
+  s.packed = true;
+  s.table0 = block_tables;
+  s.table_step = table_stride;
+  s.cache0 = cache;
+  s.len0 = seqlens;
+  return kv4::append(nseg, rows, qkv, nullptr, qkv_stride, s, table_len, num_pages, hq, hkv, head_dim, page, cos_sin, max_pos,
+                     q_rot, k_rot, stream);
+}
+
+SWL_EXPORT int swl_kv4_gather(int nseg, const int* starts, const int* lens, const void* const* block_tables,
+                              int table_len, const void* const* caches, int64_t num_pages, int hkv,
+                              int head_dim, int page, void* k_out, void* v_out, void* stream) {
+  kv4::Slots s;
+  s.block_tables = block_tables;
+  s.caches = const_cast<void* const*>(caches);
+  return kv4::gather(nseg, starts, lens, s, table_len, num_pages, hkv, head_dim, page, k_out, v_out, stream);
 }
 
 SWL_EXPORT int swl_kv4_gather_packed(int nseg, const int* starts, const int* lens, const int* block_tables,
                                      int64_t table_stride, int table_len, const void* cache, int64_t num_pages, int hkv,
                                      int head_dim, int page, void* k_out, void* v_out, void* stream) {
-  kv4::Packed t;
-  SWL_TRY(kv4::fill_packed(&t, "kv4_gather", nseg, lens, nullptr, 0, block_tables, table_stride, const_cast<void*>(cache),
-                           nullptr));
-  return swl_kv4_gather(nseg, starts, lens, t.tables, table_len, t.caches, num_pages, hkv, head_dim, page, k_out, v_out, stream);
+  kv4::Slots s;
+  s.packed = true;
+  s.table0 = block_tables;
+  s.table_step = table_stride;
+  s.cache0 = const_cast<void*>(cache);
+  return kv4::gather(nseg, starts, lens, s, table_len, num_pages, hkv, head_dim, page, k_out, v_out, stream);
 }
