@@ -14,8 +14,6 @@
 // way between two codes goes to the even one.
 #include <cuda_bf16.h>
 
-#include <algorithm>
-
 #include "common.h"
 #include "kv4.cuh"
 #include "launch.h"

@@ -37,7 +37,6 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
-#include <cstring>
 
 #include "common.h"
 #include "kv4.cuh"
@@ -319,8 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int klen = tab.k_len[it.seq];
         for (int j = 0; j < it.nk && ok; ++j, ++tiles) {
           // every tile's barrier is waited for and released, so that it never runs two phases ahead
-          ok = ptx::mbar_wait(&v_full[tiles % ST], (tiles / ST) & 1, err, kErrTma, kWaitNs);
-          __syncwarp();
+          ok = __all_sync(0xffffffffu, ptx::mbar_wait(&v_full[tiles % ST], (tiles / ST) & 1, err, kErrTma, kWaitNs));
           if (ok && j < it.clean && lane == 0) ptx::mbar_arrive(&v_empty[tiles % ST]);
           if (!ok || j < it.clean) continue;
           uint4* const v = reinterpret_cast<uint4*>(v_ring + (tiles % ST) * C::kTileBytes);
@@ -361,7 +359,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           ++looked;
         }
-        ok = __all_sync(0xffffffffu, ok);
         ++busy;
       }
     } else if (lane == 0) {
@@ -486,9 +483,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int whole = max(0, it.first[x]) / kTile - it.kb;  // tiles before this one need no mask
       float m = -INFINITY, l = 0.f;  // reference (scaled, base 2) and sum of weights
       for (int j = 0; j < n; ++j, ++sn) {
-        ok = ptx::mbar_wait(&s_full[x], sn & 1, err, kErrSoftmax, kWaitNs);
+        // (the warp's lanes go on or give up together)
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&s_full[x], sn & 1, err, kErrSoftmax, kWaitNs));
         if (!ok) break;
-        __syncwarp();
         ptx::tc_fence_after();
         uint32_t s[4][32];
 #pragma unroll
@@ -559,10 +556,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t o[D / 32][32];
       bool fix = false;
       if (n > 0) {
-        ok = ptx::mbar_wait(&o_full[x], on & 1, err, kErrSoftmax, kWaitNs);
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&o_full[x], on & 1, err, kErrSoftmax, kWaitNs));
         if (!ok) break;
         ++on;
-        __syncwarp();
         ptx::tc_fence_after();
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) ptx::tmem_ld_32x32b_x32(to + c * 32, o[c]);
@@ -595,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (p.splits > 1) {
-        if (!real) continue;
+        if (!real) continue;  // (joined again by the next item's first warp-wide wait)
         const int64_t rec = (grow * p.hq + head) * p.splits + it.split;
         float* ml = p.part + p.part_rows * D + rec * 2;
         ml[0] = n > 0 ? m : -INFINITY;

@@ -84,6 +84,28 @@ def test_kv4_call_refuses_its_own(native, call, bad, word):
     assert st != 0 and word in msg, (st, msg)
 
 
+@pytest.mark.parametrize("bad,word", [
+    (dict(d=96), "head_dim"), (dict(page=24), "page"), (dict(bt=None), "null"), (dict(cache=None), "null"),
+    (dict(cache=F + 8), "aligned"), (dict(rows=(-1,)), "negative"), (dict(table_len=0), "empty"), (dict(pages=0), "empty"),
+    (dict(rows=(1,) * 129), "segment count"), (dict(seqlen=None), "null")])
+def test_packed_kv4_calls_refuse(native, bad, word):
+    a = dict(rows=(1,), d=128, page=16, table_len=4, pages=8, bt=F, cache=F, seqlen=F) | bad
+    lib, n, rows = native.lib(), len(a["rows"]), native.i32_array(a["rows"])
+    calls = [lib.swl_kv4_append_packed(n, rows, F, 1024, a["bt"], 4, a["table_len"], a["cache"], a["pages"], a["seqlen"], 4, 2,
+                                       a["d"], a["page"], F, 64, F, None, None), native.last_error(),
+             lib.swl_paged_attention_kv4_packed(n, rows, a["bt"], 4, a["table_len"], a["cache"], a["pages"], a["seqlen"], F, 512,
+                                                4, 2, a["d"], a["page"], 0.1, 64, F, None, None), native.last_error()]
+    if "seqlen" not in bad:
+        calls += [lib.swl_kv4_gather_packed(n, native.i32_array([0] * n), rows, a["bt"], 4, a["table_len"], a["cache"],
+                                            a["pages"], 2, a["d"], a["page"], F, F, None), native.last_error()]
+    for st, msg in zip(calls[::2], calls[1::2]):
+        assert st != 0 and word in msg, (st, msg)
+
+
+def test_error_word_needs_a_place(native):
+    assert native.lib().swl_attention_device_error(None) != 0 and "null" in native.last_error()
+
+
 @pytest.mark.parametrize("call", ["append", "gather", "attention"])
 def test_kv4_calls_of_nothing_are_done(native, call):
     assert _kv4(native, call, rows=(0, 0), starts=(0, 64))[0] == 0

@@ -459,3 +459,130 @@ def test_a_prompt_goes_through_all_of_them(native, cuda):
             _near(out[i].reshape(1, hq, d), ref.attend_fast(x, k, v, scale),
                   ref.attend_fast(x, k, v.abs() + 8.0, scale), f"token {t} of slot {i}")
         lens += 1
+
+
+# ---- strides, streams and far offsets ------------------------------------------------------------
+def test_prompt_rows_with_strides(native, cuda):
+    """q, k, v and out as row-strided views; what lies between the rows is left alone."""
+    from swarmlora_b200 import worker_ops as wo
+    g = _gen(cuda, 50)
+    lens = [70, 5, 131]
+    T, hq, hkv, d = sum(lens), 8, 2, 128
+
+    def view(heads):
+        return _randn(g, T, heads * d + 64)[:, 8:8 + heads * d].unflatten(-1, (heads, d))
+    q, k, v = view(hq), view(hkv), view(hkv)
+    wide = torch.full((T, hq * d + 128), 7.0, dtype=BF, device=cuda)
+    out = wide[:, 64:64 + hq * d].unflatten(-1, (hq, d))
+    wo.prompt_attention(q, k, v, lens, out=out)
+    assert torch.equal(out, wo.prompt_attention(q.contiguous(), k.contiguous(), v.contiguous(), lens))
+    assert bool((wide[:, :64] == 7.0).all()) and bool((wide[:, 64 + hq * d:] == 7.0).all())
+
+
+def test_calls_on_two_streams_at_once(native, cuda):
+    """Overlapping calls, each with its own scratch, give what they give alone."""
+    from swarmlora_b200 import worker_ops as wo
+    g = _gen(cuda, 51)
+    hq, hkv, d, n = 8, 2, 128, 3
+    tables = _tables(g, n, 130)
+    cache = wo.kv4_cache(n * 130 + 2, hkv, d, device=cuda)
+    for i in range(n):
+        ref.write_cache(cache, tables[i], torch.arange(2000, device=cuda),
+                        *(_randn(g, 2000, hkv, d, dtype=torch.float32) for _ in range(2)))
+    lens = torch.tensor([1990, 700, 3], dtype=torch.int32, device=cuda)
+    qs = [_randn(g, n, hq * d) for _ in range(2)]
+    pq, pk, pv = _randn(g, 40, hq, d), _randn(g, 3000, hkv, d), _randn(g, 3000, hkv, d)
+
+    def work(q, out):
+        wo.paged_attention_kv4([1] * n, tables, cache, lens, out, q, hq, hkv, 2048, 0.1)
+        return wo.prompt_attention(pq, pk, pv, [40], [3000])
+    want = []
+    for q in qs:
+        o = torch.empty(n, hq * d, dtype=BF, device=cuda)
+        want.append((o, work(q, o)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    got = [torch.empty(n, hq * d, dtype=BF, device=cuda) for _ in qs]
+    prompts = [None, None]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                prompts[i] = work(qs[i], got[i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(got[i], want[i][0]) and torch.equal(prompts[i], want[i][1])
+
+
+def test_two_graphs_with_their_own_scratch(native, cuda):
+    """Attention that needs scratch, captured twice with the scratch left to the call: replays in
+    either order and on both streams do not meet."""
+    from swarmlora_b200 import worker_ops as wo
+    g = _gen(cuda, 52)
+    hq, hkv, d = 8, 2, 128
+    tables = _tables(g, 1, 300)
+    cache = wo.kv4_cache(302, hkv, d, device=cuda)
+    ref.write_cache(cache, tables[0], torch.arange(4700, device=cuda),
+                    *(_randn(g, 4700, hkv, d, dtype=torch.float32) for _ in range(2)))
+    lens = [torch.tensor([n], dtype=torch.int32, device=cuda) for n in (4600, 3100)]
+    q = _randn(g, 1, hq * d)
+    assert wo.kv4_part_floats([1], hq, hkv, 4800) > 0
+    want, outs, graphs, streams = [], [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for n, s in zip(lens, streams):
+        w, o = (torch.empty(1, hq * d, dtype=BF, device=cuda) for _ in range(2))
+        wo.paged_attention_kv4([1], tables, cache, n, w, q, hq, hkv, 4800, 0.1)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            wo.paged_attention_kv4([1], tables, cache, n, o, q, hq, hkv, 4800, 0.1)
+        want.append(w)
+        outs.append(o)
+        graphs.append(graph)
+    for _ in range(10):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, outs))
+
+
+def test_pages_and_rows_beyond_32_bit_offsets(native, cuda):
+    """A cache of 5.5 GB whose last pages are used, and prompt rows more than 2^31 elements
+    into their tensor."""
+    from swarmlora_b200 import worker_ops as wo
+    g = _gen(cuda, 53)
+    hq, hkv, d, pages = 8, 8, 128, 300_000
+    cache = torch.empty(pages, 1, hkv, 18 * d, dtype=torch.uint8, device=cuda)
+    small = wo.kv4_cache(4, hkv, d, device=cuda)
+    far = torch.tensor([[pages - 1, pages - 3, pages // 2 + 1, 0]], dtype=torch.int32, device=cuda)
+    near = torch.tensor([[0, 1, 2, 3]], dtype=torch.int32, device=cuda)
+    cache[far[0].long()] = 0
+    lens, cs = torch.zeros(1, dtype=torch.int32, device=cuda), _cos_sin(64, d, cuda)
+    qkv = _randn(g, 60, (hq + 2 * hkv) * d)
+    res = []
+    for c, t in ((cache, far), (small, near)):
+        q_rot = torch.empty(60, hq * d, dtype=BF, device=cuda)
+        k, v = (torch.empty(60, hkv, d, dtype=BF, device=cuda) for _ in range(2))
+        out = torch.empty(2, hq * d, dtype=BF, device=cuda)
+        wo.kv4_append(qkv, t, c, lens, q_rot, cs, hq, hkv, rows=[60])
+        wo.kv4_gather(t, c, [0], [60], k, v, hkv)
+        wo.paged_attention_kv4([2], t, c, lens + 58, out, q_rot[:2].contiguous(), hq, hkv, 64, 0.1)
+        res.append((q_rot, k, v, out))
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+    del cache
+    rows, stride = 2200, 1 << 20
+    big = torch.empty(rows, stride, dtype=BF, device=cuda)
+    k, v = (big[:, o:o + 2 * d].unflatten(-1, (2, d)) for o in (0, 4096))
+    for t in (k, v):
+        t.copy_(_randn(g, rows, 2, d))
+    q = _randn(g, 90, 4, d)
+    got = wo.prompt_attention(q, k, v, [30, 60], [200, 2000])
+    assert torch.equal(got, wo.prompt_attention(q, k.contiguous(), v.contiguous(), [30, 60], [200, 2000]))
+
+
+def test_no_wait_ran_out(native, cuda):
+    """The bounded-wait status after this file's launches (it is cleared by reading)."""
+    import ctypes as C
+    torch.cuda.synchronize()
+    code = C.c_uint(7)
+    native.check(native.lib().swl_attention_device_error(C.byref(code)))
+    assert code.value == 0
