@@ -18,8 +18,9 @@
 //   warps 9, 10      issue the products of row tile 0 and 1 (one lane); 9 owns the tensor memory
 //   warp 11          looks over the V tiles of the masked range (below)
 //
-// A CTA stays and takes one item after the other: the copies and score products
-// of the next item run while the rows of the last one are written.
+// A CTA stays and takes one item after the other, the next of the list whenever it is
+// free: the copies and score products of the next item run while the rows of the last
+// one are written.
 //
 // O is rescaled only when a row's maximum passes its reference by more than
 // 2^8 (then by the softmax warps themselves, which have just seen the MMA
@@ -112,13 +113,18 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
 }
 
 // One unit of a CTA's work: a block of queries of one sequence and kv head, over a range of its keys.
-struct Item {
-  int seq, head, split;
-  int t0[2], nt[2];   // first token and token count of each tile (0: no rows)
-  int first[2];       // keys the first row of a tile sees (may be negative)
-  int kb;             // first key tile
-  int n[2], nk;       // key tiles of each row tile, and of the item
-  int clean;          // key tiles of the item from this one on hold keys that some row does not see
+struct ItemTile {
+  int t0, nt;  // first token and token count (0: no rows)
+  int first;   // keys the first row sees (may be negative)
+  int n;       // key tiles
+};
+struct __align__(16) Item {
+  ItemTile tile[2];
+  int head, split;
+  int kb, nk;           // first key tile, key tiles
+  int clean;            // key tiles of the item from this one on hold keys that some row does not see
+  int q_row, k_row;     // first rows of the sequence
+  int k_len;
 };
 
 __device__ __forceinline__ Item find_item(const PromptTable& t, const PromptParams& p, int i) {
@@ -133,44 +139,79 @@ __device__ __forceinline__ Item find_item(const PromptTable& t, const PromptPara
     if (t.item_start[mid] <= i) lo = mid;
     else hi = mid - 1;
   }
-  it.seq = lo;
   // the last block of a sequence has the most keys: it goes first
   const int block = t.item_start[lo + 1] - 1 - i;
   const int ql = t.q_len[lo], kl = t.k_len[lo];
+  it.q_row = t.q_start[lo];
+  it.k_row = t.k_start[lo];
+  it.k_len = kl;
   int n[2];
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    it.t0[x] = (2 * block + x) * p.tokens;
-    it.nt[x] = max(0, min(p.tokens, ql - it.t0[x]));
-    it.first[x] = it.t0[x] + kl - ql + 1;
-    const int last = min(kl, it.first[x] + it.nt[x] - 1);
-    n[x] = it.nt[x] > 0 ? (max(0, last) + kTile - 1) / kTile : 0;
+    ItemTile& tl = it.tile[x];
+    tl.t0 = (2 * block + x) * p.tokens;
+    tl.nt = max(0, min(p.tokens, ql - tl.t0));
+    tl.first = tl.t0 + kl - ql + 1;
+    const int last = min(kl, tl.first + tl.nt - 1);
+    n[x] = tl.nt > 0 ? (max(0, last) + kTile - 1) / kTile : 0;
   }
   const int all = max(n[0], n[1]);
   it.kb = static_cast<int>(static_cast<int64_t>(all) * it.split / p.splits);
   const int ke = static_cast<int>(static_cast<int64_t>(all) * (it.split + 1) / p.splits);
 #pragma unroll
-  for (int x = 0; x < 2; ++x) it.n[x] = max(0, min(n[x], ke) - it.kb);
-  it.nk = max(it.n[0], it.n[1]);
-  it.clean = max(0, max(0, it.first[0]) / kTile - it.kb);
+  for (int x = 0; x < 2; ++x) it.tile[x].n = max(0, min(n[x], ke) - it.kb);
+  it.nk = max(it.tile[0].n, it.tile[1].n);
+  it.clean = max(0, max(0, it.tile[0].first) / kTile - it.kb);
   return it;
 }
 
-// The items of a CTA, from the heaviest: every second round runs the other way
-// round, so that no CTA always gets the heavier end of one.
-struct Rounds {
-  int round = 0;
-  __device__ __forceinline__ bool next(int items, int* i) {
-    for (;;) {
-      const int64_t base = static_cast<int64_t>(round) * gridDim.x;
-      if (base >= items) return false;
-      const int at = (round & 1) ? static_cast<int>(gridDim.x - 1 - blockIdx.x) : static_cast<int>(blockIdx.x);
-      ++round;
-      if (base + at < items) {
-        *i = static_cast<int>(base + at);
-        return true;
-      }
-    }
+// The items of a CTA: its own block's, then those of blocks that it cancels before they
+// start, so that whoever is done first takes the next item of the list. The copying lane asks
+// and works the item out, a ring hands it to the other roles.
+constexpr int kItems = 4, kReaders = 11;  // the scanning and 2 issuing warps, 8 softmax warps
+struct Items {
+  Item item[kItems];
+  uint4 answer;
+  uint64_t answered, full[kItems], empty[kItems];
+};
+struct ItemReader {
+  uint32_t k = 0;  // items so far
+  // The next item, or null (none left, or a wait gave up: then *ok is false). kWarp: called by
+  // a whole warp together, else by one lane. It is there until release().
+  template <bool kWarp>
+  __device__ __forceinline__ const Item* next(Items& a, unsigned int* err, unsigned int code, bool* ok) {
+    *ok = ptx::mbar_wait(&a.full[k % kItems], (k / kItems) & 1, err, code, kWaitNs);
+    if (kWarp) *ok = __all_sync(0xffffffffu, *ok);
+    const Item* const it = &a.item[k % kItems];
+    return *ok && it->nk >= 0 ? it : nullptr;
+  }
+  template <bool kWarp>
+  __device__ __forceinline__ void release(Items& a) {
+    if (kWarp) __syncwarp();
+    if (!kWarp || (threadIdx.x & 31) == 0) ptx::mbar_arrive(&a.empty[k % kItems]);
+    ++k;
+  }
+};
+struct ItemWriter {
+  uint32_t k = 0, asked = 0, taken = 0;  // items written, requests, answers read
+  __device__ __forceinline__ bool put(Items& a, const Item& it, unsigned int* err, unsigned int code) {
+    if (k >= kItems && !ptx::mbar_wait(&a.empty[k % kItems], (k / kItems - 1) & 1, err, code, kWaitNs)) return false;
+    a.item[k % kItems] = it;
+    ptx::mbar_arrive(&a.full[k++ % kItems]);
+    return true;
+  }
+  __device__ __forceinline__ void ask(Items& a) {
+    ptx::mbar_arrive_expect_tx(&a.answered, 16);
+    ptx::try_cancel_block(&a.answer, &a.answered);
+    ++asked;
+  }
+  // The number of the item that was asked for, -1: none left.
+  __device__ __forceinline__ bool answer(Items& a, int* i, unsigned int* err, unsigned int code) {
+    if (!ptx::mbar_wait(&a.answered, taken & 1, err, code, kWaitNs)) return false;
+    ++taken;
+    *i = ptx::cancelled_block(&a.answer);
+    ptx::fence_proxy_async_smem();  // read before the next answer is written
+    return true;
   }
 };
 
@@ -196,6 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int bad[8];
   // the launch's table: reading it from the parameter space costs a miss an entry, for every item anew
   __shared__ PromptTable tab;
+  __shared__ Items items;
   unsigned int* const err = &g_prompt_error_word;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -220,6 +262,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::mbar_init(&v_empty[i], 3);
     }
     for (int i = 0; i < 8; ++i) bad[i] = 0;
+    ptx::mbar_init(&items.answered, 1);
+    for (int i = 0; i < kItems; ++i) {
+      ptx::mbar_init(&items.full[i], 1);
+      ptx::mbar_init(&items.empty[i], kReaders);
+    }
     ptx::fence_mbar_init();
   }
   for (int i = threadIdx.x; i < table.nseq; i += kThreads) {
@@ -249,46 +296,46 @@ __global__ void __launch_bounds__(kThreads, 1)
   // registers at launch: 384 x 168 = 64512; 256 x 208 + 128 x 80 = 63488
   if (warp >= 8) {
     ptx::reg_dec<80>();
-    Rounds rounds;
-    int i;
+    ItemReader work;
     uint32_t tiles = 0;  // key tiles of the items so far: ring position
     bool ok = true;
     if (warp == 8) {
       // ---- copies
       if (lane == 0) {
         uint32_t qn[2] = {0, 0}, issued = 0;  // copies of each row tile, and of K and V tiles
-        bool have = rounds.next(p.items, &i);
-        Item it;
-        if (have) it = find_item(tab, p, i);
-        while (ok && have) {
+        ItemWriter list;
+        int i = blockIdx.x;
+        do {
+          const Item it = find_item(tab, p, i);
+          ok = list.put(items, it, err, kErrTma);
+          // the rows of Q come from memory: they are on their way while the last item's tiles are used
+          if (ok && list.k > 1)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (!ok || it.n[x] == 0) continue;
+            for (int x = 0; x < 2; ++x)
+              if (it.tile[x].n > 0)
+                for (int h = 0; h < C::kHalves; ++h)
+                  ptx::tma_prefetch_3d(&qmap, h * 64, it.head * p.group, it.q_row + it.tile[x].t0);
+          auto load_q = [&](int x) {
+            if (!ok || it.tile[x].n == 0) return;
             ok = qn[x] == 0 || ptx::mbar_wait(&q_empty[x], (qn[x] - 1) & 1, err, kErrTma, kWaitNs);
-            if (!ok) continue;
+            if (!ok) return;
             ++qn[x];
             ptx::mbar_arrive_expect_tx(&q_full[x], p.tokens * p.group * D * 2);
             for (int h = 0; h < C::kHalves; ++h)
               ptx::tma_load_3d(ptx::smem_addr(q_sm + x * C::kTileBytes + h * kTile * 128), &qmap, &q_full[x], h * 64,
-                               it.head * p.group, tab.q_start[it.seq] + it.t0[x]);
-          }
-          // the next item's rows of Q come from memory: they are asked for an item ahead
-          have = rounds.next(p.items, &i);
-          Item next = it;
-          if (have) {
-            next = find_item(tab, p, i);
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-              if (next.n[x] > 0)
-                for (int h = 0; h < C::kHalves; ++h)
-                  ptx::tma_prefetch_3d(&qmap, h * 64, next.head * p.group, tab.q_start[next.seq] + next.t0[x]);
-          }
-          const int row0 = tab.k_start[it.seq] + it.kb * kTile;
+                               it.head * p.group, it.q_row + it.tile[x].t0);
+          };
+          // Q of row tile 0, K, Q of row tile 1, V: tile 0 starts on the item while tile 1 is at the last one
+          load_q(0);
+          const int row0 = it.k_row + it.kb * kTile;
           for (int j = 0; j < it.nk && ok; ++j, ++tiles) {
             const int s = tiles % ST;
             const uint32_t ph = ((tiles / ST) & 1) ^ 1;
+            // (a CTA that asked for the next item earlier could be left with two while another has none)
+            if (j + 1 == it.nk) list.ask(items);
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv) {
+              if (j == 0 && kv == 1) load_q(1);
               uint64_t* const bar = kv ? &v_full[s] : &k_full[s];
               ok = ok && (tiles < ST || ptx::mbar_wait(kv ? &v_empty[s] : &k_empty[s], ph, err, kErrTma, kWaitNs));
               if (!ok) break;
@@ -299,28 +346,35 @@ __global__ void __launch_bounds__(kThreads, 1)
               ++issued;
             }
           }
-          it = next;
+          if (ok && it.nk == 0) list.ask(items);
+          ok = ok && list.answer(items, &i, err, kErrTma);
+        } while (ok && i >= 0);
+        if (ok) {
+          Item end;
+          end.nk = -1;
+          ok = list.put(items, end, err, kErrTma);
         }
         if (!ok) {  // a wait gave up: the copies that were issued land before the CTA ends
           for (uint32_t n = issued > 2 * ST ? issued - 2 * ST : 0; n < issued; ++n)
             ptx::mbar_wait((n & 1) ? &v_full[n / 2 % ST] : &k_full[n / 2 % ST], (n / 2 / ST) & 1, err, kErrTma, kWaitNs);
           for (int x = 0; x < 2; ++x)
             if (qn[x]) ptx::mbar_wait(&q_full[x], (qn[x] - 1) & 1, err, kErrTma, kWaitNs);
+          if (list.asked > list.taken) ptx::mbar_wait(&items.answered, list.taken & 1, err, kErrTma, kWaitNs);
         }
       }
     } else if (warp == 11) {
       // ---- takes non-finite values out of the V tiles that some row sees only in part
       uint32_t looked = 0;
       int busy = 0;
-      while (ok && rounds.next(p.items, &i)) {
-        const Item it = find_item(tab, p, i);
-        if (it.nk == 0) continue;
-        const int klen = tab.k_len[it.seq];
-        for (int j = 0; j < it.nk && ok; ++j, ++tiles) {
+      while (const Item* const it = work.next<true>(items, err, kErrTma, &ok)) {
+        const int nk = it->nk, clean = it->clean, kb = it->kb, klen = it->k_len;
+        work.release<true>(items);
+        if (nk == 0) continue;
+        for (int j = 0; j < nk && ok; ++j, ++tiles) {
           // every tile's barrier is waited for and released, so that it never runs two phases ahead
           ok = __all_sync(0xffffffffu, ptx::mbar_wait(&v_full[tiles % ST], (tiles / ST) & 1, err, kErrTma, kWaitNs));
-          if (ok && j < it.clean && lane == 0) ptx::mbar_arrive(&v_empty[tiles % ST]);
-          if (!ok || j < it.clean) continue;
+          if (ok && j < clean && lane == 0) ptx::mbar_arrive(&v_empty[tiles % ST]);
+          if (!ok || j < clean) continue;
           uint4* const v = reinterpret_cast<uint4*>(v_ring + (tiles % ST) * C::kTileBytes);
           const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
 #pragma unroll 1
@@ -346,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int e = 0; e < 8; ++e)
                   if (!isfinite(__bfloat162float(w[e]))) {
                     w[e] = __float2bfloat16_rn(0.f);
-                    if ((it.kb + j) * kTile + (b + 32 * q) / 8 % kTile < klen) bad[busy & 7] = busy + 1;
+                    if ((kb + j) * kTile + (b + 32 * q) / 8 % kTile < klen) bad[busy & 7] = busy + 1;
                   }
               }
             }
@@ -359,6 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           ++looked;
         }
+        if (!ok) break;
         ++busy;
       }
     } else if (lane == 0) {
@@ -385,10 +440,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         ptx::tc_commit(&s_full[x]);
         ptx::tc_commit(&k_empty[tile % ST]);
       };
-      while (ok && rounds.next(p.items, &i)) {
-        const Item it = find_item(tab, p, i);
-        const int n = it.n[x];
-        if (it.nk == 0) continue;
+      while (const Item* const it = work.next<false>(items, err, kErrMma, &ok)) {
+        const int n = it->tile[x].n, nk = it->nk, clean = it->clean;
+        work.release<false>(items);
+        if (nk == 0) continue;
         ok = ptx::mbar_wait(&k_full[tiles % ST], (tiles / ST) & 1, err, kErrMma, kWaitNs);
         if (ok && n > 0) {
           ok = ptx::mbar_wait(&q_full[x], qn & 1, err, kErrMma, kWaitNs);
@@ -399,15 +454,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else if (ok) {
           ptx::mbar_arrive(&k_empty[tiles % ST]);
         }
-        for (int j = 0; j < it.nk && ok; ++j, ++tiles) {
+        for (int j = 0; j < nk && ok; ++j, ++tiles) {
           const int s = tiles % ST;
           // everything this step needs is waited for, used or not, so that no barrier is ever two phases ahead
           ok = ptx::mbar_wait(&v_full[s], (tiles / ST) & 1, err, kErrMma, kWaitNs);
-          if (ok && j >= it.clean) {
+          if (ok && j >= clean) {
             ok = ptx::mbar_wait(&seen[looked & 1], (looked >> 1) & 1, err, kErrMma, kWaitNs);
             ++looked;
           }
-          if (ok && j + 1 < it.nk)
+          if (ok && j + 1 < nk)
             ok = ptx::mbar_wait(&k_full[(tiles + 1) % ST], ((tiles + 1) / ST) & 1, err, kErrMma, kWaitNs);
           if (ok && j < n) {
             if (j == 0 && qn > 0) ok = ptx::mbar_wait(&o_empty[x], (qn - 1) & 1, err, kErrMma, kWaitNs);
@@ -442,9 +497,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
             ptx::mbar_arrive(&v_empty[s]);
           }
-          if (j + 1 >= n && j + 1 < it.nk) ptx::mbar_arrive(&k_empty[(tiles + 1) % ST]);
+          if (j + 1 >= n && j + 1 < nk) ptx::mbar_arrive(&k_empty[(tiles + 1) % ST]);
           if (j + 1 >= n) ptx::mbar_arrive(&turn[x ^ 1]);
         }
+        if (!ok) break;
         if (n > 0) ++qn;
       }
       if (!ok) {  // a wait gave up: what was issued finishes before the tensor memory is freed
@@ -471,16 +527,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       w_token[q] = row / p.group;
       w_off[q] = w_token[q] * p.out_stride + row % p.group * D + (lane & 3) * 8;
     }
-    Rounds rounds;
-    int i, busy = 0;
+    ItemReader work;
+    int busy = 0;
     uint32_t sn = 0, on = 0;  // key tiles and items of this row tile so far
     bool ok = true;
-    while (ok && rounds.next(p.items, &i)) {
-      const Item it = find_item(tab, p, i);
-      const int n = it.n[x];
-      const bool real = token < it.nt[x];
-      const int sees = real ? max(0, min(tab.k_len[it.seq], it.first[x] + token)) : 0;  // keys 0 .. sees - 1
-      const int whole = max(0, it.first[x]) / kTile - it.kb;  // tiles before this one need no mask
+    while (const Item* const next = work.next<true>(items, err, kErrSoftmax, &ok)) {
+      const Item& it = *next;
+      const ItemTile tl = it.tile[x];
+      const int n = tl.n, kb = it.kb;
+      const bool real = token < tl.nt;
+      const int sees = real ? max(0, min(it.k_len, tl.first + token)) : 0;  // keys 0 .. sees - 1
+      const int whole = max(0, tl.first) / kTile - kb;  // tiles before this one need no mask
       float m = -INFINITY, l = 0.f;  // reference (scaled, base 2) and sum of weights
       for (int j = 0; j < n; ++j, ++sn) {
         // (the warp's lanes go on or give up together)
@@ -493,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) ptx::tmem_wait_regs(s[c]);
         if (j >= whole) {
-          const int lim = sees - (it.kb + j) * kTile;
+          const int lim = sees - (kb + j) * kTile;
 #pragma unroll
           for (int c = 0; c < 4; ++c)
             if (__any_sync(0xffffffffu, lim < c * 32 + 32)) {  // columns 32 c .. that some row does not see
@@ -575,12 +632,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int e = 0; e < 32; ++e) o[c][e] = 0u;
       }
       if (it.nk > 0) ++busy;
-      const int64_t grow = static_cast<int64_t>(tab.q_start[it.seq]) + it.t0[x] + token;
+      const int64_t grow = static_cast<int64_t>(it.q_row) + tl.t0 + token;
       const int head = it.head * p.group + head_in;
       if (fix && real) {
         // non-finite values of V that this row does see
-        for (int key = (it.kb + it.clean) * kTile; key < min(sees, (it.kb + n) * kTile); ++key) {
-          const __nv_bfloat16* vr = p.v + (tab.k_start[it.seq] + static_cast<int64_t>(key)) * p.v_stride + it.head * D;
+        for (int key = (kb + it.clean) * kTile; key < min(sees, (kb + n) * kTile); ++key) {
+          const __nv_bfloat16* vr = p.v + (it.k_row + static_cast<int64_t>(key)) * p.v_stride + it.head * D;
 #pragma unroll
           for (int c = 0; c < D / 32; ++c)
 #pragma unroll
@@ -590,8 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
       }
-      if (p.splits > 1) {
-        if (!real) continue;  // (joined again by the next item's first warp-wide wait)
+      if (p.splits > 1 && real) {
         const int64_t rec = (grow * p.hq + head) * p.splits + it.split;
         float* ml = p.part + p.part_rows * D + rec * 2;
         ml[0] = n > 0 ? m : -INFINITY;
@@ -603,12 +659,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int e = 0; e < 8; ++e)
             dst[c * 8 + e] = make_float4(__uint_as_float(o[c][4 * e]), __uint_as_float(o[c][4 * e + 1]),
                                          __uint_as_float(o[c][4 * e + 2]), __uint_as_float(o[c][4 * e + 3]));
-      } else {
+      } else if (p.splits == 1) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
         // through shared memory, 32 dimensions a pass: a row straight from its thread would
         // touch 32 lines with every store (4096 line accesses an item, now 1024)
         __nv_bfloat16* const dst =
-            p.out + (static_cast<int64_t>(tab.q_start[it.seq]) + it.t0[x]) * p.out_stride + it.head * p.group * D;
+            p.out + (static_cast<int64_t>(it.q_row) + tl.t0) * p.out_stride + it.head * p.group * D;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
 #pragma unroll
@@ -624,11 +680,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int q = 0; q < 4; ++q) {
             const int row = 8 * q + (lane >> 2);
             const uint4 w = *reinterpret_cast<const uint4*>(stage + row * 64 + (((lane & 3) ^ (row >> 1 & 3)) << 4));
-            if (w_token[q] < it.nt[x]) *reinterpret_cast<uint4*>(dst + w_off[q] + c * 32) = w;
+            if (w_token[q] < tl.nt) *reinterpret_cast<uint4*>(dst + w_off[q] + c * 32) = w;
           }
           __syncwarp();
         }
       }
+      work.release<true>(items);
     }
     ptx::tc_fence_before();
   }
@@ -744,8 +801,7 @@ int launch_prompt(const Plan& pl, const PromptParams& p, const CUtensorMap& qm, 
     SWL_CUDA_TRY(cudaFuncSetAttribute(prompt_attention_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem));
     done.fetch_or(bit);
   }
-  const int sms = sm_count_prompt();
-  SWL_CUDA_TRY(launch_kernel(prompt_attention_kernel<D>, dim3(std::min(p.items, sms)), dim3(kThreads),
+  SWL_CUDA_TRY(launch_kernel(prompt_attention_kernel<D>, dim3(p.items), dim3(kThreads),
                              Cfg<D>::kSmem, st, 1, pl.t, p, qm, km, vm));
   if (p.splits > 1)
     SWL_CUDA_TRY(launch_kernel(prompt_combine_kernel<D>, dim3(static_cast<unsigned>((pl.total_q * p.hq * (D / 4) + 127) / 128)),

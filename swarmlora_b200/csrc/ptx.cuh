@@ -412,6 +412,33 @@ __host__ __device__ constexpr uint32_t idesc_bf16_f32(int m, int n) {
          (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// ---- cluster launch control ---------------------------------------------------------
+// Asks for a block of this grid that has not started yet: it is cancelled and its index
+// comes back in the 16 bytes at `dst`, completing them on `bar`. Once an answer says that there
+// was none left, no further request is made.
+__device__ __forceinline__ void try_cancel_block(uint4* dst, uint64_t* bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+          smem_addr(dst)),
+      "r"(smem_addr(bar))
+      : "memory");
+}
+// The x index of the cancelled block, or -1.
+__device__ __forceinline__ int cancelled_block(const uint4* answer) {
+  uint32_t x, got;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\t"
+      "ld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.u32 %1, 1, 0, p;\n\t"
+      "mov.u32 %0, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n\t}\n"
+      : "=r"(x), "=r"(got)
+      : "r"(smem_addr(answer))
+      : "memory");
+  return got ? static_cast<int>(x) : -1;
+}
+
 // ---- clusters ------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
