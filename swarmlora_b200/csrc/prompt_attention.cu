@@ -20,7 +20,16 @@
 //
 // A CTA stays and takes one item after the other, the next of the list whenever it is
 // free: the copies and score products of the next item run while the rows of the last
-// one are written.
+// one are written. Against a list dealt out beforehand by length, sixteen prompts of 17 to
+// 2048 tokens went from 248 to 218 us and five of up to 2000 with heads of 64 from 38 to 33 (a row
+// tile's 128 keys take 2.1 us, what is fixed in an item 3 to 4, so shares counted in keys are uneven).
+//
+// One prompt of 8191 tokens, 32 query and 8 kv heads of 128: 498 us, 1.1 PFLOP/s. What bounds
+// it is the chain of one row tile (product, 128 exponentials a thread, product: 2.1 us, of
+// which its products take 0.55), two of which are in flight: tensor memory has no room for a third. Without the two issuing warps' turns it is 607 us, with the turn
+// handed over before the score product 574, half way through it 519, two steps before its end
+// 500. Two threads a row for the exponentials: 597 us. One in 2 to 8 of them as a polynomial, in an
+// earlier build: 589 to 637 for 531.
 //
 // O is rescaled only when a row's maximum passes its reference by more than
 // 2^8 (then by the softmax warps themselves, which have just seen the MMA
@@ -230,7 +239,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* const out_sm = v_ring + ST * C::kTileBytes;
   // Who completes each barrier: *_full the copy or product that fills, *_empty who has used it.
   __shared__ __align__(8) uint64_t q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2];
-  __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], seen[2], turn[2], drained[2];
+  __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], turn[2], drained[2];
+  // as many as V tiles: with fewer, the scan could run two phases ahead of an issuing warp's wait
+  __shared__ __align__(8) uint64_t seen[ST];
   __shared__ uint32_t tmem_base;
   // [n & 7] == n + 1: a non-finite value of its sequence was taken out of a V tile of the
   // CTA's n-th item with keys (copies run at most 4 items ahead of the rows, so n's are done when n + 8 comes)
@@ -251,7 +262,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::mbar_init(&p_full[i], 4);
       ptx::mbar_init(&o_full[i], 1);
       ptx::mbar_init(&o_empty[i], 4);
-      ptx::mbar_init(&seen[i], 1);
       ptx::mbar_init(&turn[i], 1);
       ptx::mbar_init(&drained[i], 1);
     }
@@ -260,6 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::mbar_init(&k_empty[i], 2);
       ptx::mbar_init(&v_full[i], 1);
       ptx::mbar_init(&v_empty[i], 3);
+      ptx::mbar_init(&seen[i], 1);
     }
     for (int i = 0; i < 8; ++i) bad[i] = 0;
     ptx::mbar_init(&items.answered, 1);
@@ -408,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ptx::fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            ptx::mbar_arrive(&seen[looked & 1]);
+            ptx::mbar_arrive(&seen[looked % ST]);
             ptx::mbar_arrive(&v_empty[tiles % ST]);
           }
           ++looked;
@@ -459,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // everything this step needs is waited for, used or not, so that no barrier is ever two phases ahead
           ok = ptx::mbar_wait(&v_full[s], (tiles / ST) & 1, err, kErrMma, kWaitNs);
           if (ok && j >= clean) {
-            ok = ptx::mbar_wait(&seen[looked & 1], (looked >> 1) & 1, err, kErrMma, kWaitNs);
+            ok = ptx::mbar_wait(&seen[looked % ST], (looked / ST) & 1, err, kErrMma, kWaitNs);
             ++looked;
           }
           if (ok && j + 1 < nk)
@@ -567,7 +578,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 2; e < 32; e += 2)
 #pragma unroll
           for (int c = 0; c < 4; ++c) mx[c] = max3(mx[c], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
-        const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * p.scale_log2;
+        // (rows behind the tile's last one hold anything: they have no say in when the others rescale)
+        const float top = real ? fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * p.scale_log2 : -INFINITY;
         if (__any_sync(0xffffffffu, top > m + kRescaleLog2)) {
           const float mn = fmaxf(m, top);
           const float f = m == mn ? 1.f : ex2(m - mn);

@@ -579,6 +579,49 @@ def test_pages_and_rows_beyond_32_bit_offsets(native, cuda):
     assert torch.equal(got, wo.prompt_attention(q, k.contiguous(), v.contiguous(), [30, 60], [200, 2000]))
 
 
+def _no_wait_ran_out(native):
+    import ctypes as C
+    torch.cuda.synchronize()
+    code = C.c_uint(7)
+    native.check(native.lib().swl_attention_device_error(C.byref(code)))
+    return code.value == 0
+
+
+def test_items_whose_masked_tiles_follow_one_another(native, cuda):
+    """Blocks of which only the second row tile reaches the second key tile, mixed with
+    blocks of one row tile that crosses into it: four V tiles in a row hold masked keys,
+    and the scan of the last may be done while a product still waits for the second."""
+    from swarmlora_b200 import worker_ops as wo
+    for d, hq, hkv in ((64, 64, 8), (128, 64, 8), (64, 8, 8)):
+        two, one = (32, 136), (16, 136)  # tokens, keys at a group of 8
+        lens = [two, one, one] * 20 if hq > hkv else [(256, 264), (128, 264)] * 20
+        q_lens, k_lens = [a for a, _ in lens], [b for _, b in lens]
+        first = _check_prompt(cuda, q_lens, k_lens, hq, hkv, d, seed=11)
+        g = _gen(cuda, 11)
+        q, k, v = (_randn(g, sum(n), h, d) for n, h in ((q_lens, hq), (k_lens, hkv), (k_lens, hkv)))
+        for _ in range(100):
+            again = wo.prompt_attention(q, k, v, q_lens, k_lens, scale=d ** -0.5)
+        assert torch.equal(again, first) and _no_wait_ran_out(native)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("group", [1, 2, 5, 8])
+def test_mixed_batches_are_the_same_every_time(native, cuda, d, group):
+    from swarmlora_b200 import worker_ops as wo
+    import random
+    r = random.Random(d + group)
+    for n in (3, 14, 40):
+        q_lens = [r.choice([1, 7, 16, 33, 100, 128, 130, 266, 500]) for _ in range(n)]
+        k_lens = [a + r.choice([0, 0, 3, 10, 120, 700]) for a in q_lens]
+        hkv = 8 // group if group < 8 else 4
+        g = _gen(cuda, n)
+        q, k, v = (_randn(g, sum(m), h, d) for m, h in ((q_lens, hkv * group), (k_lens, hkv), (k_lens, hkv)))
+        first = wo.prompt_attention(q, k, v, q_lens, k_lens)
+        outs = [wo.prompt_attention(q, k, v, q_lens, k_lens) for _ in range(30)]
+        assert all(torch.equal(o, first) for o in outs)
+    assert _no_wait_ran_out(native)
+
+
 def test_no_wait_ran_out(native, cuda):
     """The bounded-wait status after this file's launches (it is cleared by reading)."""
     import ctypes as C
