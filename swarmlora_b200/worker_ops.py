@@ -207,22 +207,25 @@ NOALLOC_ATTN_SCRATCH_FLOATS = 1 << 20
 
 # ---- whole prompts, and the key/value cache held in 4 bits --------------------------------------
 # A decode step makes these calls once a layer with kernels of a few microseconds, so their
-# host side is kept short: tables go through array.array, contexts are entered only where needed.
-def _elsewhere(device: torch.device, stream) -> bool:
+# host side is kept short: tables go through array.array, contexts are entered only where
+# needed, and devices are compared by number (`at`: the CUDA device of the call).
+_BF16 = torch.bfloat16
+
+
+def _elsewhere(at: int, stream) -> bool:
     """Whether a call has to switch to its tensors' device or to a stream of its own."""
-    return stream is not None or device.index != torch.cuda.current_device()
+    return at < 0 or stream is not None or at != torch._C._cuda_getDevice()
 
 
-def _current(device: torch.device) -> int:
-    """The current stream's handle, without making a Stream object (3 us)."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+# The current stream's handle, without making a Stream object (3 us).
+_current = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
-def _there(device: torch.device, stream):
-    if device.type != "cuda":
+def _there(at: int, stream):
+    if at < 0:
         raise ValueError("CUDA tensors are needed")
     ctx = contextlib.ExitStack()
-    ctx.enter_context(torch.cuda.device(device))
+    ctx.enter_context(torch.cuda.device(at))
     ctx.enter_context(torch.cuda.stream(stream))
     return ctx
 
@@ -235,25 +238,26 @@ def _addr(table: array) -> int:
     return table.buffer_info()[0]
 
 
-def _bf16_rows(name: str, t: torch.Tensor, device, heads=None, head_dim=None) -> None:
-    """A bf16 tensor [rows, heads, head_dim] on `device` whose heads are contiguous."""
-    if t.dtype is not torch.bfloat16 or t.device != device:
+def _bf16_rows(name: str, t: torch.Tensor, at: int, heads=None, head_dim=None) -> tuple:
+    """A bf16 tensor [rows, heads, head_dim] on the call's device whose heads are
+    contiguous: its rows, heads, head_dim and the elements between rows."""
+    if t.dtype is not _BF16 or t.get_device() != at:
         raise ValueError(f"{name}: a bf16 tensor on the call's CUDA device is needed")
     shape = t.shape
     if len(shape) != 3 or (heads is not None and shape[1] != heads) or (head_dim is not None and shape[2] != head_dim):
         raise ValueError(f"{name}: shape {tuple(shape)} does not fit")
-    st = t.stride()
-    if st[2] != 1 or (shape[1] > 1 and st[1] != shape[2]):
+    n, h, d = shape
+    by, st, one = t.stride()
+    if one != 1 or (h > 1 and st != d):
         if t.numel():
             raise ValueError(f"{name}: heads must be contiguous")
+    return n, h, d, by if n > 1 else -(-h * d // 8) * 8  # a single row's stride is never used (torch leaves it arbitrary)
 
 
 def _row_stride(t: torch.Tensor) -> int:
-    """Elements between rows; a single row's stride is never used (torch leaves it arbitrary)."""
-    shape = t.shape
-    if shape[0] > 1:
-        return t.stride(0)
-    return -(-shape[-1] * (shape[-2] if len(shape) == 3 else 1) // 8) * 8
+    """Elements between rows of a [rows, width] tensor; a single row's stride is never used."""
+    n, width = t.shape
+    return t.stride()[0] if n > 1 else -(-width // 8) * 8
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_lens, k_lens=None, scale: float | None = None,
@@ -263,37 +267,34 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_lens, 
     r of a sequence sees its keys 0 .. r + k_len - q_len (k_lens defaults to
     q_lens; longer ones hold a prefix); a row without keys gives zeros.
     Returns out [rows of q, hq, D] (rows behind the last sequence are left as they are)."""
-    dev = q.device
-    if dev.type != "cuda" or _elsewhere(dev, stream):
-        with _there(dev, stream):
+    at = q.get_device()
+    if _elsewhere(at, stream):
+        with _there(at, stream):
             return prompt_attention(q, k, v, q_lens, k_lens, scale, out)
-    _bf16_rows("q", q, dev)
-    hq, D = q.shape[1], q.shape[2]
-    _bf16_rows("k", k, dev, None, D)
-    hkv = k.shape[1]
-    _bf16_rows("v", v, dev, hkv, D)
+    q_rows, hq, D, q_by = _bf16_rows("q", q, at)
+    k_rows, hkv, _, k_by = _bf16_rows("k", k, at, None, D)
+    v_rows, _, _, v_by = _bf16_rows("v", v, at, hkv, D)
     if k_lens is None:
         k_lens = q_lens
     n, total = len(q_lens), sum(q_lens)
     if len(k_lens) != n:
         raise ValueError("prompt_attention: one key length per sequence")
-    if total > q.shape[0] or sum(k_lens) > min(k.shape[0], v.shape[0]):
+    if total > q_rows or sum(k_lens) > min(k_rows, v_rows):
         raise ValueError("prompt_attention: the lengths add up to more rows than there are")
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out, out_by = torch.empty_like(q, memory_format=torch.contiguous_format), -(-hq * D // 8) * 8
     else:
-        _bf16_rows("out", out, dev, hq, D)
-        if total > out.shape[0]:
+        out_rows, _, _, out_by = _bf16_rows("out", out, at, hq, D)
+        if total > out_rows:
             raise ValueError("prompt_attention: out has fewer rows than q_lens")
     ql, kl = _ints(q_lens), _ints(k_lens)
     pq, pk = _addr(ql), _addr(kl)
     L = lib()
     need = L.swl_prompt_attention_part_floats(n, pq, pk, hq, hkv, D)
-    part = torch.empty(need, dtype=torch.float32, device=dev) if need > 0 else None
-    check(L.swl_prompt_attention(n, pq, pk, q.data_ptr(), _row_stride(q), k.data_ptr(), _row_stride(k), v.data_ptr(),
-                                 _row_stride(v), out.data_ptr(), _row_stride(out), hq, hkv, D,
-                                 float(scale) if scale is not None else D ** -0.5,
-                                 part.data_ptr() if part is not None else None, _current(dev)))
+    part = torch.empty(need, dtype=torch.float32, device=at) if need > 0 else None
+    check(L.swl_prompt_attention(n, pq, pk, q.data_ptr(), q_by, k.data_ptr(), k_by, v.data_ptr(), v_by, out.data_ptr(), out_by,
+                                 hq, hkv, D, float(scale) if scale is not None else D ** -0.5,
+                                 part.data_ptr() if part is not None else None, _current(at)))
     return out
 
 
@@ -316,40 +317,43 @@ def kv4_cache(num_pages: int, hkv: int, head_dim: int = 128, page: int = 16, dev
                        device=device if device is not None else "cuda")
 
 
-def _check_slots(what: str, t: torch.Tensor, n: int, dtype, device, dims: int) -> int:
+def _check_slots(what: str, t: torch.Tensor, n: int, dtype, at: int, dims: int) -> int:
     """One row per slot, contiguous inside; returns the rows' stride."""
     st = t.stride()
-    if t.dtype is not dtype or t.device != device or len(st) != dims or t.size(0) != n or st[-1] != 1:
-        raise ValueError(f"{what}: {dtype} on {device}, one row per slot, contiguous inside")
+    if t.dtype is not dtype or t.get_device() != at or len(st) != dims or t.shape[0] != n or st[-1] != 1:
+        raise ValueError(f"{what}: {dtype} on cuda:{at}, one row per slot, contiguous inside")
     return st[0]
 
 
-def _slot_rows(ts, n: int, what: str, dtype, size: int, device, first=None) -> array:
+def _slot_rows(ts, n: int, what: str, dtype, size: int, at: int, first=None) -> array:
     """Addresses of each slot's rows (elements of `size` bytes): a list of tensors,
     or one tensor with a row per slot (first: the first row of each slot)."""
     if isinstance(ts, torch.Tensor):
         if first is None:
-            by = size * _check_slots(what, ts, n, dtype, device, ts.dim())
+            by = size * _check_slots(what, ts, n, dtype, at, ts.dim())
             first = range(n)
         else:
             by = size * ts.stride(0)
-            if ts.dtype is not dtype or ts.device != device:
-                raise ValueError(f"{what}: {dtype} on {device} is needed")
+            if ts.dtype is not dtype or ts.get_device() != at:
+                raise ValueError(f"{what}: {dtype} on cuda:{at} is needed")
         base = ts.data_ptr()
         return array("Q", [base + i * by for i in first])
-    if len(ts) != n or any(t.dtype is not dtype or t.device != device or
+    if len(ts) != n or any(t.dtype is not dtype or t.get_device() != at or
                            (t.dim() and t.numel() > 1 and t.stride(-1) != 1) for t in ts):
-        raise ValueError(f"{what}: one {dtype} tensor per slot on {device}, contiguous inside")
+        raise ValueError(f"{what}: one {dtype} tensor per slot on cuda:{at}, contiguous inside")
     return array("Q", [t.data_ptr() for t in ts])
 
 
-def _kv4_check(cache: torch.Tensor, hkv: int, head_dim: int, page: int, device) -> None:
+def _kv4_check(cache: torch.Tensor, hkv: int, head_dim: int, page: int, at: int) -> int:
+    """A cache as kv4_cache makes it; returns its pages."""
     want = (page // 16, hkv, kv4_block_bytes(head_dim))
-    if cache.dtype is not torch.uint8 or cache.device != device or not cache.is_contiguous() or cache.shape[1:] != want:
-        raise ValueError(f"4-bit cache: contiguous uint8 [pages, {want[0]}, {want[1]}, {want[2]}] on {device} is needed")
+    shape = cache.shape
+    if cache.dtype is not torch.uint8 or cache.get_device() != at or not cache.is_contiguous() or shape[1:] != want:
+        raise ValueError(f"4-bit cache: contiguous uint8 [pages, {want[0]}, {want[1]}, {want[2]}] on cuda:{at} is needed")
+    return shape[0]
 
 
-def _kv4_slots(block_tables, caches, n: int, hkv: int, head_dim: int, page: int, device):
+def _kv4_slots(block_tables, caches, n: int, hkv: int, head_dim: int, page: int, at: int):
     """Block tables, their length, caches and their pages of a call over slots."""
     if isinstance(block_tables, torch.Tensor):
         if block_tables.dim() != 2:
@@ -357,36 +361,46 @@ def _kv4_slots(block_tables, caches, n: int, hkv: int, head_dim: int, page: int,
         table_len = block_tables.size(1)
     else:
         table_len = min((t.shape[0] for t in block_tables), default=1)
-    tables = _slot_rows(block_tables, n, "block tables", torch.int32, 4, device)
+    tables = _slot_rows(block_tables, n, "block tables", torch.int32, 4, at)
     if isinstance(caches, torch.Tensor):
         caches = [caches] * n
     for c in {id(c): c for c in caches}.values():
-        _kv4_check(c, hkv, head_dim, page, device)
+        _kv4_check(c, hkv, head_dim, page, at)
     if len(caches) != n:
         raise ValueError("4-bit cache: one for all slots, or one per slot")
     return tables, table_len, array("Q", [c.data_ptr() for c in caches]), min((c.size(0) for c in caches), default=1)
 
 
-def _all_packed(*tensors) -> bool:
-    return all(isinstance(t, torch.Tensor) for t in tensors)
+def _packed_slots(block_tables, caches, n: int, hkv: int, head_dim: int, page: int, at: int) -> tuple:
+    """Of one table of block tables and one cache: the table, the elements between
+    its rows and its length, the cache and its pages."""
+    by = _check_slots("block tables", block_tables, n, torch.int32, at, 2)
+    pages = _kv4_check(caches, hkv, head_dim, page, at)
+    return block_tables.data_ptr(), by, block_tables.shape[1], caches.data_ptr(), pages
+
+
+def _tensors(a, b) -> bool:
+    return isinstance(a, torch.Tensor) and isinstance(b, torch.Tensor)
 
 
 def _first_rows(rows) -> list:
     return [0, *itertools.accumulate(rows)][:len(rows)]
 
 
-def _packed(name: str, t: torch.Tensor, rows: int, width: int, device) -> None:
-    have = t.size(0)
-    if t.dtype is not torch.bfloat16 or t.device != device or not t.is_contiguous() or have < rows or \
-            t.numel() != have * width:
-        raise ValueError(f"{name}: contiguous bf16 with at least {rows} rows of {width} on {device} is needed")
+def _packed(name: str, t: torch.Tensor, rows: int, width: int, at: int) -> int:
+    """Contiguous bf16 rows of `width` elements; returns their number."""
+    have = t.shape[0]
+    if t.dtype is not _BF16 or t.get_device() != at or not t.is_contiguous() or have < rows or t.numel() != have * width:
+        raise ValueError(f"{name}: contiguous bf16 with at least {rows} rows of {width} on cuda:{at} is needed")
+    return have
 
 
 def _slots_of_rows(name: str, ts, rows, total: int, width: int) -> int:
     """Checks rows packed in one tensor or given per slot; returns their stride."""
     if isinstance(ts, torch.Tensor):
-        if ts.dim() != 2 or ts.shape[1] < width or ts.shape[0] < total:
-            raise ValueError(f"{name}: {tuple(ts.shape)} holds fewer than {total} rows of {width}")
+        shape = ts.shape
+        if len(shape) != 2 or shape[1] < width or shape[0] < total:
+            raise ValueError(f"{name}: {tuple(shape)} holds fewer than {total} rows of {width}")
         return _row_stride(ts)
     if len(ts) != len(rows) or any(t.dim() != 2 or t.shape[1] < width or t.shape[0] < r for t, r in zip(ts, rows)):
         raise ValueError(f"{name}: each slot must hold its rows of {width}")
@@ -404,9 +418,9 @@ def kv4_append(qkvs, block_tables, caches, seqlens, q_rot, cos_sin, hq: int, hkv
     in one tensor (then `rows` counts them per slot); block_tables: int32, one per
     slot or [slots, pages]; caches: kv4_cache, one or one per slot; seqlens: int32,
     tokens cached before."""
-    dev = q_rot.device
-    if dev.type != "cuda" or _elsewhere(dev, stream):
-        with _there(dev, stream):
+    at = q_rot.get_device()
+    if _elsewhere(at, stream):
+        with _there(at, stream):
             return kv4_append(qkvs, block_tables, caches, seqlens, q_rot, cos_sin, hq, hkv, head_dim, page, rows, k_rot)
     packed = isinstance(qkvs, torch.Tensor)
     if rows is None:
@@ -415,25 +429,23 @@ def kv4_append(qkvs, block_tables, caches, seqlens, q_rot, cos_sin, hq: int, hkv
         rows = [t.shape[0] for t in qkvs]
     n, total = len(rows), sum(rows)
     stride = _slots_of_rows("kv4_append: qkv", qkvs, rows, total, (hq + 2 * hkv) * head_dim)
-    _packed("kv4_append: q_rot", q_rot, total, hq * head_dim, dev)
+    _packed("kv4_append: q_rot", q_rot, total, hq * head_dim, at)
     if k_rot is not None:
-        _packed("kv4_append: k_rot", k_rot, total, hkv * head_dim, dev)
-    _packed("kv4_append: cos_sin", cos_sin, 1, head_dim, dev)
+        _packed("kv4_append: k_rot", k_rot, total, hkv * head_dim, at)
+    max_pos = _packed("kv4_append: cos_sin", cos_sin, 1, head_dim, at)
     counts = _ints(rows)
-    tail = (hq, hkv, head_dim, page, cos_sin.data_ptr(), cos_sin.size(0), q_rot.data_ptr(),
-            k_rot.data_ptr() if k_rot is not None else None, _current(dev))
-    if n and _all_packed(qkvs, block_tables, caches, seqlens):  # no tables of addresses to make
-        if qkvs.dtype is not torch.bfloat16 or qkvs.device != dev or qkvs.stride(1) != 1:
-            raise ValueError(f"kv4_append: qkv: bf16 rows on {dev} are needed")
-        by = _check_slots("block tables", block_tables, n, torch.int32, dev, 2)
-        _check_slots("kv4_append: seqlens", seqlens, n, torch.int32, dev, 1)
-        _kv4_check(caches, hkv, head_dim, page, dev)
-        check(lib().swl_kv4_append_packed(n, _addr(counts), qkvs.data_ptr(), stride, block_tables.data_ptr(), by,
-                                          block_tables.size(1), caches.data_ptr(), caches.size(0), seqlens.data_ptr(), *tail))
+    tail = (hq, hkv, head_dim, page, cos_sin.data_ptr(), max_pos, q_rot.data_ptr(),
+            k_rot.data_ptr() if k_rot is not None else None, _current(at))
+    if n and packed and _tensors(block_tables, caches) and isinstance(seqlens, torch.Tensor):  # no tables of addresses to make
+        if qkvs.dtype is not torch.bfloat16 or qkvs.get_device() != at or qkvs.stride()[1] != 1:
+            raise ValueError(f"kv4_append: qkv: bf16 rows on cuda:{at} are needed")
+        _check_slots("kv4_append: seqlens", seqlens, n, torch.int32, at, 1)
+        slots = _packed_slots(block_tables, caches, n, hkv, head_dim, page, at)
+        check(lib().swl_kv4_append_packed(n, _addr(counts), qkvs.data_ptr(), stride, *slots, seqlens.data_ptr(), *tail))
         return
-    src = _slot_rows(qkvs, n, "kv4_append: qkv", torch.bfloat16, 2, dev, _first_rows(rows) if packed else None)
-    tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, dev)
-    lens = _slot_rows(seqlens, n, "kv4_append: seqlens", torch.int32, 4, dev)
+    src = _slot_rows(qkvs, n, "kv4_append: qkv", torch.bfloat16, 2, at, _first_rows(rows) if packed else None)
+    tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, at)
+    lens = _slot_rows(seqlens, n, "kv4_append: seqlens", torch.int32, 4, at)
     check(lib().swl_kv4_append(n, _addr(counts), _addr(src), stride, _addr(tables), table_len, _addr(cache), pages,
                                _addr(lens), *tail))
 
@@ -443,24 +455,22 @@ def kv4_gather(block_tables, caches, starts, lens, k_out, v_out, hkv: int, head_
     """Tokens starts[i] .. starts[i] + lens[i] - 1 of each slot's 4-bit cache as
     packed bf16 rows of K and V (k_out, v_out [sum lens, hkv, D]): the keys
     that prompt_attention reads for a chunk behind a cached prefix."""
-    dev = k_out.device
-    if dev.type != "cuda" or _elsewhere(dev, stream):
-        with _there(dev, stream):
+    at = k_out.get_device()
+    if _elsewhere(at, stream):
+        with _there(at, stream):
             return kv4_gather(block_tables, caches, starts, lens, k_out, v_out, hkv, head_dim, page)
     n, total = len(lens), sum(lens)
     if len(starts) != n:
         raise ValueError("kv4_gather: one start per slot is needed")
-    _packed("kv4_gather: k_out", k_out, total, hkv * head_dim, dev)
-    _packed("kv4_gather: v_out", v_out, total, hkv * head_dim, dev)
+    _packed("kv4_gather: k_out", k_out, total, hkv * head_dim, at)
+    _packed("kv4_gather: v_out", v_out, total, hkv * head_dim, at)
     begin, count = _ints(starts), _ints(lens)
-    tail = (hkv, head_dim, page, k_out.data_ptr(), v_out.data_ptr(), _current(dev))
-    if n and _all_packed(block_tables, caches):
-        by = _check_slots("block tables", block_tables, n, torch.int32, dev, 2)
-        _kv4_check(caches, hkv, head_dim, page, dev)
-        check(lib().swl_kv4_gather_packed(n, _addr(begin), _addr(count), block_tables.data_ptr(), by, block_tables.size(1),
-                                          caches.data_ptr(), caches.size(0), *tail))
+    tail = (hkv, head_dim, page, k_out.data_ptr(), v_out.data_ptr(), _current(at))
+    if n and _tensors(block_tables, caches):
+        slots = _packed_slots(block_tables, caches, n, hkv, head_dim, page, at)
+        check(lib().swl_kv4_gather_packed(n, _addr(begin), _addr(count), *slots, *tail))
         return
-    tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, dev)
+    tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, at)
     check(lib().swl_kv4_gather(n, _addr(begin), _addr(count), _addr(tables), table_len, _addr(cache), pages, *tail))
 
 
@@ -476,37 +486,35 @@ def paged_attention_kv4(rows, block_tables, caches, seqlens, outs, q_rot, hq: in
     appended) at positions seqlens[i] + t. outs: one tensor of rows per slot,
     or all rows packed in one [rows, hq * D]. part: kv4_part_floats fp32 of scratch for
     this call alone (allocated here when None)."""
-    dev = q_rot.device
-    if dev.type != "cuda" or _elsewhere(dev, stream):
-        with _there(dev, stream):
+    at = q_rot.get_device()
+    if _elsewhere(at, stream):
+        with _there(at, stream):
             return paged_attention_kv4(rows, block_tables, caches, seqlens, outs, q_rot, hq, hkv, max_len, scale, head_dim,
                                        page, part)
     n, total, width = len(rows), sum(rows), hq * head_dim
-    _packed("paged_attention_kv4: q_rot", q_rot, total, width, dev)
+    _packed("paged_attention_kv4: q_rot", q_rot, total, width, at)
     stride = _slots_of_rows("paged_attention_kv4: out", outs, rows, total, width)
     counts = _ints(rows)
     L = lib()
     need = L.swl_kv4_part_floats(n, _addr(counts), hq, hkv, head_dim, max_len)
     if part is None:
         if need > 0:
-            part = torch.empty(need, dtype=torch.float32, device=dev)
-    elif part.dtype is not torch.float32 or part.device != dev or not part.is_contiguous() or part.numel() < need:
-        raise ValueError(f"paged_attention_kv4: part needs {need} contiguous fp32 values on {dev}")
+            part = torch.empty(need, dtype=torch.float32, device=at)
+    elif part.dtype is not torch.float32 or part.get_device() != at or not part.is_contiguous() or part.numel() < need:
+        raise ValueError(f"paged_attention_kv4: part needs {need} contiguous fp32 values on cuda:{at}")
     tail = (stride, hq, hkv, head_dim, page, float(scale), max_len, q_rot.data_ptr(),
-            part.data_ptr() if part is not None else None, _current(dev))
-    if n and _all_packed(block_tables, caches, seqlens, outs):
-        if outs.dtype is not torch.bfloat16 or outs.device != dev or outs.stride(1) != 1:
-            raise ValueError(f"paged_attention_kv4: out: bf16 rows on {dev} are needed")
-        by = _check_slots("block tables", block_tables, n, torch.int32, dev, 2)
-        _check_slots("paged_attention_kv4: seqlens", seqlens, n, torch.int32, dev, 1)
-        _kv4_check(caches, hkv, head_dim, page, dev)
-        check(L.swl_paged_attention_kv4_packed(n, _addr(counts), block_tables.data_ptr(), by, block_tables.size(1),
-                                               caches.data_ptr(), caches.size(0), seqlens.data_ptr(), outs.data_ptr(), *tail))
+            part.data_ptr() if part is not None else None, _current(at))
+    if n and _tensors(block_tables, caches) and _tensors(seqlens, outs):
+        if outs.dtype is not torch.bfloat16 or outs.get_device() != at or outs.stride()[1] != 1:
+            raise ValueError(f"paged_attention_kv4: out: bf16 rows on cuda:{at} are needed")
+        _check_slots("paged_attention_kv4: seqlens", seqlens, n, torch.int32, at, 1)
+        slots = _packed_slots(block_tables, caches, n, hkv, head_dim, page, at)
+        check(L.swl_paged_attention_kv4_packed(n, _addr(counts), *slots, seqlens.data_ptr(), outs.data_ptr(), *tail))
         return
     first = _first_rows(rows) if isinstance(outs, torch.Tensor) else None
-    dst = _slot_rows(outs, n, "paged_attention_kv4: out", torch.bfloat16, 2, dev, first)
-    tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, dev)
-    lens = _slot_rows(seqlens, n, "paged_attention_kv4: seqlens", torch.int32, 4, dev)
+    dst = _slot_rows(outs, n, "paged_attention_kv4: out", torch.bfloat16, 2, at, first)
+    tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, at)
+    lens = _slot_rows(seqlens, n, "paged_attention_kv4: seqlens", torch.int32, 4, at)
     check(L.swl_paged_attention_kv4(n, _addr(counts), _addr(tables), table_len, _addr(cache), pages, _addr(lens),
                                     _addr(dst), *tail))
 
