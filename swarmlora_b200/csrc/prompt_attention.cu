@@ -24,13 +24,14 @@
 // 2048 tokens went from 248 to 218 us and five of up to 2000 with heads of 64 from 38 to 33 (a row
 // tile's 128 keys take 2.1 us, what is fixed in an item 3 to 4, so shares counted in keys are uneven).
 //
-// One prompt of 8191 tokens, 32 query and 8 kv heads of 128: 443 us in a burst at 1965 MHz (1.24
-// PFLOP/s), 498 to 518 in a loop, where the power cap holds the clock at 1620 (1.06 to 1.10; the
-// figures here are of loops). At full clock what bounds it is the chain of one row tile (product, 128 exponentials a thread, product: 2.1 us, of
-// which its products take 0.55), two of which are in flight: tensor memory has no room for a third. Without the two issuing warps' turns it is 607 us, with the turn
-// handed over before the score product 574, half way through it 519, two steps before its end
-// 500. Two threads a row for the exponentials: 597 us. One in 2 to 8 of them as a polynomial, in an
-// earlier build: 589 to 637 for 531.
+// One prompt of 8191 tokens, 32 query and 8 kv heads of 128: 443 us in a burst at 1965 MHz
+// (1.24 PFLOP/s), 498 to 518 in a loop, where the power cap holds the clock at 1620 (1.06 to
+// 1.10; the figures here are of loops). At full clock what bounds it is the chain of one row
+// tile (product, 128 exponentials a thread, product: 2.1 us, of which its products take 0.55),
+// two of which are in flight: tensor memory has no room for a third. Without the two issuing
+// warps' turns it is 607 us, with the turn handed over before the score product 574, half way
+// through it 519, two steps before its end 500. Two threads a row for the exponentials: 597 us.
+// One in 2 to 8 of them as a polynomial, in an earlier build: 589 to 637 for 531.
 //
 // O is rescaled only when a row's maximum passes its reference by more than
 // 2^8 (then by the softmax warps themselves, which have just seen the MMA
