@@ -419,7 +419,7 @@ int swl_paged_attention_shrink(int nseg, const int* rows, const void* const* blo
                                const void* q_rot, float* part, const void* const* A_o, int r,
                                float* ws_o, const void* pf, int64_t pf_bytes, void* stream);
 /* Causal GQA attention over whole prompts (no counterpart in the reference,
- * whose prompts go through flash_attn_with_kvcache): nseg sequences packed one
+ * whose prompts go through a library): nseg sequences packed one
  * behind the other, sequence i with q_lens[i] query rows and k_lens[i] key
  * rows (host arrays). Row r of a sequence sees its keys 0 .. r + k_len - q_len,
  * so k_len > q_len is a chunk behind a prefix, q_len 1 a single token; a row
