@@ -23,14 +23,14 @@
 // so the common step needs one vote instead of a reduction.
 //
 // Work is shared out on the device, which alone knows the context lengths: with
-// few blocks per (slot, kv head) a CTA takes whole pairs; otherwise every CTA takes an equal
+// short contexts a CTA takes whole (slot, kv head) pairs; otherwise every CTA takes an equal
 // contiguous range of all blocks, a pair cut by a range boundary leaves partial
 // records (at most two a CTA) and a second launch joins them.
 //
 // What bounds it: integer logic, which runs at half rate. Turning a block's codes into operands
 // is 112 of the 200 or so logic operations it takes, a fifth of the time; without any
 // arithmetic the copies alone take 73 us where the whole takes 103 (16 slots of 16k-32k
-// tokens, 8 kv heads of 128: 435 MB, 4.2 TB/s; 28 slots of 256-768 tokens 14.5 us). Four
+// tokens, 8 kv heads of 128: 435 MB, 4.2 TB/s; 28 slots of 256-768 tokens 12.6 us). Four
 // warps with 168 registers, three CTAs an SM: 113 us before blocks shared their scores, against
 // 119 with 16 warps of 128 registers and 124 with 8 of 255. Measured and left out: fp8 operands for
 // the score product (208 us, the warp-level product is slow in that type), two-byte fixed-point
@@ -57,7 +57,7 @@ __device__ unsigned int g_kv4_error_word = 0;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr unsigned kErrBlock = 111;
 constexpr float kRescaleLog2 = 8.f;
-constexpr int kWarps = 4;
+constexpr int kWarps = 4, kManyWarps = 6;  // of a CTA; the larger where whole pairs leave SMs half empty
 
 struct AttnTable4 {
   RowSegments seg;
@@ -77,14 +77,14 @@ struct AttnParams4 {
   float* part;             // equal ranges: O [record][column][D], then (m, l) [record][column][2]
 };
 
-template <int D, int NT>
+template <int D, int NT, int NW>
 struct Cfg4 {
   static constexpr int W = D / 32, NG = D / kGroup, kBlock = block_bytes(D);
   static constexpr int kStages = (NT == 1 ? 2 : 3) * (128 / D);  // of two blocks
   static constexpr int kCols = 8 * NT;
   static constexpr int kLd = D + 4;  // floats between columns of the merge buffer: no bank twice in a quarter warp
-  static constexpr int kRing = kWarps * kStages * 2 * kBlock;
-  static constexpr int kMerge = kWarps * 8 * kLd * 4;
+  static constexpr int kRing = NW * kStages * 2 * kBlock;
+  static constexpr int kMerge = NW * 8 * kLd * 4;
   static constexpr int kSmem = kRing + kMerge;
 };
 
@@ -270,15 +270,15 @@ struct Walk {
 // four go with the first block of a pair and the other four with its second, so that
 // scores, exponentials and weights of two blocks are computed at once (columns
 // that would otherwise be empty). The two sets keep their own references and meet at the merge.
-template <int D, int NT, bool kDual>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
+template <int D, int NT, bool kDual, int NW>
+__global__ void __launch_bounds__(NW * 32, NT == 1 && NW == kWarps ? 3 : 2)
     kv4_attention_kernel(const __grid_constant__ AttnTable4 tab, const __grid_constant__ AttnParams4 p) {
-  using C = Cfg4<D, NT>;
+  using C = Cfg4<D, NT, NW>;
   constexpr int W = C::W, NG = C::NG, ST = C::kStages;
   extern __shared__ __align__(128) uint8_t dyn[];
   __shared__ Shares sh;
-  __shared__ __align__(8) uint64_t bars[kWarps][ST];
-  __shared__ float ml_sm[kWarps][8][2], corr_sm[kWarps][8][NG];
+  __shared__ __align__(8) uint64_t bars[NW][ST];
+  __shared__ float ml_sm[NW][8][2], corr_sm[NW][8][NG];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   uint8_t* const ring = dyn + warp * ST * 2 * C::kBlock;
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
   uint32_t ok0 = 0, ok1 = 0, ring_ok = 0;  // a bit per batch entry; two bits per stage: the blocks exist
   auto issue = [&]() {
     while (more && taken == batch) {      // the next up to 32 pairs of this warp
-      const int left = lp.b1 > lb ? (lp.b1 - lb + 2 * kWarps - 1) / (2 * kWarps) : 0;
+      const int left = lp.b1 > lb ? (lp.b1 - lb + 2 * NW - 1) / (2 * NW) : 0;
       if (left == 0) {
         more = lw.next(sh, tab, p, &lp);
         lb = lp.b0 + 2 * warp;
@@ -330,12 +330,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
       }
       batch = min(left, 32);
       taken = 0;
-      const int b = lb + lane * 2 * kWarps;
+      const int b = lb + lane * 2 * NW;
       addr0 = lane < batch ? block_of<D, true>(tab.c, lp.slot, b, lp.head) : nullptr;
       addr1 = lane < batch && b + 1 < lp.b1 ? block_of<D, true>(tab.c, lp.slot, b + 1, lp.head) : nullptr;
       ok0 = __ballot_sync(0xffffffffu, addr0 != nullptr);
       ok1 = __ballot_sync(0xffffffffu, addr1 != nullptr);
-      lb += batch * 2 * kWarps;
+      lb += batch * 2 * NW;
     }
     if (!more) return;
     const int st = issued % ST;
@@ -604,7 +604,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
       }
     };
 #pragma unroll 1
-    for (int b = x.b0 + 2 * warp; b < x.b1; b += 2 * kWarps) {
+    for (int b = x.b0 + 2 * warp; b < x.b1; b += 2 * NW) {
       const int st = used % ST;
       const uint8_t* const blk = ring + st * 2 * C::kBlock;
       const uint32_t there = ring_ok >> 2 * st & 3u;
@@ -649,19 +649,19 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
       }
       __syncthreads();
       constexpr int kMerged = kDual ? 4 : 8;  // columns of the pass, and sets of results for each
-      constexpr int kSets = kDual ? 2 * kWarps : kWarps;
-      for (int at = threadIdx.x; at < kMerged * (D / 4); at += kWarps * 32) {
+      constexpr int kSets = kDual ? 2 * NW : NW;
+      for (int at = threadIdx.x; at < kMerged * (D / 4); at += NW * 32) {
         const int mc = at / (D / 4), d4 = at % (D / 4) * 4;  // column, dimensions
         const int col = col0 + nt * 8 + mc;
         if (col >= ncols) continue;
         float top = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < kSets; ++e) top = fmaxf(top, ml_sm[e % kWarps][mc + e / kWarps * 4][0]);
+        for (int e = 0; e < kSets; ++e) top = fmaxf(top, ml_sm[e % NW][mc + e / NW * 4][0]);
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < kSets; ++e) {
-          const int w = e % kWarps, mw_c = mc + e / kWarps * 4;
+          const int w = e % NW, mw_c = mc + e / NW * 4;
           const float mw = ml_sm[w][mw_c][0], lw_ = ml_sm[w][mw_c][1];
           // no reference: nothing seen (no sum), or nothing but NaN, which stays
           const float f = mw == -INFINITY ? (lw_ == 0.f ? 0.f : 1.f) : ex2(mw - top);
@@ -703,7 +703,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
 template <int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32)
     kv4_join_kernel(const __grid_constant__ AttnTable4 tab, const __grid_constant__ AttnParams4 p, int ctas) {
-  using C = Cfg4<D, NT>;
+  using C = Cfg4<D, NT, kWarps>;
   __shared__ Shares sh;
   // the context lengths were complete before the attention launch, which started this one only then
   share_out<D, NT>(tab, p, &sh, ctas);
@@ -751,7 +751,7 @@ __global__ void __launch_bounds__(kWarps * 32)
 }
 
 struct Plan4 {
-  int nt, ctas, whole;
+  int nt, ctas, whole, warps;
   bool dual;
   int64_t pairs;
 };
@@ -773,30 +773,47 @@ Plan4 make_plan4(int nseg, const int* rows, int hq, int hkv, int max_len) {
   pl.pairs = 0;
   for (int i = 0; i < nseg; ++i) pl.pairs += (static_cast<int64_t>(rows[i]) * group + 8 * pl.nt - 1) / (8 * pl.nt) * hkv;
   const int64_t blocks = (max_len + kBlockTok - 1) / kBlockTok;
-  const int64_t slots = static_cast<int64_t>(sm_count4()) * (pl.nt == 1 ? 3 : 2);  // CTAs at a time
-  // whole pairs where cutting them would at most halve what a CTA has to do
-  pl.whole = blocks <= 2 * std::max<int64_t>((pl.pairs * blocks + slots - 1) / slots, 2 * kWarps) ? 1 : 0;
+  const int64_t sms = sm_count4();
+  const int64_t slots = sms * (pl.nt == 1 ? 3 : 2);  // CTAs at a time
+  // Whole pairs need no join (9 us with the records of a short one), equal ranges
+  // keep every SM busy. Measured, one row a slot, 8 kv heads of 128, whole (six warps) against cut: 4 slots of
+  // up to 1000 tokens 11.1 and 16.1 us, 3000 22.5 and 22.1; 28 slots 1000 14.4 and 21.5, 3000 30.7 and 30.7, 8000
+  // 69 and 52. Two column tiles, 28 slots of 4 rows: 4000 55 and 61, 8000 102 and 85. More pairs than
+  // CTAs at a time (28 slots of 5 rows): 1000 37 and 50, 2000 58 and 60, 4000 104 and 85.
+  pl.whole = blocks <= (pl.pairs > slots ? 136 : pl.nt == 1 ? 200 : 320) ? 1 : 0;
   pl.ctas = static_cast<int>(std::max<int64_t>(
       1, std::min<int64_t>(slots, pl.whole ? pl.pairs : (pl.pairs * blocks + 2 * kWarps - 1) / (2 * kWarps))));
+  // Whole pairs that fill two CTAs an SM at most have registers for six warps each: 28 slots of
+  // 256 to 768 tokens 14.5 -> 12.5 us, of up to 1000 16.4 -> 14.4.
+  pl.warps = pl.whole && pl.nt == 1 && blocks > 2 * kWarps && pl.pairs <= 2 * sms ? kManyWarps : kWarps;
   return pl;
 }
 
-template <int D, int NT, bool kDual>
+template <int D, int NT, bool kDual, int NW>
 int launch_kv4(const AttnTable4& t, const AttnParams4& p, const Plan4& pl, cudaStream_t st) {
   int dev = 0;
   SWL_CUDA_TRY(cudaGetDevice(&dev));
   static std::atomic<uint64_t> done{0};  // devices whose kernel has its shared memory limit raised
   const uint64_t bit = uint64_t{1} << (dev & 63);
   if (!(done.load(std::memory_order_relaxed) & bit)) {
-    SWL_CUDA_TRY(cudaFuncSetAttribute(kv4_attention_kernel<D, NT, kDual>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      Cfg4<D, NT>::kSmem));
+    SWL_CUDA_TRY(cudaFuncSetAttribute(kv4_attention_kernel<D, NT, kDual, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      Cfg4<D, NT, NW>::kSmem));
     done.fetch_or(bit);
   }
-  SWL_CUDA_TRY(launch_kernel(kv4_attention_kernel<D, NT, kDual>, dim3(pl.ctas), dim3(kWarps * 32), Cfg4<D, NT>::kSmem, st, 1, t, p));
+  SWL_CUDA_TRY(launch_kernel(kv4_attention_kernel<D, NT, kDual, NW>, dim3(pl.ctas), dim3(NW * 32), Cfg4<D, NT, NW>::kSmem, st, 1,
+                             t, p));
   if (!pl.whole)
     SWL_CUDA_TRY(launch_kernel(kv4_join_kernel<D, NT>, dim3(static_cast<unsigned>(pl.pairs)), dim3(kWarps * 32), 0, st, 1, t, p,
                                pl.ctas));
   return SWL_OK;
+}
+
+template <int D>
+int launch_kv4_of(const AttnTable4& t, const AttnParams4& p, const Plan4& pl, cudaStream_t st) {
+  if (pl.nt == 2) return launch_kv4<D, 2, false, kWarps>(t, p, pl, st);
+  if (pl.warps == kManyWarps)
+    return pl.dual ? launch_kv4<D, 1, true, kManyWarps>(t, p, pl, st) : launch_kv4<D, 1, false, kManyWarps>(t, p, pl, st);
+  return pl.dual ? launch_kv4<D, 1, true, kWarps>(t, p, pl, st) : launch_kv4<D, 1, false, kWarps>(t, p, pl, st);
 }
 
 }  // namespace
@@ -862,13 +879,7 @@ int attention(int nseg, const int* rows, const kv4::Slots& slots, int table_len,
   p.part = part;
   t.passes_each = (t.c.rows_each * p.group + 8 * pl.nt - 1) / (8 * pl.nt);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (head_dim == 128)
-    return pl.dual      ? kv4::launch_kv4<128, 1, true>(t, p, pl, st)
-           : pl.nt == 1 ? kv4::launch_kv4<128, 1, false>(t, p, pl, st)
-                        : kv4::launch_kv4<128, 2, false>(t, p, pl, st);
-  return pl.dual      ? kv4::launch_kv4<64, 1, true>(t, p, pl, st)
-         : pl.nt == 1 ? kv4::launch_kv4<64, 1, false>(t, p, pl, st)
-                      : kv4::launch_kv4<64, 2, false>(t, p, pl, st);
+  return head_dim == 128 ? kv4::launch_kv4_of<128>(t, p, pl, st) : kv4::launch_kv4_of<64>(t, p, pl, st);
 }
 
 }  // namespace
