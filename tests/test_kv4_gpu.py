@@ -328,7 +328,7 @@ def test_gather_reads_any_range(native, cuda, d, hkv, page):
     assert bool((k_out[at:] == 9.0).all()) and bool((v_out[at:] == 9.0).all())
 
 
-def _check_cached(dev, rows, ctx, hq, hkv, d, page, seed=0, bias=0.0, scale=None, gain=1.0):
+def _check_cached(dev, rows, ctx, hq, hkv, d, page, seed=0, bias=0.0, scale=None, gain=1.0, bound=0):
     from swarmlora_b200 import worker_ops as wo
     g = _gen(dev, seed)
     n = len(rows)
@@ -342,7 +342,7 @@ def _check_cached(dev, rows, ctx, hq, hkv, d, page, seed=0, bias=0.0, scale=None
     lens = torch.tensor(ctx, dtype=torch.int32, device=dev)
     out = torch.full((sum(rows) + 2, hq * d + 8), 9.0, dtype=BF, device=dev)
     scale = d ** -0.5 if scale is None else scale
-    wo.paged_attention_kv4(rows, tables, cache, lens, out, q, hq, hkv, longest, scale, head_dim=d, page=page)
+    wo.paged_attention_kv4(rows, tables, cache, lens, out, q, hq, hkv, max(longest, bound), scale, head_dim=d, page=page)
     assert bool((out[sum(rows):] == 9.0).all()) and bool((out[:, hq * d:] == 9.0).all())
     at = 0
     for i, r in enumerate(rows):
@@ -374,6 +374,23 @@ def test_cached_attention_of_a_full_decode_step(native, cuda):
     g = torch.Generator().manual_seed(1)
     _check_cached(cuda, [1] * 28, torch.randint(256, 768, (28,), generator=g).tolist(), 32, 8, 128, 16, seed=2)
     _check_cached(cuda, [1] * 128, torch.randint(0, 90, (128,), generator=g).tolist(), 4, 2, 64, 16, seed=3)
+
+
+@pytest.mark.parametrize("rows,ctx", [
+    ([1], [0]), ([1], [40]), ([1, 1, 1], [255, 0, 700]), ([2, 0, 2], [15, 3, 600]), ([4, 1], [1000, 2]), ([16, 1, 0, 3], [100, 0, 9, 333]),
+    ([1] * 30, list(range(0, 900, 30)))])
+@pytest.mark.parametrize("d,hq,hkv,page", [(128, 8, 2, 16), (64, 8, 2, 32), (128, 6, 6, 16), (64, 24, 1, 16), (128, 32, 8, 16)])
+def test_cached_attention_under_a_long_bound(native, cuda, rows, ctx, d, hq, hkv, page):
+    """The bound on the contexts is long (the work is cut into equal ranges), the contexts themselves are not."""
+    _check_cached(cuda, rows, ctx, hq, hkv, d, page, seed=sum(ctx) + hq + 1, bound=9000)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hkv,rows,ctx", [
+    (32, 8, [1] * 6, [129, 130, 400, 1023, 1500, 3000]), (32, 8, [1] * 36, [600] * 36), (16, 8, [1] * 40, [16 * i for i in range(40)]),
+    (64, 8, [1] * 5, [127, 128, 200, 2000, 3100]), (32, 8, [1] * 60, [17 * i for i in range(60)]), (32, 4, [2, 1, 3], [900, 3190, 0])])
+def test_cached_attention_by_whole_pairs(native, cuda, d, hq, hkv, rows, ctx):
+    _check_cached(cuda, rows, ctx, hq, hkv, d, 16, seed=len(rows) + hq)
 
 
 def test_cached_attention_offsets_and_large_scores(native, cuda):
