@@ -29,8 +29,8 @@
 //
 // What bounds it: integer logic, which runs at half rate. Turning a block's codes into operands
 // is 112 of the 200 or so logic operations it takes, a fifth of the time; without any
-// arithmetic the copies alone take 73 us where the whole takes 103 (16 slots of 16k-32k
-// tokens, 8 kv heads of 128: 435 MB, 4.2 TB/s; 28 slots of 256-768 tokens 12.6 us). Four
+// arithmetic the copies alone take 73 us where the whole takes 102 (16 slots of 16k-32k
+// tokens, 8 kv heads of 128: 435 MB, 4.2 TB/s; 28 slots of 256-768 tokens 12.8 us). Four
 // warps with 168 registers, three CTAs an SM: 113 us before blocks shared their scores, against
 // 119 with 16 warps of 128 registers and 124 with 8 of 255. Measured and left out: fp8 operands for
 // the score product (208 us, the warp-level product is slow in that type), two-byte fixed-point
@@ -725,21 +725,24 @@ __global__ void __launch_bounds__(kWarps * 32)
     auto record = [&](int cta) {
       return (2 * static_cast<int64_t>(cta) + (cta == c0 && u0 != c0 * sh.per_cta ? 1 : 0)) * C::kCols + mc;
     };
+    // a pair may lie in a dozen records: their loads are in flight together
     float top = -INFINITY;
+#pragma unroll 4
     for (int cta = c0; cta <= c1; ++cta) top = fmaxf(top, mls[record(cta) * 2]);
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f;
+#pragma unroll 4
     for (int cta = c0; cta <= c1; ++cta) {
       const int64_t r = record(cta);
-      const float mw = mls[2 * r], lw = mls[2 * r + 1];
-      const float f = mw == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : ex2(mw - top);
-      if (f == 0.f) continue;
+      const float2 mlw = *reinterpret_cast<const float2*>(mls + 2 * r);
       const float4 v = *reinterpret_cast<const float4*>(p.part + r * D + d4);
-      sum += f * lw;
-      a.x += f * v.x;
-      a.y += f * v.y;
-      a.z += f * v.z;
-      a.w += f * v.w;
+      const float f = mlw.x == -INFINITY ? (mlw.y == 0.f ? 0.f : 1.f) : ex2(mlw.x - top);
+      const bool none = f == 0.f;  // what it holds has no say, an infinity neither
+      sum += none ? 0.f : f * mlw.y;
+      a.x += none ? 0.f : f * v.x;
+      a.y += none ? 0.f : f * v.y;
+      a.z += none ? 0.f : f * v.z;
+      a.w += none ? 0.f : f * v.w;
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     uint2 w2;
@@ -775,16 +778,16 @@ Plan4 make_plan4(int nseg, const int* rows, int hq, int hkv, int max_len) {
   const int64_t blocks = (max_len + kBlockTok - 1) / kBlockTok;
   const int64_t sms = sm_count4();
   const int64_t slots = sms * (pl.nt == 1 ? 3 : 2);  // CTAs at a time
-  // Whole pairs need no join (9 us with the records of a short one), equal ranges
-  // keep every SM busy. Measured, one row a slot, 8 kv heads of 128, whole (six warps) against cut: 4 slots of
-  // up to 1000 tokens 11.1 and 16.1 us, 3000 22.5 and 22.1; 28 slots 1000 14.4 and 21.5, 3000 30.7 and 30.7, 8000
-  // 69 and 52. Two column tiles, 28 slots of 4 rows: 4000 55 and 61, 8000 102 and 85. More pairs than
-  // CTAs at a time (28 slots of 5 rows): 1000 37 and 50, 2000 58 and 60, 4000 104 and 85.
-  pl.whole = blocks <= (pl.pairs > slots ? 136 : pl.nt == 1 ? 200 : 320) ? 1 : 0;
+  // Whole pairs need no join (4 us and more), equal ranges keep every SM busy. Measured, whole
+  // against cut, one row a slot, 32 query and 8 kv heads of 128 (six warps): 4 slots of up to 1000
+  // tokens 11.0 and 15.2 us, 3000 22.5 and 18.7; 28 slots 1000 14.3 and 21.2, 3000 30.7 and 30.0, 8000 69
+  // and 52. Two column tiles (28 slots of 4 rows): 4000 55 and 61, 8000 102 and 85. More pairs
+  // than CTAs at a time (28 slots of 5 rows): 1000 37 and 50, 2000 58 and 60, 4000 104 and 85.
+  pl.whole = blocks <= (pl.pairs > slots ? 136 : pl.nt == 1 ? 176 : 320) ? 1 : 0;
   pl.ctas = static_cast<int>(std::max<int64_t>(
       1, std::min<int64_t>(slots, pl.whole ? pl.pairs : (pl.pairs * blocks + 2 * kWarps - 1) / (2 * kWarps))));
   // Whole pairs that fill two CTAs an SM at most have registers for six warps each: 28 slots of
-  // 256 to 768 tokens 14.5 -> 12.5 us, of up to 1000 16.4 -> 14.4.
+  // 256 to 768 tokens 14.5 -> 12.8 us, of up to 1000 16.4 -> 14.4.
   pl.warps = pl.whole && pl.nt == 1 && blocks > 2 * kWarps && pl.pairs <= 2 * sms ? kManyWarps : kWarps;
   return pl;
 }

@@ -720,20 +720,22 @@ __global__ void __launch_bounds__(128) prompt_combine_kernel(const __grid_consta
   if (at >= rows * p.hq) return;
   const int64_t rec = at * p.splits;
   const float* ml = p.part + p.part_rows * D + rec * 2;
-  float m = -INFINITY;
+  float m = -INFINITY;  // (the splits' loads are in flight together)
+#pragma unroll 4
   for (int s = 0; s < p.splits; ++s) m = fmaxf(m, ml[2 * s]);
   float l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
   for (int s = 0; s < p.splits; ++s) {
     // no reference: nothing seen (no sum), or nothing but NaN, which stays
     const float ms = ml[2 * s], ls = ml[2 * s + 1], f = ms == -INFINITY ? (ls == 0.f ? 0.f : 1.f) : ex2(ms - m);
-    if (f == 0.f) continue;
     const float4 v = *reinterpret_cast<const float4*>(p.part + (rec + s) * D + d4);
-    l += f * ls;
-    o.x += f * v.x;
-    o.y += f * v.y;
-    o.z += f * v.z;
-    o.w += f * v.w;
+    const bool none = f == 0.f;  // what it holds has no say, an infinity neither
+    l += none ? 0.f : f * ls;
+    o.x += none ? 0.f : f * v.x;
+    o.y += none ? 0.f : f * v.y;
+    o.z += none ? 0.f : f * v.z;
+    o.w += none ? 0.f : f * v.w;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint2 w;
