@@ -483,6 +483,19 @@ int swl_paged_attention_kv4(int nseg, const int* rows, const void* const* block_
                             const void* const* caches, int64_t num_pages, const void* const* seqlens,
                             void* const* out, int64_t out_stride, int hq, int hkv, int head_dim, int page,
                             float scale, int max_len, const void* q_rot, float* part, void* stream);
+/* The same three calls for slots whose block tables and caches differ in size: table_lens[i]
+ * entries and num_pages[i] pages bound slot i (host arrays). */
+int swl_kv4_append_each(int nseg, const int* rows, const void* const* qkv, int64_t qkv_stride,
+                        const void* const* block_tables, const int* table_lens, void* const* caches,
+                        const int64_t* num_pages, const void* const* seqlens, int hq, int hkv, int head_dim, int page,
+                        const void* cos_sin, int max_pos, void* q_rot, void* k_rot, void* stream);
+int swl_kv4_gather_each(int nseg, const int* starts, const int* lens, const void* const* block_tables,
+                        const int* table_lens, const void* const* caches, const int64_t* num_pages, int hkv,
+                        int head_dim, int page, void* k_out, void* v_out, void* stream);
+int swl_paged_attention_kv4_each(int nseg, const int* rows, const void* const* block_tables, const int* table_lens,
+                                 const void* const* caches, const int64_t* num_pages, const void* const* seqlens,
+                                 void* const* out, int64_t out_stride, int hq, int hkv, int head_dim, int page,
+                                 float scale, int max_len, const void* q_rot, float* part, void* stream);
 /* The same three calls for slots whose rows are packed one behind the other
  * (qkv, out), whose block tables are rows of one array (table_stride entries
  * apart), whose context lengths are one array and which share one cache. */

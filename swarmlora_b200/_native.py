@@ -143,6 +143,10 @@ SIGNATURES: dict[str, tuple] = {
     "swl_kv4_part_floats": (_i64, [_i32, _p, _i32, _i32, _i32, _i32]),
     "swl_paged_attention_kv4": (_i32, [_i32, _p, _p, _i32, _p, _i64, _p, _p, _i64, _i32, _i32, _i32, _i32, _f32, _i32, _p,
                                        _p, _p]),
+    "swl_kv4_append_each": (_i32, [_i32, _p, _p, _i64, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _p, _i32, _p, _p, _p]),
+    "swl_kv4_gather_each": (_i32, [_i32, _p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _p, _p, _p]),
+    "swl_paged_attention_kv4_each": (_i32, [_i32, _p, _p, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _f32, _i32, _p,
+                                            _p, _p]),
     "swl_kv4_append_packed": (_i32, [_i32, _p, _p, _i64, _p, _i64, _i32, _p, _i64, _p, _i32, _i32, _i32, _i32, _p, _i32, _p,
                                      _p, _p]),
     "swl_kv4_gather_packed": (_i32, [_i32, _p, _p, _p, _i64, _i32, _p, _i64, _i32, _i32, _i32, _p, _p, _p]),

@@ -899,6 +899,20 @@ SWL_EXPORT int swl_paged_attention_kv4(int nseg, const int* rows, const void* co
                    q_rot, part, stream);
 }
 
+SWL_EXPORT int swl_paged_attention_kv4_each(int nseg, const int* rows, const void* const* block_tables, const int* table_lens,
+                                            const void* const* caches, const int64_t* num_pages, const void* const* seqlens,
+                                            void* const* out, int64_t out_stride, int hq, int hkv, int head_dim, int page,
+                                            float scale, int max_len, const void* q_rot, float* part, void* stream) {
+  if (nseg > 0 && (!table_lens || !num_pages)) return set_error(SWL_ERR_ARG, "attention_kv4: null table lengths or page counts");
+  kv4::Slots s;
+  s.block_tables = block_tables;
+  s.caches = const_cast<void* const*>(caches);
+  s.seqlens = seqlens;
+  s.table_lens = table_lens;
+  s.num_pages = num_pages;
+  return attention(nseg, rows, s, 1, 1, nullptr, out, out_stride, hq, hkv, head_dim, page, scale, max_len, q_rot, part, stream);
+}
+
 SWL_EXPORT int swl_paged_attention_kv4_packed(int nseg, const int* rows, const int* block_tables, int64_t table_stride,
                                               int table_len, const void* cache, int64_t num_pages, const int* seqlens,
                                               void* out, int64_t out_stride, int hq, int hkv, int head_dim, int page,

@@ -14,6 +14,8 @@
 // way between two codes goes to the even one.
 #include <cuda_bf16.h>
 
+#include <algorithm>
+
 #include "common.h"
 #include "kv4.cuh"
 #include "launch.h"
@@ -308,9 +310,11 @@ int fill_cache(Cache* c, const char* what, int nseg, const int* rows, const Slot
   if (hkv < 1 || hkv > 1024) return set_error(SWL_ERR_ARG, "%s: kv heads outside 1..1024", what);
   if (page < kBlockTok || page > 1024 || (page & (page - 1)))
     return set_error(SWL_ERR_ARG, "%s: page must be 16, 32, 64, .. 1024 tokens", what);
-  if (table_len < 1 || num_pages < 1) return set_error(SWL_ERR_ARG, "%s: empty block table or cache", what);
-  c->table_len = table_len;
-  c->num_pages = num_pages;
+  const auto empty = [&] { return set_error(SWL_ERR_ARG, "%s: empty block table or cache", what); };
+  if ((!s.table_lens && table_len < 1) || (!s.num_pages && num_pages < 1)) return empty();
+  const auto bounded = [](int64_t pages) { return static_cast<uint32_t>(std::min(pages, int64_t{1} << 31)); };
+  c->table_len0 = table_len;
+  c->pages0 = bounded(num_pages);
   c->hkv = hkv;
   c->page_shift = 0;
   while ((kBlockTok << c->page_shift) < page) ++c->page_shift;
@@ -327,6 +331,11 @@ int fill_cache(Cache* c, const char* what, int nseg, const int* rows, const Slot
     return set_error(SWL_ERR_ARG, "%s: null block tables, caches or context lengths", what);
   uintptr_t align = reinterpret_cast<uintptr_t>(s.cache0);
   for (int i = 0; i < nseg && !c->packed; ++i) {
+    const int entries = s.table_lens ? s.table_lens[i] : table_len;
+    const int64_t pages = s.num_pages ? s.num_pages[i] : num_pages;
+    if (entries < 1 || pages < 1) return empty();
+    c->table_len[i] = entries;
+    c->pages[i] = bounded(pages);
     c->block_table[i] = s.packed ? s.table0 + i * s.table_step : static_cast<const int*>(s.block_tables[i]);
     c->cache[i] = static_cast<uint8_t*>(s.packed ? s.cache0 : s.caches[i]);
     c->seqlen[i] = !lens ? nullptr : s.packed ? s.len0 + i : static_cast<const int*>(s.seqlens[i]);
@@ -395,7 +404,7 @@ int gather(int nseg, const int* starts, const int* lens, const Slots& slots, int
   int64_t tiles = 0;
   for (int i = 0; i < nseg; ++i) {
     const int64_t end = static_cast<int64_t>(starts[i]) + lens[i];
-    if (starts[i] < 0 || end > static_cast<int64_t>(table_len) * page)
+    if (starts[i] < 0 || end > static_cast<int64_t>(t.c.table_len[i]) * page)
       return set_error(SWL_ERR_ARG, "kv4_gather: tokens %d..%lld of slot %d lie outside its block table", starts[i],
                        static_cast<long long>(end), i);
     t.start[i] = starts[i];
@@ -435,6 +444,21 @@ SWL_EXPORT int swl_kv4_append(int nseg, const int* rows, const void* const* qkv,
                      q_rot, k_rot, stream);
 }
 
+SWL_EXPORT int swl_kv4_append_each(int nseg, const int* rows, const void* const* qkv, int64_t qkv_stride,
+                                   const void* const* block_tables, const int* table_lens, void* const* caches,
+                                   const int64_t* num_pages, const void* const* seqlens, int hq, int hkv, int head_dim,
+                                   int page, const void* cos_sin, int max_pos, void* q_rot, void* k_rot, void* stream) {
+  if (nseg > 0 && (!table_lens || !num_pages)) return set_error(SWL_ERR_ARG, "kv4_append: null table lengths or page counts");
+  kv4::Slots s;
+  s.block_tables = block_tables;
+  s.caches = caches;
+  s.seqlens = seqlens;
+  s.table_lens = table_lens;
+  s.num_pages = num_pages;
+  return kv4::append(nseg, rows, nullptr, qkv, qkv_stride, s, 1, 1, hq, hkv, head_dim, page, cos_sin, max_pos, q_rot, k_rot,
+                     stream);
+}
+
 SWL_EXPORT int swl_kv4_append_packed(int nseg, const int* rows, const void* qkv, int64_t qkv_stride, const int* block_tables,
                                      int64_t table_stride, int table_len, void* cache, int64_t num_pages, const int* seqlens,
                                      int hq, int hkv, int head_dim, int page, const void* cos_sin, int max_pos, void* q_rot,
@@ -456,6 +480,18 @@ SWL_EXPORT int swl_kv4_gather(int nseg, const int* starts, const int* lens, cons
   s.block_tables = block_tables;
   s.caches = const_cast<void* const*>(caches);
   return kv4::gather(nseg, starts, lens, s, table_len, num_pages, hkv, head_dim, page, k_out, v_out, stream);
+}
+
+SWL_EXPORT int swl_kv4_gather_each(int nseg, const int* starts, const int* lens, const void* const* block_tables,
+                                   const int* table_lens, const void* const* caches, const int64_t* num_pages, int hkv,
+                                   int head_dim, int page, void* k_out, void* v_out, void* stream) {
+  if (nseg > 0 && (!table_lens || !num_pages)) return set_error(SWL_ERR_ARG, "kv4_gather: null table lengths or page counts");
+  kv4::Slots s;
+  s.block_tables = block_tables;
+  s.caches = const_cast<void* const*>(caches);
+  s.table_lens = table_lens;
+  s.num_pages = num_pages;
+  return kv4::gather(nseg, starts, lens, s, 1, 1, hkv, head_dim, page, k_out, v_out, stream);
 }
 
 SWL_EXPORT int swl_kv4_gather_packed(int nseg, const int* starts, const int* lens, const int* block_tables,

@@ -354,13 +354,15 @@ def _kv4_check(cache: torch.Tensor, hkv: int, head_dim: int, page: int, at: int)
 
 
 def _kv4_slots(block_tables, caches, n: int, hkv: int, head_dim: int, page: int, at: int):
-    """Block tables, their length, caches and their pages of a call over slots."""
+    """Block tables, their lengths, caches and their pages of a call over slots."""
     if isinstance(block_tables, torch.Tensor):
         if block_tables.dim() != 2:
             raise ValueError("block tables: [slots, pages] or one tensor per slot")
-        table_len = block_tables.size(1)
+        lens = [block_tables.shape[1]] * n
     else:
-        table_len = min((t.shape[0] for t in block_tables), default=1)
+        lens = [t.numel() for t in block_tables]
+        if any(not t.dim() or t.shape[-1] != k for t, k in zip(block_tables, lens)):
+            raise ValueError("block tables: one row of page ids per slot")
     tables = _slot_rows(block_tables, n, "block tables", torch.int32, 4, at)
     if isinstance(caches, torch.Tensor):
         caches = [caches] * n
@@ -368,7 +370,7 @@ def _kv4_slots(block_tables, caches, n: int, hkv: int, head_dim: int, page: int,
         _kv4_check(c, hkv, head_dim, page, at)
     if len(caches) != n:
         raise ValueError("4-bit cache: one for all slots, or one per slot")
-    return tables, table_len, array("Q", [c.data_ptr() for c in caches]), min((c.size(0) for c in caches), default=1)
+    return tables, _ints(lens), array("Q", [c.data_ptr() for c in caches]), array("q", [c.shape[0] for c in caches])
 
 
 def _packed_slots(block_tables, caches, n: int, hkv: int, head_dim: int, page: int, at: int) -> tuple:
@@ -416,8 +418,8 @@ def kv4_append(qkvs, block_tables, caches, seqlens, q_rot, cos_sin, hq: int, hkv
     to q_rot [rows, hq * D], k to k_rot [rows, hkv * D] when given) and appends k
     and v quantised. qkvs: one tensor of rows per slot, or all rows packed
     in one tensor (then `rows` counts them per slot); block_tables: int32, one per
-    slot or [slots, pages]; caches: kv4_cache, one or one per slot; seqlens: int32,
-    tokens cached before."""
+    slot (of any lengths) or [slots, pages]; caches: kv4_cache, one or one per slot (of
+    any page counts); seqlens: int32, tokens cached before."""
     at = q_rot.get_device()
     if _elsewhere(at, stream):
         with _there(at, stream):
@@ -444,10 +446,10 @@ def kv4_append(qkvs, block_tables, caches, seqlens, q_rot, cos_sin, hq: int, hkv
         check(lib().swl_kv4_append_packed(n, _addr(counts), qkvs.data_ptr(), stride, *slots, seqlens.data_ptr(), *tail))
         return
     src = _slot_rows(qkvs, n, "kv4_append: qkv", torch.bfloat16, 2, at, _first_rows(rows) if packed else None)
-    tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, at)
+    tables, table_lens, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, at)
     lens = _slot_rows(seqlens, n, "kv4_append: seqlens", torch.int32, 4, at)
-    check(lib().swl_kv4_append(n, _addr(counts), _addr(src), stride, _addr(tables), table_len, _addr(cache), pages,
-                               _addr(lens), *tail))
+    check(lib().swl_kv4_append_each(n, _addr(counts), _addr(src), stride, _addr(tables), _addr(table_lens), _addr(cache),
+                                    _addr(pages), _addr(lens), *tail))
 
 
 def kv4_gather(block_tables, caches, starts, lens, k_out, v_out, hkv: int, head_dim: int = 128, page: int = 16,
@@ -470,8 +472,9 @@ def kv4_gather(block_tables, caches, starts, lens, k_out, v_out, hkv: int, head_
         slots = _packed_slots(block_tables, caches, n, hkv, head_dim, page, at)
         check(lib().swl_kv4_gather_packed(n, _addr(begin), _addr(count), *slots, *tail))
         return
-    tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, at)
-    check(lib().swl_kv4_gather(n, _addr(begin), _addr(count), _addr(tables), table_len, _addr(cache), pages, *tail))
+    tables, table_lens, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, at)
+    check(lib().swl_kv4_gather_each(n, _addr(begin), _addr(count), _addr(tables), _addr(table_lens), _addr(cache),
+                                    _addr(pages), *tail))
 
 
 def kv4_part_floats(rows, hq: int, hkv: int, max_len: int, head_dim: int = 128) -> int:
@@ -513,10 +516,10 @@ def paged_attention_kv4(rows, block_tables, caches, seqlens, outs, q_rot, hq: in
         return
     first = _first_rows(rows) if isinstance(outs, torch.Tensor) else None
     dst = _slot_rows(outs, n, "paged_attention_kv4: out", torch.bfloat16, 2, at, first)
-    tables, table_len, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, at)
+    tables, table_lens, cache, pages = _kv4_slots(block_tables, caches, n, hkv, head_dim, page, at)
     lens = _slot_rows(seqlens, n, "paged_attention_kv4: seqlens", torch.int32, 4, at)
-    check(L.swl_paged_attention_kv4(n, _addr(counts), _addr(tables), table_len, _addr(cache), pages, _addr(lens),
-                                    _addr(dst), *tail))
+    check(L.swl_paged_attention_kv4_each(n, _addr(counts), _addr(tables), _addr(table_lens), _addr(cache), _addr(pages),
+                                         _addr(lens), _addr(dst), *tail))
 
 
 def rms_norm(xs, outs, w: torch.Tensor, eps: float, rows=None, x_stride: int | None = None,

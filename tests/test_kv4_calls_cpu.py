@@ -1,0 +1,55 @@
+"""What the 4-bit cache calls take and refuse, without a GPU: the slots' own tables and
+caches, and what the host side makes of them."""
+import ctypes as C
+
+import pytest
+import torch
+
+F = 0x1000  # an aligned address that is never dereferenced
+
+
+def _each(native, call, rows=(1, 1), table_lens=(4, 2), pages=(8, 3), starts=(0, 0), null=()):
+    n, lib, p = len(rows), native.lib(), native.ptr_array
+    ptrs = p([F] * n)
+    lens = None if "table_lens" in null else native.i32_array(table_lens)
+    count = None if "pages" in null else (C.c_int64 * n)(*pages)
+    counts = native.i32_array(rows)
+    if call == "append":
+        st = lib.swl_kv4_append_each(n, counts, ptrs, 1024, ptrs, lens, ptrs, count, ptrs, 4, 2, 128, 16, F, 64, F, None, None)
+    elif call == "gather":
+        st = lib.swl_kv4_gather_each(n, native.i32_array(starts), counts, ptrs, lens, ptrs, count, 2, 128, 16, F, F, None)
+    else:
+        st = lib.swl_paged_attention_kv4_each(n, counts, ptrs, lens, ptrs, count, ptrs, ptrs, 512, 4, 2, 128, 16, 0.1, 64, F,
+                                              None, None)
+    return st, native.last_error()
+
+
+@pytest.mark.parametrize("call", ["append", "gather", "attention"])
+@pytest.mark.parametrize("bad,word", [
+    (dict(null=("table_lens",)), "null table lengths"), (dict(null=("pages",)), "page counts"),
+    (dict(table_lens=(4, 0)), "empty"), (dict(pages=(0, 3)), "empty"), (dict(pages=(8, -1)), "empty")])
+def test_slots_of_their_own_sizes_refuse(native, call, bad, word):
+    st, msg = _each(native, call, **bad)
+    assert st != 0 and word in msg, (st, msg)
+
+
+def test_a_gather_is_bounded_by_the_slots_own_table(native):
+    st, msg = _each(native, "gather", rows=(64, 33))
+    assert st != 0 and "33 of slot 1 lie outside" in msg, msg
+
+
+def test_each_slot_keeps_its_own_sizes(native):
+    from swarmlora_b200 import worker_ops as wo
+    pages = [8, 3, 5]
+    caches = [wo.kv4_cache(n, 2, device="cpu") for n in pages]
+    tables = [torch.zeros(n, dtype=torch.int32) for n in (2, 6, 1)]
+    _, lens, _, count = wo._kv4_slots(tables, caches, 3, 2, 128, 16, -1)
+    assert list(lens) == [2, 6, 1] and list(count) == pages
+    # one row of a table of tables is as good as the row itself
+    _, lens, _, _ = wo._kv4_slots([torch.zeros(4, 7, dtype=torch.int32)[i:i + 1] for i in range(3)], caches, 3, 2, 128, 16, -1)
+    assert list(lens) == [7, 7, 7]
+    _, lens, _, count = wo._kv4_slots(torch.zeros(3, 5, dtype=torch.int32), caches[0], 3, 2, 128, 16, -1)
+    assert list(lens) == [5, 5, 5] and list(count) == [8, 8, 8]
+    for bad in (torch.zeros(2, 7, dtype=torch.int32), torch.tensor(1, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="block tables"):
+            wo._kv4_slots([bad] * 3, caches, 3, 2, 128, 16, -1)

@@ -1,0 +1,127 @@
+"""Forms in which the 4-bit cache and prompt calls take their slots, rows and streams. What is
+written is compared with the plain forms entry by entry; attention with 64 bits, under the
+bound of tests/test_kv4_gpu.py: an output is rounded to bf16 once (2^-8 of itself), its weights
+enter the value product in bf16 (2^-8 of sum p |v|, a 4-bit value counting as |s code| + |m|) and
+what else fp32 and fp16 round is below 2^-10 of that sum."""
+import pytest
+import torch
+
+from tests import kv4_reference as ref
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+def _randn(g, *shape, dtype=BF):
+    return torch.randn(*shape, generator=g, device=g.device).to(dtype)
+
+
+def _gen(dev, seed):
+    return torch.Generator(device=dev).manual_seed(seed)
+
+
+def _cos_sin(n, d, dev):
+    a = torch.outer(torch.arange(n, dtype=torch.float64), 10000.0 ** (-torch.arange(0, d, 2, dtype=torch.float64) / d))
+    return torch.cat([a.cos(), a.sin()], -1).to(BF).to(dev)
+
+
+def _near_cached(got, q, cache, table, tokens, scale, what):
+    """got, q [rows, hq, D]: attention of the newest rows over `tokens` cached ones of one slot."""
+    d = q.shape[-1]
+    (_, k), (code, v) = ref.read_cache(cache, table, torch.arange(tokens, device=q.device), d)
+    bare = cache.clone()
+    bare[..., 9 * d:17 * d] = 0
+    low = ref.read_cache(bare, table, torch.arange(tokens, device=q.device), d)[1][1]  # the minima alone
+    want = ref.attend_fast(q, k, v, scale)
+    mass = ref.attend_fast(q, k, (v - low).abs() + low.abs(), scale)
+    got = got.double()
+    assert torch.isfinite(got).all(), what
+    bound = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -10) * mass + 1e-30
+    worst = ((got - want).abs() / bound).max().item()
+    assert worst <= 1.0, f"{what}: {worst:.3g} of the bound"
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(128, 8, 2), (64, 4, 4)])
+@pytest.mark.parametrize("as_rows", [False, True])
+@pytest.mark.parametrize("bound", [0, 9000])
+def test_tables_and_caches_of_different_sizes(native, cuda, d, hq, hkv, as_rows, bound):
+    """Per-slot block tables of different lengths and caches of different page counts: every slot
+    reaches its own last page, in all three calls."""
+    from swarmlora_b200 import worker_ops as wo
+    g = _gen(cuda, d + hq)
+    page, ctx, rows = 16, [20, 630, 0, 75], [3, 1, 40, 5]
+    per = [2, 40, 3, 5]        # table entries
+    pages = [4, 61, 3, 90]     # pages of each slot's cache
+    tables, caches = [], []
+    for n, m in zip(per, pages):
+        # distinct pages, the cache's last one in the table's last entry
+        t = torch.randperm(m - 1, generator=g, device=cuda)[:n - 1].to(torch.int32)
+        t = torch.cat([t, torch.tensor([m - 1], dtype=torch.int32, device=cuda)])
+        tables.append(t)
+        caches.append(wo.kv4_cache(m, hkv, d, page, device=cuda))
+    for t, c, n in zip(tables, caches, ctx):
+        if n:
+            ref.write_cache(c, t, torch.arange(n, device=cuda),
+                            *(_randn(g, n, hkv, d, dtype=torch.float32) for _ in range(2)))
+    qkv = [_randn(g, r, (hq + 2 * hkv) * d) for r in rows]
+    cs = _cos_sin(700, d, cuda)
+    lens = [torch.tensor([n], dtype=torch.int32, device=cuda) for n in ctx]
+    total = [a + b for a, b in zip(ctx, rows)]
+    assert all((a - 1) // page == n - 1 for a, n in zip(total, per))  # the last entry holds a new token
+    given = [torch.stack([t, t])[:1] for t in tables] if as_rows else tables
+    q_rot = torch.empty(sum(rows), hq * d, dtype=BF, device=cuda)
+    wo.kv4_append(qkv, given, caches, lens, q_rot, cs, hq, hkv, head_dim=d)
+    for i, (x, t, c) in enumerate(zip(qkv, tables, caches)):
+        pos = torch.arange(ctx[i], total[i], device=cuda)
+        x = x.unflatten(-1, (-1, d))
+        new = ref.rotate(x[:, hq:hq + hkv], cs[pos]), x[:, hq + hkv:].float()
+        for (code, _), y in zip(ref.read_cache(c, t, pos, d), new):
+            _, s, m = ref.quantise(y)
+            quot = ((y.unflatten(-1, (-1, 64)).double() - m.double()) / s.double()).clamp(0, 15).flatten(-2)
+            # half a step, and what fp32 rounds of the difference and of the quotient: 2^-23 of at most 16
+            assert bool(((code - quot).abs() <= 0.5 + 2.0 ** -19).all()), f"slot {i}"
+    k_out, v_out = (torch.empty(sum(total), hkv, d, dtype=BF, device=cuda) for _ in range(2))
+    wo.kv4_gather(given, caches, [0] * 4, total, k_out, v_out, hkv, head_dim=d)
+    for i, (k, v) in enumerate(zip(k_out.split(total), v_out.split(total))):
+        for (_, x), got in zip(ref.read_cache(caches[i], tables[i], torch.arange(total[i], device=cuda), d), (k, v)):
+            assert torch.equal(got, x.float().to(BF)), f"slot {i}"
+    outs = [torch.empty(r, hq * d, dtype=BF, device=cuda) for r in rows]
+    wo.paged_attention_kv4(rows, given, caches, lens, outs, q_rot, hq, hkv, max(*total, bound), d ** -0.5, head_dim=d)
+    for i, (o, q) in enumerate(zip(outs, q_rot.split(rows))):
+        _near_cached(o.view(-1, hq, d), q.reshape(-1, hq, d), caches[i], tables[i], total[i], d ** -0.5, f"slot {i}")
+
+
+def test_one_size_given_once(native, cuda):
+    """The C calls with one table length and page count for all slots write and read what the calls with
+    each slot's own do."""
+    from swarmlora_b200 import worker_ops as wo
+    g = _gen(cuda, 3)
+    hq, hkv, d, rows, ctx = 8, 2, 128, [2, 19], [30, 5]
+    n, total = len(rows), [a + b for a, b in zip(rows, ctx)]
+    tables = torch.randperm(8, generator=g, device=cuda).to(torch.int32).reshape(2, 4)
+    lens = torch.tensor(ctx, dtype=torch.int32, device=cuda)
+    qkv = _randn(g, sum(rows), (hq + 2 * hkv) * d)
+    cs, L, p = _cos_sin(64, d, cuda), native.lib(), native.ptr_array
+    stream = torch.cuda.current_stream().cuda_stream
+    counts, width = native.i32_array(rows), (hq + 2 * hkv) * d
+    tp, lp = p([t.data_ptr() for t in tables]), p([t.data_ptr() for t in lens.split(1)])
+    src = p([t.data_ptr() for t in qkv.split(rows)])
+    got = []
+    for each in (False, True):
+        cache = wo.kv4_cache(8, hkv, d, device=cuda)
+        q, out = (torch.zeros(sum(rows), hq * d, dtype=BF, device=cuda) for _ in range(2))
+        k, v = (torch.zeros(sum(total), hkv, d, dtype=BF, device=cuda) for _ in range(2))
+        if each:
+            wo.kv4_append(list(qkv.split(rows)), list(tables), cache, lens, q, cs, hq, hkv)
+            wo.kv4_gather(list(tables), cache, [0, 0], total, k, v, hkv)
+            wo.paged_attention_kv4(rows, list(tables), cache, lens, out, q, hq, hkv, 64, 0.1)
+        else:
+            cp = p([cache.data_ptr()] * n)
+            native.check(L.swl_kv4_append(n, counts, src, width, tp, 4, cp, 8, lp, hq, hkv, d, 16, cs.data_ptr(), 64,
+                                          q.data_ptr(), None, stream))
+            native.check(L.swl_kv4_gather(n, native.i32_array([0, 0]), native.i32_array(total), tp, 4, cp, 8, hkv, d, 16,
+                                          k.data_ptr(), v.data_ptr(), stream))
+            native.check(L.swl_paged_attention_kv4(n, counts, tp, 4, cp, 8, lp, p([o.data_ptr() for o in out.split(rows)]),
+                                                   hq * d, hq, hkv, d, 16, 0.1, 64, q.data_ptr(), None, stream))
+        got.append((cache, q, k, v, out))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
