@@ -334,8 +334,8 @@ def _slot_rows(ts, n: int, what: str, dtype, size: int, at: int, first=None) -> 
             first = range(n)
         else:
             by = size * ts.stride(0)
-            if ts.dtype is not dtype or ts.get_device() != at:
-                raise ValueError(f"{what}: {dtype} on cuda:{at} is needed")
+            if ts.dtype is not dtype or ts.get_device() != at or (ts.stride(-1) != 1 and ts.shape[-1] > 1):
+                raise ValueError(f"{what}: {dtype} rows on cuda:{at}, contiguous inside")
         base = ts.data_ptr()
         return array("Q", [base + i * by for i in first])
     if len(ts) != n or any(t.dtype is not dtype or t.get_device() != at or

@@ -53,3 +53,15 @@ def test_each_slot_keeps_its_own_sizes(native):
     for bad in (torch.zeros(2, 7, dtype=torch.int32), torch.tensor(1, dtype=torch.int32)):
         with pytest.raises(ValueError, match="block tables"):
             wo._kv4_slots([bad] * 3, caches, 3, 2, 128, 16, -1)
+
+
+def test_packed_rows_are_contiguous_inside(native):
+    """Packed rows beside listed tables: rows whose elements lie apart are refused."""
+    from swarmlora_b200 import worker_ops as wo
+    rows = torch.zeros(3, 8, dtype=torch.bfloat16)
+    first = [0, 2]
+    got = wo._slot_rows(rows[:, :6], 2, "rows", torch.bfloat16, 2, -1, first)
+    assert list(got) == [rows.data_ptr(), rows.data_ptr() + 2 * 16]
+    for bad in (torch.zeros(8, 3, dtype=torch.bfloat16).t(), torch.zeros(3, 16, dtype=torch.bfloat16)[:, ::2], rows.float()):
+        with pytest.raises(ValueError, match="rows"):
+            wo._slot_rows(bad, 2, "rows", torch.bfloat16, 2, -1, first)

@@ -125,3 +125,32 @@ def test_one_size_given_once(native, cuda):
                                                    hq * d, hq, hkv, d, 16, 0.1, 64, q.data_ptr(), None, stream))
         got.append((cache, q, k, v, out))
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_packed_rows_beside_listed_tables(native, cuda):
+    """Rows packed in one tensor with a list of tables and caches give what all-packed calls give; rows whose elements
+    lie apart are refused in both forms, and nothing is written."""
+    from swarmlora_b200 import worker_ops as wo
+    g = _gen(cuda, 7)
+    hq, hkv, d, rows = 4, 2, 128, [3, 1, 20]
+    T, width = sum(rows), (hq + 2 * hkv) * d
+    tables = torch.arange(12, dtype=torch.int32, device=cuda).reshape(3, 4)
+    lens = torch.tensor([9, 0, 30], dtype=torch.int32, device=cuda)
+    qkv, cs = _randn(g, T, width + 8)[:, :width], _cos_sin(64, d, cuda)
+    res = []
+    for listed in (False, True):
+        cache = wo.kv4_cache(12, hkv, d, device=cuda)
+        q, wide = torch.empty(T, hq * d, dtype=BF, device=cuda), torch.zeros(T, hq * d + 16, dtype=BF, device=cuda)
+        out = wide[:, 8:8 + hq * d]
+        t, c = (list(tables), [cache] * 3) if listed else (tables, cache)
+        wo.kv4_append(qkv, t, c, lens, q, cs, hq, hkv, rows=rows)
+        wo.paged_attention_kv4(rows, t, c, lens, out, q, hq, hkv, 64, 0.1)
+        apart = torch.zeros(width, T, dtype=BF, device=cuda).t()
+        kept = torch.full((hq * d, T), 9.0, dtype=BF, device=cuda)
+        with pytest.raises(ValueError, match="qkv"):
+            wo.kv4_append(apart, t, c, lens, q, cs, hq, hkv, rows=rows)
+        with pytest.raises(ValueError, match="out"):
+            wo.paged_attention_kv4(rows, t, c, lens, kept.t(), q, hq, hkv, 64, 0.1)
+        assert bool((kept == 9.0).all())
+        res.append((cache, q, wide))
+    assert all(torch.equal(a, b) for a, b in zip(*res))
