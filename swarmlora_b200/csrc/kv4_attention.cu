@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(NW * 32, NT == 1 && NW == kWarps ? 3 : 2)
       ++used;
       issue();  // into the stage that the previous pair left
       // some column ends here, or a block is missing
-      if ((b + 2) * kBlockTok > all_see || there != 3u) two(blk, b * kBlockTok, there, std::true_type{});
+      if (b * kBlockTok > all_see - 2 * kBlockTok || there != 3u) two(blk, b * kBlockTok, there, std::true_type{});
       else two(blk, b * kBlockTok, there, std::false_type{});
       __syncwarp();  // every lane has read the stage before it is filled again
     }
@@ -775,7 +775,7 @@ Plan4 make_plan4(int nseg, const int* rows, int hq, int hkv, int max_len) {
   pl.dual = static_cast<int64_t>(most) * group <= 4;
   pl.pairs = 0;
   for (int i = 0; i < nseg; ++i) pl.pairs += (static_cast<int64_t>(rows[i]) * group + 8 * pl.nt - 1) / (8 * pl.nt) * hkv;
-  const int64_t blocks = (max_len + kBlockTok - 1) / kBlockTok;
+  const int64_t blocks = (static_cast<int64_t>(max_len) + kBlockTok - 1) / kBlockTok;
   const int64_t sms = sm_count4();
   const int64_t slots = sms * (pl.nt == 1 ? 3 : 2);  // CTAs at a time
   // Whole pairs need no join (4 us and more), equal ranges keep every SM busy. Measured, whole

@@ -65,3 +65,13 @@ def test_packed_rows_are_contiguous_inside(native):
     for bad in (torch.zeros(8, 3, dtype=torch.bfloat16).t(), torch.zeros(3, 16, dtype=torch.bfloat16)[:, ::2], rows.float()):
         with pytest.raises(ValueError, match="rows"):
             wo._slot_rows(bad, 2, "rows", torch.bfloat16, 2, -1, first)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [[1], [1] * 28, [5] * 28])
+def test_the_largest_bound_plans_as_a_long_one_does(native, d, rows):
+    from swarmlora_b200 import worker_ops as wo
+    long = wo.kv4_part_floats(rows, 32, 8, 1 << 20, head_dim=d)
+    assert long > 0
+    for bound in (2 ** 31 - 17, 2 ** 31 - 16, 2 ** 31 - 15, 2 ** 31 - 1):
+        assert wo.kv4_part_floats(rows, 32, 8, bound, head_dim=d) == long, bound

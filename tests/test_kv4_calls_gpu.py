@@ -154,3 +154,19 @@ def test_packed_rows_beside_listed_tables(native, cuda):
         assert bool((kept == 9.0).all())
         res.append((cache, q, wide))
     assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+def test_attention_under_the_largest_bound(native, cuda):
+    from swarmlora_b200 import worker_ops as wo
+    g = _gen(cuda, 9)
+    hq, hkv, d, rows, ctx = 8, 2, 128, [1, 3, 1], [0, 500, 3000]
+    tables = torch.randperm(3 * 190, generator=g, device=cuda).to(torch.int32).reshape(3, 190)
+    cache = wo.kv4_cache(3 * 190, hkv, d, device=cuda)
+    for t, n in zip(tables, ctx):
+        ref.write_cache(cache, t, torch.arange(n + 3, device=cuda),
+                        *(_randn(g, n + 3, hkv, d, dtype=torch.float32) for _ in range(2)))
+    q, out = _randn(g, sum(rows), hq * d), torch.empty(sum(rows), hq * d, dtype=BF, device=cuda)
+    lens = torch.tensor(ctx, dtype=torch.int32, device=cuda)
+    wo.paged_attention_kv4(rows, tables, cache, lens, out, q, hq, hkv, 2 ** 31 - 1, d ** -0.5)
+    for i, (o, x) in enumerate(zip(out.split(rows), q.split(rows))):
+        _near_cached(o.view(-1, hq, d), x.view(-1, hq, d), cache, tables[i], ctx[i] + rows[i], d ** -0.5, f"slot {i}")
