@@ -17,10 +17,12 @@
 //
 // Tokens are the M dimension of the score product and dimensions that of the value
 // product; the columns are the slot's new rows times the query heads of the kv
-// head (8 NT of them a pass). The weights go from one layout to the other as fp16
-// (2^-11; they are at most 2^8 by the lazy reference) through a transposing
-// register move. The reference maximum moves only when a score passes it by 2^8,
-// so the common step needs one vote instead of a reduction.
+// head (8 NT of them a pass). The weights go from one layout to the other as fp16,
+// times 2^7, through a transposing register move: they are at most 2^8 by the lazy
+// reference, so that each is off by 2^-11 of itself or, below 2^-21, by 2^-32 (unscaled, a
+// long flat tail behind one large score would fall below fp16's smallest number, 2^-24, and be lost:
+// the sum of the weights keeps it). The reference maximum moves only when a score passes it
+// by 2^8, so the common step needs one vote instead of a reduction.
 //
 // Work is shared out on the device, which alone knows the context lengths: with
 // short contexts a CTA takes whole (slot, kv head) pairs; otherwise every CTA takes an equal
@@ -57,6 +59,9 @@ __device__ unsigned int g_kv4_error_word = 0;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr unsigned kErrBlock = 111;
 constexpr float kRescaleLog2 = 8.f;
+// The weights are taken 2^7 times as large until they have been fp16: 2^8 * 2^7 is half of its range. (Left
+// so for the sums as well, drafts take 55.5 us for 56.0, but values would overflow 2^7 sooner.)
+constexpr float kHalfUp = 7.f, kHalfDown = 1.f / 128.f;
 constexpr int kWarps = 4, kManyWarps = 6;  // of a CTA; the larger where whole pairs leave SMs half empty
 
 struct AttnTable4 {
@@ -92,6 +97,12 @@ __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+// Two fp32 products in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -401,7 +412,7 @@ __global__ void __launch_bounds__(NW * 32, NT == 1 && NW == kWarps ? 3 : 2)
       seen_g[nt] = sees(col);
     }
     all_see = sees(col0);  // the pass's first column belongs to its first row
-    // m: reference (scaled, base 2), nm: -m, bar_: the raw score that moves it
+    // m: reference (scaled, base 2), nm: 7 - m, bar_: the raw score that moves it, l: sum of the weights times 2^7
     float o[NT][2 * W][4], ps[NT][NG][4], corr[NT][NG], m[NT][2], nm[NT][2], bar_[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -478,7 +489,7 @@ __global__ void __launch_bounds__(NW * 32, NT == 1 && NW == kWarps ? 3 : 2)
             const float mn = fmaxf(m[nt][k], mx * p.scale_log2);
             f[k] = m[nt][k] == mn ? 1.f : ex2(m[nt][k] - mn);
             m[nt][k] = mn;
-            nm[nt][k] = mn == -INFINITY ? 0.f : -mn;  // nothing seen yet: every weight is zero
+            nm[nt][k] = mn == -INFINITY ? 0.f : kHalfUp - mn;  // nothing seen yet: every weight is zero
             bar_[nt][k] = (mn + kRescaleLog2) * p.inv_scale;
             l[nt][k] *= f[k];
           }
@@ -516,7 +527,8 @@ __global__ void __launch_bounds__(NW * 32, NT == 1 && NW == kWarps ? 3 : 2)
           l[nt][1] += po;
           const __half2 hp = __floats2half2_rn(pe, po);
           const uint32_t tr = transpose8x8(*reinterpret_cast<const uint32_t*>(&hp));
-          const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&tr));  // column g, tokens 2c, 2c + 1 (+ 8 h)
+          // column g, tokens 2c, 2c + 1 (+ 8 h)
+          const float2 w = mul2(__half22float2(*reinterpret_cast<const __half2*>(&tr)), make_float2(kHalfDown, kHalfDown));
 #pragma unroll
           for (int i = 0; i < NG; ++i) {
             uint32_t w0 = vp[h][i], w1 = vp[h][NG + i];
@@ -630,7 +642,7 @@ __global__ void __launch_bounds__(NW * 32, NT == 1 && NW == kWarps ? 3 : 2)
         for (int q = 4; q < 32; q <<= 1) s += __shfl_xor_sync(0xffffffffu, s, q);
         if (g == 0) {
           ml_sm[warp][2 * c + k][0] = m[nt][k];
-          ml_sm[warp][2 * c + k][1] = s;
+          ml_sm[warp][2 * c + k][1] = s * kHalfDown;
         }
         float* dst = merge + (warp * 8 + 2 * c + k) * C::kLd + 4 * g;
 #pragma unroll

@@ -170,3 +170,37 @@ def test_attention_under_the_largest_bound(native, cuda):
     wo.paged_attention_kv4(rows, tables, cache, lens, out, q, hq, hkv, 2 ** 31 - 1, d ** -0.5)
     for i, (o, x) in enumerate(zip(out.split(rows), q.split(rows))):
         _near_cached(o.view(-1, hq, d), x.view(-1, hq, d), cache, tables[i], ctx[i] + rows[i], d ** -0.5, f"slot {i}")
+
+
+@pytest.mark.parametrize("ctx,bound", [(2700, 0), (2700, 9000), (30000, 0)])
+@pytest.mark.parametrize("d,hq,hkv,rows", [(128, 8, 2, 1), (128, 16, 2, 1), (64, 8, 2, 1), (64, 16, 2, 1), (128, 8, 2, 4), (64, 8, 2, 4)])
+def test_a_flat_tail_behind_one_large_score(native, cuda, ctx, bound, d, hq, hkv, rows):
+    """The first key's weight is 2^20 to 2^28 times that of each other key, and its value is 0, so
+    the output is the tail's alone. A weight passes through fp16 as 2^7 times itself: below 2^-21 of the
+    largest it is off by up to 2^-32 of that, here so much of every token's |s code| + |m|."""
+    from swarmlora_b200 import worker_ops as wo
+    g = _gen(cuda, ctx + hq)
+    n = ctx + rows
+    table = torch.randperm(-(-n // 16), generator=g, device=cuda).to(torch.int32)
+    cache = wo.kv4_cache(table.numel(), hkv, d, device=cuda)
+    k = torch.zeros(n, hkv, d, device=cuda)
+    k[0, :, :64] = 1.0
+    v = 1.0 + 0.25 * torch.randn(n, hkv, d, generator=g, device=cuda)
+    v[0] = 0.0
+    ref.write_cache(cache, table, torch.arange(n, device=cuda), k, v)
+    powers = torch.tensor([20.0, 24.4, 25.2, 28.0], device=cuda).repeat(hq // 4)
+    q = torch.zeros(rows, hq, d, dtype=BF, device=cuda)
+    q[..., :64] = (powers * 0.6931471805599453 / 64).to(BF)[:, None]
+    out = torch.empty(rows, hq * d, dtype=BF, device=cuda)
+    lens = torch.tensor([ctx], dtype=torch.int32, device=cuda)
+    wo.paged_attention_kv4([rows], table[None], cache, lens, out, q.flatten(1), hq, hkv, max(n, bound), 1.0, head_dim=d)
+    (_, kk), (code, vv) = ref.read_cache(cache, table, torch.arange(n, device=cuda), d)
+    bare = cache.clone()
+    bare[..., 9 * d:17 * d] = 0
+    low = ref.read_cache(bare, table, torch.arange(n, device=cuda), d)[1][1]
+    parts = (vv - low).abs() + low.abs()
+    want, mass = ref.attend_fast(q, kk, vv, 1.0), ref.attend_fast(q, kk, parts, 1.0)
+    lost = 2.0 ** -32 * parts.sum(0).repeat_interleave(hq // hkv, 0)
+    off = (out.view(rows, hq, d).double() - want).abs()
+    limit = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -10) * mass + lost
+    assert bool((off <= limit).all()), f"{(off / limit).max().item():.3g} of the bound"
