@@ -453,7 +453,8 @@ int swl_attention_device_error(unsigned int* code);
  * outside the table are treated as absent: nothing is written for them, a gather gives
  * zeros and attention leaves their tokens out. seqlens[i] points to the
  * tokens cached before this step (device int). The slots of one call must not share
- * a page that the call writes. */
+ * a page that the call writes. Of a slot without rows in a call nothing is looked at: its
+ * pointers may be NULL, and those of the rows too when no slot has any. */
 int64_t swl_kv4_block_bytes(int head_dim); /* 18 * head_dim; 0 for another head_dim */
 /* Appends rows[i] new tokens to slot i at positions *seqlens[i] + t: q and k
  * are rotated (NeoX, cos/sin bf16 as swl_rope_append's table, arithmetic in fp32 and

@@ -865,18 +865,18 @@ int attention(int nseg, const int* rows, const kv4::Slots& slots, int table_len,
   if (hq < 1 || hq > 4096 || hq % hkv) return set_error(SWL_ERR_ARG, "attention_kv4: query heads must be a multiple of kv heads");
   if (!(scale > 0.f) || !std::isfinite(scale)) return set_error(SWL_ERR_ARG, "attention_kv4: scale must be positive and finite");
   if (max_len < 1) return set_error(SWL_ERR_ARG, "attention_kv4: max_len must be positive");
-  if (!q_rot || (reinterpret_cast<uintptr_t>(q_rot) & 15)) return set_error(SWL_ERR_ARG, "attention_kv4: q must be 16-byte aligned");
   if (out_stride < static_cast<int64_t>(hq) * head_dim || out_stride % 8)
     return set_error(SWL_ERR_ARG, "attention_kv4: output stride must hold all heads and be a multiple of 8");
-  if (nseg > 0 && !out && !out0) return set_error(SWL_ERR_ARG, "attention_kv4: null outputs");
+  if (t.seg.total_rows == 0) return SWL_OK;
+  if (!q_rot || (reinterpret_cast<uintptr_t>(q_rot) & 15)) return set_error(SWL_ERR_ARG, "attention_kv4: q must be 16-byte aligned");
+  if (!out && !out0) return set_error(SWL_ERR_ARG, "attention_kv4: null outputs");
   t.out0 = static_cast<__nv_bfloat16*>(out0);
   bool good = (reinterpret_cast<uintptr_t>(out0) & 15) == 0;
   for (int i = 0; i < nseg && !out0; ++i) {
     t.out[i] = static_cast<__nv_bfloat16*>(out[i]);
-    good = good && t.out[i] && (reinterpret_cast<uintptr_t>(t.out[i]) & 15) == 0;
+    good = good && (rows[i] == 0 || (t.out[i] && (reinterpret_cast<uintptr_t>(t.out[i]) & 15) == 0));
   }
   if (!good) return set_error(SWL_ERR_ARG, "attention_kv4: outputs must be 16-byte aligned");
-  if (t.seg.total_rows == 0) return SWL_OK;
   if (static_cast<int64_t>(t.seg.total_rows) * hq > (1 << 30)) return set_error(SWL_ERR_ARG, "attention_kv4: too many rows");
   const kv4::Plan4 pl = kv4::make_plan4(nseg, rows, hq, hkv, max_len);
   if (!pl.whole && (!part || (reinterpret_cast<uintptr_t>(part) & 15)))

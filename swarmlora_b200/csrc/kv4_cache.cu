@@ -310,8 +310,10 @@ int fill_cache(Cache* c, const char* what, int nseg, const int* rows, const Slot
   if (hkv < 1 || hkv > 1024) return set_error(SWL_ERR_ARG, "%s: kv heads outside 1..1024", what);
   if (page < kBlockTok || page > 1024 || (page & (page - 1)))
     return set_error(SWL_ERR_ARG, "%s: page must be 16, 32, 64, .. 1024 tokens", what);
+  // a slot without rows in this call is not looked at: it may have no table, cache or rows at all
+  const bool any = std::any_of(rows, rows + nseg, [](int r) { return r > 0; });
   const auto empty = [&] { return set_error(SWL_ERR_ARG, "%s: empty block table or cache", what); };
-  if ((!s.table_lens && table_len < 1) || (!s.num_pages && num_pages < 1)) return empty();
+  if (any && ((!s.table_lens && table_len < 1) || (!s.num_pages && num_pages < 1))) return empty();
   const auto bounded = [](int64_t pages) { return static_cast<uint32_t>(std::min(pages, int64_t{1} << 31)); };
   c->table_len0 = table_len;
   c->pages0 = bounded(num_pages);
@@ -326,16 +328,17 @@ int fill_cache(Cache* c, const char* what, int nseg, const int* rows, const Slot
   c->table_step = s.table_step;
   c->cache0 = static_cast<uint8_t*>(s.cache0);
   c->len0 = s.len0;
-  if (nseg == 0) return SWL_OK;
+  if (!any) return SWL_OK;
   if (s.packed ? !s.table0 || !s.cache0 || (lens && !s.len0) : !s.block_tables || !s.caches || (lens && !s.seqlens))
     return set_error(SWL_ERR_ARG, "%s: null block tables, caches or context lengths", what);
   uintptr_t align = reinterpret_cast<uintptr_t>(s.cache0);
   for (int i = 0; i < nseg && !c->packed; ++i) {
     const int entries = s.table_lens ? s.table_lens[i] : table_len;
     const int64_t pages = s.num_pages ? s.num_pages[i] : num_pages;
-    if (entries < 1 || pages < 1) return empty();
     c->table_len[i] = entries;
     c->pages[i] = bounded(pages);
+    if (rows[i] == 0) continue;
+    if (entries < 1 || pages < 1) return empty();
     c->block_table[i] = s.packed ? s.table0 + i * s.table_step : static_cast<const int*>(s.block_tables[i]);
     c->cache[i] = static_cast<uint8_t*>(s.packed ? s.cache0 : s.caches[i]);
     c->seqlen[i] = !lens ? nullptr : s.packed ? s.len0 + i : static_cast<const int*>(s.seqlens[i]);
@@ -357,24 +360,25 @@ int append(int nseg, const int* rows, const void* qkv0, const void* const* qkv, 
   SWL_TRY(fill_rows(&t.seg, "kv4_append", nseg, rows));
   SWL_TRY(fill_cache(&t.c, "kv4_append", nseg, rows, slots, true, false, table_len, num_pages, hkv, head_dim, page));
   if (hq < 1 || hq > 4096) return set_error(SWL_ERR_ARG, "kv4_append: query heads outside 1..4096");
-  if (max_pos < 1 || !cos_sin || !q_rot) return set_error(SWL_ERR_ARG, "kv4_append: null or empty cos/sin table, or null q_rot");
   if (qkv_stride < static_cast<int64_t>(hq + 2 * hkv) * head_dim || qkv_stride % 8)
     return set_error(SWL_ERR_ARG, "kv4_append: row stride must hold all heads and be a multiple of 8");
+  if (t.seg.total_rows == 0) return SWL_OK;
+  if (max_pos < 1 || !cos_sin || !q_rot) return set_error(SWL_ERR_ARG, "kv4_append: null or empty cos/sin table, or null q_rot");
   uintptr_t align = reinterpret_cast<uintptr_t>(cos_sin) | reinterpret_cast<uintptr_t>(q_rot) |
                     reinterpret_cast<uintptr_t>(k_rot) | reinterpret_cast<uintptr_t>(qkv0);
-  if (nseg > 0 && !qkv && !qkv0) return set_error(SWL_ERR_ARG, "kv4_append: null rows");
+  if (!qkv && !qkv0) return set_error(SWL_ERR_ARG, "kv4_append: null rows");
   int64_t tiles = 0;
   for (int i = 0; i < nseg; ++i) {
     t.qkv[i] = qkv0 ? static_cast<const __nv_bfloat16*>(qkv0) + t.seg.row_start[i] * qkv_stride
                     : static_cast<const __nv_bfloat16*>(qkv[i]);
+    t.tile_start[i] = static_cast<int>(tiles);
+    if (rows[i] == 0) continue;
     if (!t.qkv[i]) return set_error(SWL_ERR_ARG, "kv4_append: null per-slot pointer");
     align |= reinterpret_cast<uintptr_t>(t.qkv[i]);
-    t.tile_start[i] = static_cast<int>(tiles);
-    tiles += rows[i] ? (rows[i] + 30) / 16 : 0;
+    tiles += (rows[i] + 30) / 16;
   }
   t.tile_start[nseg] = static_cast<int>(tiles);
   if (align & 15) return set_error(SWL_ERR_ARG, "kv4_append: rows, cos/sin table and outputs must be 16-byte aligned");
-  if (tiles == 0) return SWL_OK;
   AppendParams p;
   p.hq = hq;
   p.qkv_stride = qkv_stride;
@@ -398,7 +402,8 @@ int gather(int nseg, const int* starts, const int* lens, const Slots& slots, int
   GatherTable t;
   SWL_TRY(fill_rows(&t.seg, "kv4_gather", nseg, lens));
   SWL_TRY(fill_cache(&t.c, "kv4_gather", nseg, lens, slots, false, false, table_len, num_pages, hkv, head_dim, page));
-  if (nseg > 0 && !starts) return set_error(SWL_ERR_ARG, "kv4_gather: null starts");
+  if (t.seg.total_rows == 0) return SWL_OK;
+  if (!starts) return set_error(SWL_ERR_ARG, "kv4_gather: null starts");
   if (!k_out || !v_out || ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15))
     return set_error(SWL_ERR_ARG, "kv4_gather: outputs must be 16-byte aligned");
   int64_t tiles = 0;
@@ -412,7 +417,6 @@ int gather(int nseg, const int* starts, const int* lens, const Slots& slots, int
     if (lens[i]) tiles += (end - 1) / 16 - starts[i] / 16 + 1;
   }
   t.tile_start[nseg] = static_cast<int>(tiles);
-  if (tiles == 0) return SWL_OK;
   const dim3 grid(static_cast<unsigned>(tiles), (hkv + kGatherHeads - 1) / kGatherHeads);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   __nv_bfloat16 *ko = static_cast<__nv_bfloat16*>(k_out), *vo = static_cast<__nv_bfloat16*>(v_out);

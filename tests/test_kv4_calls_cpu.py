@@ -75,3 +75,24 @@ def test_the_largest_bound_plans_as_a_long_one_does(native, d, rows):
     assert long > 0
     for bound in (2 ** 31 - 17, 2 ** 31 - 16, 2 ** 31 - 15, 2 ** 31 - 1):
         assert wo.kv4_part_floats(rows, 32, 8, bound, head_dim=d) == long, bound
+
+
+@pytest.mark.parametrize("rows", [(), (0,), (0, 0, 0)])
+def test_calls_without_a_row_need_no_tensors(native, rows):
+    """Empty tensors have no address."""
+    n, lib = len(rows), native.lib()
+    counts, none, zeros = native.i32_array(rows or (0,)), native.ptr_array([None] * max(n, 1)), native.i32_array([0] * max(n, 1))
+    pages = (C.c_int64 * max(n, 1))(*[0] * max(n, 1))
+    calls = [
+        lib.swl_kv4_append(n, counts, none, 1024, none, 0, none, 0, none, 4, 2, 128, 16, F, 64, None, None, None),
+        lib.swl_kv4_append_each(n, counts, none, 1024, none, zeros, none, pages, none, 4, 2, 128, 16, F, 64, None, None, None),
+        lib.swl_kv4_append_packed(n, counts, None, 1024, None, 0, 0, None, 0, None, 4, 2, 128, 16, F, 64, None, None, None),
+        lib.swl_kv4_gather(n, zeros, counts, none, 0, none, 0, 2, 128, 16, None, None, None),
+        lib.swl_kv4_gather_each(n, zeros, counts, none, zeros, none, pages, 2, 128, 16, None, None, None),
+        lib.swl_kv4_gather_packed(n, zeros, counts, None, 0, 0, None, 0, 2, 128, 16, None, None, None),
+        lib.swl_paged_attention_kv4(n, counts, none, 0, none, 0, none, none, 512, 4, 2, 128, 16, 0.1, 64, None, None, None),
+        lib.swl_paged_attention_kv4_each(n, counts, none, zeros, none, pages, none, none, 512, 4, 2, 128, 16, 0.1, 64, None,
+                                         None, None),
+        lib.swl_paged_attention_kv4_packed(n, counts, None, 0, 0, None, 0, None, None, 512, 4, 2, 128, 16, 0.1, 64, None, None,
+                                           None)]
+    assert calls == [0] * len(calls), native.last_error()

@@ -204,3 +204,46 @@ def test_a_flat_tail_behind_one_large_score(native, cuda, ctx, bound, d, hq, hkv
     off = (out.view(rows, hq, d).double() - want).abs()
     limit = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -10) * mass + lost
     assert bool((off <= limit).all()), f"{(off / limit).max().item():.3g} of the bound"
+
+
+@pytest.mark.parametrize("bound", [64, 9000])
+def test_slots_without_rows_may_be_empty(native, cuda, bound):
+    """Slots that take no part have empty rows, tables and lengths: the others get what they get without them."""
+    from swarmlora_b200 import worker_ops as wo
+    g = _gen(cuda, 12)
+    hq, hkv, d, rows = 4, 2, 128, [0, 3, 0, 1, 0]
+    width, cs = (hq + 2 * hkv) * d, _cos_sin(64, d, cuda)
+    ints = dict(dtype=torch.int32, device=cuda)
+    tables = torch.arange(8, **ints).reshape(2, 4)
+    lens = torch.tensor([9, 30], **ints)
+    qkv = _randn(g, 4, width)
+    want, got = [], []
+    for idle, res in ((False, want), (True, got)):
+        cache = wo.kv4_cache(8, hkv, d, device=cuda)
+        q, out = torch.empty(4, hq * d, dtype=BF, device=cuda), torch.empty(4, hq * d, dtype=BF, device=cuda)
+        k, v = (torch.zeros(43, hkv, d, dtype=BF, device=cuda) for _ in range(2))
+        if idle:
+            nothing = torch.empty(0, **ints)
+            spare = wo.kv4_cache(0, hkv, d, device=cuda)
+            x, o = ([t[:0], t[:3], t[:0], t[3:], torch.empty(0, t.shape[1], dtype=BF, device=cuda)] for t in (qkv, out))
+            t, n = [nothing, tables[0], nothing, tables[1], nothing], [nothing, lens[:1], nothing, lens[1:], nothing]
+            c = [spare, cache, spare, cache, spare]
+            wo.kv4_append(x, t, c, n, q, cs, hq, hkv)
+            wo.kv4_gather(t, c, [0] * 5, [0, 12, 0, 31, 0], k, v, hkv)
+            wo.paged_attention_kv4(rows, t, c, n, o, q, hq, hkv, bound, 0.1)
+        else:
+            wo.kv4_append(qkv, tables, cache, lens, q, cs, hq, hkv, rows=[3, 1])
+            wo.kv4_gather(tables, cache, [0, 0], [12, 31], k, v, hkv)
+            wo.paged_attention_kv4([3, 1], tables, cache, lens, out, q, hq, hkv, bound, 0.1)
+        res += [cache, q, k, v, out]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # and a step in which nobody does
+    none = torch.empty(0, width, dtype=BF, device=cuda)
+    q0, o0 = (torch.empty(0, hq * d, dtype=BF, device=cuda) for _ in range(2))
+    k0 = torch.empty(0, hkv, d, dtype=BF, device=cuda)
+    for r, t, n in (([0, 0], tables, lens), ([], tables[:0], lens[:0])):
+        wo.kv4_append(none, t, want[0], n, q0, cs, hq, hkv, rows=r)
+        wo.kv4_gather(t, want[0], r, r, k0, k0, hkv)
+        wo.paged_attention_kv4(r, t, want[0], n, o0, q0, hq, hkv, bound, 0.1)
+    torch.cuda.synchronize()
+    assert torch.equal(want[0], got[0])
