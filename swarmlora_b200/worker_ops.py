@@ -224,6 +224,8 @@ _current = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCur
 def _there(at: int, stream):
     if at < 0:
         raise ValueError("CUDA tensors are needed")
+    if stream is not None and stream.device_index != at:  # entering it would make its device the current one
+        raise ValueError(f"the stream belongs to cuda:{stream.device_index}, the tensors to cuda:{at}")
     ctx = contextlib.ExitStack()
     ctx.enter_context(torch.cuda.device(at))
     ctx.enter_context(torch.cuda.stream(stream))

@@ -96,3 +96,11 @@ def test_calls_without_a_row_need_no_tensors(native, rows):
         lib.swl_paged_attention_kv4_packed(n, counts, None, 0, 0, None, 0, None, None, 512, 4, 2, 128, 16, 0.1, 64, None, None,
                                            None)]
     assert calls == [0] * len(calls), native.last_error()
+
+
+def test_a_stream_of_another_device_is_refused(native):
+    from types import SimpleNamespace
+    from swarmlora_b200 import worker_ops as wo
+    assert wo._elsewhere(0, SimpleNamespace(device_index=1))
+    with pytest.raises(ValueError, match="stream belongs to cuda:1"):
+        wo._there(0, SimpleNamespace(device_index=1))

@@ -247,3 +247,27 @@ def test_slots_without_rows_may_be_empty(native, cuda, bound):
         wo.paged_attention_kv4(r, t, want[0], n, o0, q0, hq, hkv, bound, 0.1)
     torch.cuda.synchronize()
     assert torch.equal(want[0], got[0])
+
+
+def test_a_call_on_a_stream_of_its_own(native, cuda):
+    """Each call on a side stream, made by torch or wrapped from its handle."""
+    from swarmlora_b200 import worker_ops as wo
+    g = _gen(cuda, 14)
+    hq, hkv, d, rows = 4, 2, 128, [3, 20]
+    T, cs = sum(rows), _cos_sin(64, d, cuda)
+    tables = torch.arange(8, dtype=torch.int32, device=cuda).reshape(2, 4)
+    lens, qkv = torch.tensor([9, 30], dtype=torch.int32, device=cuda), _randn(g, T, (hq + 2 * hkv) * d)
+    side = torch.cuda.Stream()
+    res = []
+    for stream in (None, side, torch.cuda.ExternalStream(side.cuda_stream)):
+        cache = wo.kv4_cache(8, hkv, d, device=cuda)
+        q, out = (torch.zeros(T, hq * d, dtype=BF, device=cuda) for _ in range(2))
+        k, v = (torch.zeros(62, hkv, d, dtype=BF, device=cuda) for _ in range(2))
+        torch.cuda.synchronize()
+        wo.kv4_append(qkv, tables, cache, lens, q, cs, hq, hkv, rows=rows, stream=stream)
+        wo.kv4_gather(tables, cache, [0, 0], [12, 50], k, v, hkv, stream=stream)
+        wo.paged_attention_kv4(rows, tables, cache, lens, out, q, hq, hkv, 64, 0.1, stream=stream)
+        o = wo.prompt_attention(q.view(T, hq, d), k, v, rows, [12, 50], stream=stream)
+        torch.cuda.synchronize()
+        res.append((cache, q, k, v, out, o))
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(*res))
