@@ -300,6 +300,16 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_lens, 
     return out
 
 
+def attention_device_error(device=None) -> int:
+    """Synchronously reads and clears the bounded-wait error word of prompt_attention and
+    paged_attention_kv4 on a device (default: the current one). Not 0: a wait inside a kernel ran
+    out and outputs since the last reading may be wrong."""
+    code = C.c_uint(0)
+    with torch.cuda.device(device):
+        check(lib().swl_attention_device_error(C.byref(code)))
+    return int(code.value)
+
+
 _KV4_BLOCK = {64: 1152, 128: 2304}  # swl_kv4_block_bytes
 
 

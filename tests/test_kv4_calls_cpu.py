@@ -104,3 +104,21 @@ def test_a_stream_of_another_device_is_refused(native):
     assert wo._elsewhere(0, SimpleNamespace(device_index=1))
     with pytest.raises(ValueError, match="stream belongs to cuda:1"):
         wo._there(0, SimpleNamespace(device_index=1))
+
+
+def test_a_wait_that_ran_out_is_reported(native, monkeypatch):
+    """The error word and a failing read reach the caller (the library's part is a stand-in)."""
+    import contextlib
+    from swarmlora_b200 import worker_ops as wo
+    seen, status = [], [0]
+
+    class Lib:
+        def swl_attention_device_error(self, code):
+            code._obj.value = 111
+            return status[0]
+    monkeypatch.setattr(wo, "lib", Lib)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: (seen.append(d), contextlib.nullcontext())[1])
+    assert wo.attention_device_error() == 111 and wo.attention_device_error(3) == 111 and seen == [None, 3]
+    status[0] = 2
+    with pytest.raises(RuntimeError):
+        wo.attention_device_error()

@@ -271,3 +271,8 @@ def test_a_call_on_a_stream_of_its_own(native, cuda):
         torch.cuda.synchronize()
         res.append((cache, q, k, v, out, o))
     assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(*res))
+
+
+def test_no_wait_ran_out(native, cuda):
+    from swarmlora_b200 import worker_ops as wo
+    assert wo.attention_device_error() == 0 and wo.attention_device_error(cuda) == 0
