@@ -332,7 +332,7 @@ def kv4_cache(num_pages: int, hkv: int, head_dim: int = 128, page: int = 16, dev
 def _check_slots(what: str, t: torch.Tensor, n: int, dtype, at: int, dims: int) -> int:
     """One row per slot, contiguous inside; returns the rows' stride."""
     st = t.stride()
-    if t.dtype is not dtype or t.get_device() != at or len(st) != dims or t.shape[0] != n or st[-1] != 1:
+    if t.dtype is not dtype or t.get_device() != at or len(st) != dims or t.shape[0] != n or (st[-1] != 1 and t.shape[-1] > 1):
         raise ValueError(f"{what}: {dtype} on cuda:{at}, one row per slot, contiguous inside")
     return st[0]
 

@@ -122,3 +122,15 @@ def test_a_wait_that_ran_out_is_reported(native, monkeypatch):
     status[0] = 2
     with pytest.raises(RuntimeError):
         wo.attention_device_error()
+
+
+def test_the_stride_of_a_single_entry_does_not_count(native):
+    """One slot's length as a column of a wider table, one page a table as a transposed row."""
+    from swarmlora_b200 import worker_ops as wo
+    meta = torch.zeros(4, 6, dtype=torch.int32)
+    assert wo._check_slots("seqlens", meta[1:2, 3], 1, torch.int32, -1, 1) == 6
+    assert wo._check_slots("block tables", meta[:1].t()[2:5], 3, torch.int32, -1, 2) == 1
+    assert list(wo._slot_rows(meta[1:2, 3], 1, "seqlens", torch.int32, 4, -1)) == [meta[1, 3].data_ptr()]
+    for bad, n, dims in ((meta[:, 3], 4, 1), (meta.t(), 6, 2)):
+        with pytest.raises(ValueError, match="contiguous inside"):
+            wo._check_slots("tables", bad, n, torch.int32, -1, dims)
