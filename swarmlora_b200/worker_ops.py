@@ -214,11 +214,13 @@ _BF16 = torch.bfloat16
 
 def _elsewhere(at: int, stream) -> bool:
     """Whether a call has to switch to its tensors' device or to a stream of its own."""
-    return at < 0 or stream is not None or at != torch._C._cuda_getDevice()
+    return at < 0 or stream is not None or at != _device()
 
 
-# The current stream's handle, without making a Stream object (3 us).
-_current = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+# The current stream's handle and the current device, without making objects of them (3 us); torch's
+# public calls where it has no such shortcuts.
+_current = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda at: torch.cuda.current_stream(at).cuda_stream)
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _there(at: int, stream):

@@ -134,3 +134,19 @@ def test_the_stride_of_a_single_entry_does_not_count(native):
     for bad, n, dims in ((meta[:, 3], 4, 1), (meta.t(), 6, 2)):
         with pytest.raises(ValueError, match="contiguous inside"):
             wo._check_slots("tables", bad, n, torch.int32, -1, dims)
+
+
+def test_torch_without_the_shortcuts(native, monkeypatch):
+    """The current stream and device come from torch's public calls where the private ones are missing."""
+    import importlib.util
+    from types import SimpleNamespace
+    from swarmlora_b200 import worker_ops as wo
+    for name in ("_cuda_getCurrentRawStream", "_cuda_getDevice"):
+        monkeypatch.delattr(torch._C, name, raising=False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda at: SimpleNamespace(cuda_stream=100 + at))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 2)
+    spec = importlib.util.spec_from_file_location("swarmlora_b200.worker_ops_plain", wo.__file__)
+    plain = importlib.util.module_from_spec(spec)
+    monkeypatch.setitem(__import__("sys").modules, spec.name, plain)  # (dataclasses look their module up)
+    spec.loader.exec_module(plain)
+    assert plain._current(3) == 103 and plain._elsewhere(1, None) and not plain._elsewhere(2, None)
