@@ -150,3 +150,16 @@ def test_torch_without_the_shortcuts(native, monkeypatch):
     monkeypatch.setitem(__import__("sys").modules, spec.name, plain)  # (dataclasses look their module up)
     spec.loader.exec_module(plain)
     assert plain._current(3) == 103 and plain._elsewhere(1, None) and not plain._elsewhere(2, None)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows,hq,hkv,whole", [
+    ([1] * 28, 32, 8, 2816), ([1], 40, 8, 2816), ([2, 1], 32, 8, 2816),    # one column tile, pairs that fit at a time
+    ([1] * 60, 32, 8, 2176),                                                # more pairs than fit
+    ([2, 1, 3], 32, 4, 5120), ([4, 1], 32, 8, 5120),                        # two column tiles
+    ([5] * 28, 32, 8, 2176)])                                               # and more pairs than fit
+def test_up_to_which_bound_whole_pairs_are_taken(native, d, rows, hq, hkv, whole):
+    """(Where no device says how many multiprocessors it has, the plan counts 148.)"""
+    from swarmlora_b200 import worker_ops as wo
+    assert wo.kv4_part_floats(rows, hq, hkv, whole, head_dim=d) == 0
+    assert wo.kv4_part_floats(rows, hq, hkv, whole + 1, head_dim=d) > 0

@@ -276,3 +276,47 @@ def test_a_call_on_a_stream_of_its_own(native, cuda):
 def test_no_wait_ran_out(native, cuda):
     from swarmlora_b200 import worker_ops as wo
     assert wo.attention_device_error() == 0 and wo.attention_device_error(cuda) == 0
+
+
+def _check_plan(dev, rows, ctx, hq, hkv, d, bound, whole, seed):
+    """Attention of slots over one cache whose unused tokens are NaN, under a bound whose plan is asserted."""
+    from swarmlora_b200 import worker_ops as wo
+    assert (wo.kv4_part_floats(rows, hq, hkv, bound, head_dim=d) == 0) == whole
+    g = _gen(dev, seed)
+    per = -(-max(a + b for a, b in zip(rows, ctx)) // 16)
+    tables = torch.randperm(len(rows) * per + 2, generator=g, device=dev)[:len(rows) * per].to(torch.int32).reshape(-1, per)
+    cache = torch.full((tables.numel() + 2, 1, hkv, 18 * d), 0xff, dtype=torch.uint8, device=dev)
+    for t, r, n in zip(tables, rows, ctx):
+        ref.write_cache(cache, t, torch.arange(n + r, device=dev),
+                        *(_randn(g, n + r, hkv, d, dtype=torch.float32) for _ in range(2)))
+    q = _randn(g, sum(rows), hq * d)
+    out = torch.full((sum(rows) + 1, hq * d), 9.0, dtype=BF, device=dev)
+    wo.paged_attention_kv4(rows, tables, cache, torch.tensor(ctx, dtype=torch.int32, device=dev), out, q, hq, hkv, bound,
+                           d ** -0.5, head_dim=d)
+    assert bool((out[sum(rows):] == 9.0).all())
+    for i, (o, x) in enumerate(zip(out[:sum(rows)].split(rows), q.split(rows))):
+        if rows[i]:
+            _near_cached(o.view(-1, hq, d), x.view(-1, hq, d), cache, tables[i], ctx[i] + rows[i], d ** -0.5,
+                         f"slot {i} of {rows}/{ctx}")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (10, 2), (16, 2), (24, 4)])  # groups of 4 (blocks in pairs), 5, 8 and 6
+@pytest.mark.parametrize("ctx,bound,whole", [
+    ([0, 40, 126], 127, True), ([127], 128, True), ([128, 0, 63], 129, True),  # four warps up to 128 tokens, six beyond
+    ([1007, 1000], 1008, True), ([2800, 1, 2750], 2801, True), ([2815], 2816, True),
+    ([2816, 2799, 15], 2817, False), ([3000, 100], 3100, False), ([128, 5], 2817, False)])
+def test_single_rows_on_both_sides_of_each_plan(native, cuda, d, hq, hkv, ctx, bound, whole):
+    _check_plan(cuda, [1] * len(ctx), ctx, hq, hkv, d, bound, whole, seed=sum(ctx) + hq)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows,ctx,hq,hkv,bound,whole", [
+    ([2, 1, 2], [500, 2700, 0], 8, 2, 2816, True), ([1, 2], [2814, 2815], 8, 2, 2817, False),       # one column tile
+    ([4, 0, 1, 9], [2900, 5, 31, 4], 8, 2, 2904, True), ([3, 5], [5000, 100], 8, 2, 5120, True),     # two
+    ([3, 5], [5118, 5115], 8, 2, 5121, False), ([7, 1], [900, 130], 6, 6, 5121, False),
+    ([1] * 60, [36 * i for i in range(60)], 32, 8, 2176, True),                                      # many pairs
+    ([1] * 60, [36 * i for i in range(60)], 32, 8, 2177, False),
+    ([5, 4, 3, 2, 1] * 6, [70 * i for i in range(30)], 32, 8, 2176, True)])
+def test_several_rows_on_both_sides_of_each_plan(native, cuda, d, rows, ctx, hq, hkv, bound, whole):
+    _check_plan(cuda, rows, ctx, hq, hkv, d, bound, whole, seed=sum(ctx) + sum(rows))
