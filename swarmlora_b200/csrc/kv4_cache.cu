@@ -7,11 +7,12 @@
 //
 // Rounding: the cos/sin table is bf16, so the four products of a rotated pair
 // are exact in 32 bits and each result is rounded once (to fp32), then q_rot and k_rot
-// once more to bf16; k is quantised from the fp32 result. Scale and minimum are bf16
-// (half an ulp of either is below a tenth of a code step), and the codes
-// are taken against the rounded pair, so a value is off by at most half a
-// step plus what the clamp at code 15 costs. Division is IEEE: a quotient half
-// way between two codes goes to the even one.
+// once more to bf16; k is quantised from the fp32 result. Scale and minimum are rounded to bf16
+// and the codes taken against the rounded pair: a value is off by at most half a step or, where
+// the rounded ends leave it below code 0 or above code 15, by at most 2^-8 of the group's
+// minimum and 2^-8 of its range. (A group of numbers far from zero pays for its bf16 minimum: between
+// 100.3 and 100.4 that is 100.5, and every code is 0.) Division is IEEE: a
+// quotient half way between two codes goes to the even one.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -90,9 +91,12 @@ __device__ __forceinline__ float pair_min(uint32_t p) { return __uint_as_float(p
 
 // The codes of 8 numbers: (x - m) / s rounded as IEEE division rounds it, then to
 // the nearest integer, ties to even, within 0 .. 15. In the range where nothing under- or
-// overflows the quotient comes from the correctly rounded reciprocal r of s by Markstein's
-// theorem (q = a r, then q + r (a - q s) is the correctly rounded a / s); elsewhere from a
-// division. NaN (a group without a finite scale) ends as code 0.
+// overflows the quotient comes from the rounded reciprocal r of s by Markstein's correction:
+// q = a r, then q + r (a - q s). Here it gives the IEEE quotient, although q may be two ulp off,
+// because s has 8 significant bits: a - q s is exact (10 bits), what the correction lacks is 2^-23
+// ulp, and a / s lies at least 2^-9 ulp from the middle between two fp32 numbers (a middle
+// times s, of 25 and up to 8 bits, is never a, and a multiple of the same unit). Elsewhere
+// from a division. NaN (a group without a finite scale) ends as code 0.
 __device__ __forceinline__ uint32_t codes8(const float (&x)[8], uint32_t pair) {
   const float s = pair_scale(pair), m = pair_min(pair);
   float q[8];

@@ -320,3 +320,33 @@ def test_single_rows_on_both_sides_of_each_plan(native, cuda, d, hq, hkv, ctx, b
     ([5, 4, 3, 2, 1] * 6, [70 * i for i in range(30)], 32, 8, 2176, True)])
 def test_several_rows_on_both_sides_of_each_plan(native, cuda, d, rows, ctx, hq, hkv, bound, whole):
     _check_plan(cuda, rows, ctx, hq, hkv, d, bound, whole, seed=sum(ctx) + sum(rows))
+
+
+@pytest.mark.parametrize("d,hkv", [(64, 3), (128, 2)])
+def test_codes_are_those_of_ieee_quotients(native, cuda, d, hkv):
+    """Codes of groups of all scales and offsets, bit for bit: fp32 difference, fp32 quotient, nearest even, within 0 .. 15.
+    (Angles of 0: k is quantised as it stands.)"""
+    from swarmlora_b200 import worker_ops as wo
+    g = torch.Generator().manual_seed(d)
+    T = 4096
+    x = torch.randn(T, 2 * hkv, d // 64, 64, generator=g)
+    up = torch.exp2(torch.randint(-120, 100, (T, 2 * hkv, d // 64, 1), generator=g).float())
+    offset = torch.randn(T, 2 * hkv, d // 64, 1, generator=g) * torch.exp2(torch.randint(-8, 8, up.shape, generator=g).float())
+    x[::3] = x[::3].mul(8).round().div(8)     # many quotients on or next to the middle between two codes
+    x[1::3] = torch.randint(0, 31, x[1::3].shape, generator=g).float() / 2
+    rows = ((x + offset) * up).to(BF).reshape(T, -1)
+    page = 1024
+    tables = torch.randperm(4, generator=g).to(torch.int32)[None].to(cuda)
+    cache = wo.kv4_cache(4, hkv, d, page, device=cuda)
+    qkv = torch.cat([torch.zeros(T, d, dtype=BF), rows], 1).to(cuda)
+    cs = torch.cat([torch.ones(T, d // 2), torch.zeros(T, d // 2)], 1).to(BF).to(cuda)
+    q_rot = torch.empty(T, d, dtype=BF, device=cuda)
+    wo.kv4_append(qkv, tables, cache, torch.zeros(1, dtype=torch.int32, device=cuda), q_rot, cs, 1, hkv, head_dim=d, page=page,
+                  rows=[T])
+    got = ref.read_cache(cache.cpu(), tables[0].cpu(), torch.arange(T), d)
+    for (code, _), y in zip(got, rows.float().reshape(T, 2, hkv, d).unbind(1)):
+        y = y.unflatten(-1, (-1, 64))
+        _, s, m = ref.quantise(y.flatten(-2))
+        quot = torch.where(s.float() > 0, (y - m.float()) / s.float(), torch.zeros(()))
+        want = quot.round().clamp(0, 15).long().flatten(-2)
+        assert torch.equal(code, want), int((code != want).sum())
