@@ -350,3 +350,73 @@ def test_codes_are_those_of_ieee_quotients(native, cuda, d, hkv):
         quot = torch.where(s.float() > 0, (y - m.float()) / s.float(), torch.zeros(()))
         want = quot.round().clamp(0, 15).long().flatten(-2)
         assert torch.equal(code, want), int((code != want).sum())
+
+
+@pytest.mark.parametrize("rows,hq,hkv,d", [([1, 1], 8, 2, 128), ([3, 1], 8, 2, 64), ([4, 20], 16, 2, 128)])
+@pytest.mark.parametrize("bound", [290, 3000, 5300])
+def test_contexts_beyond_the_bound_are_cut_there(native, cuda, rows, hq, hkv, d, bound):
+    """A row at or behind max_len sees the first max_len tokens."""
+    from swarmlora_b200 import worker_ops as wo
+    g = _gen(cuda, bound)
+    ctx, n = [bound + 130, bound - 2], -(-(bound + 200) // 16)
+    tables = torch.randperm(2 * n, generator=g, device=cuda).to(torch.int32).reshape(2, n)
+    cache = wo.kv4_cache(2 * n, hkv, d, device=cuda)
+    for t in tables:
+        ref.write_cache(cache, t, torch.arange(16 * n, device=cuda),
+                        *(_randn(g, 16 * n, hkv, d, dtype=torch.float32) for _ in range(2)))
+    q, out = _randn(g, sum(rows), hq * d), torch.empty(sum(rows), hq * d, dtype=BF, device=cuda)
+    wo.paged_attention_kv4(rows, tables, cache, torch.tensor(ctx, dtype=torch.int32, device=cuda), out, q, hq, hkv, bound,
+                           d ** -0.5, head_dim=d)
+    at = 0
+    for i, r in enumerate(rows):
+        for j in range(r):
+            _near_cached(out[at].view(1, hq, d), q[at].view(1, hq, d), cache, tables[i], min(ctx[i] + j + 1, bound),
+                         d ** -0.5, f"row {j} of slot {i}")
+            at += 1
+
+
+@pytest.mark.parametrize("bound", [64, 9000])
+def test_slots_of_negative_length(native, cuda, bound):
+    """Positions below 0 are not cached and see nothing; rows that reach position 0 count from there."""
+    from swarmlora_b200 import worker_ops as wo
+    g = _gen(cuda, 16)
+    hq, hkv, d, rows, ctx = 4, 2, 128, [2, 4, 1], [-100, -2, -(2 ** 31)]
+    tables = torch.tensor([[0], [1], [2]], dtype=torch.int32, device=cuda)
+    cache = torch.full((3, 1, hkv, 18 * d), 0x11, dtype=torch.uint8, device=cuda)
+    before = cache.clone()
+    lens, qkv = torch.tensor(ctx, dtype=torch.int32, device=cuda), _randn(g, 7, (hq + 2 * hkv) * d)
+    q, out = (torch.full((7, hq * d), 9.0, dtype=BF, device=cuda) for _ in range(2))
+    wo.kv4_append(qkv, tables, cache, lens, q, _cos_sin(64, d, cuda), hq, hkv, rows=rows)
+    hidden = [0, 1, 2, 3, 6]
+    assert bool((q[hidden] == 0).all()) and bool((q[[4, 5]] != 0).any())
+    assert torch.equal(cache[[0, 2]], before[[0, 2]]) and not torch.equal(cache[1], before[1])
+    wo.paged_attention_kv4(rows, tables, cache, lens, out, q, hq, hkv, bound, 0.1)
+    assert bool((out[hidden] == 0).all())
+    for r, n in ((4, 1), (5, 2)):
+        _near_cached(out[r].view(1, hq, d), q[r].view(1, hq, d), cache, tables[1], n, 0.1, f"row {r}")
+
+
+@pytest.mark.parametrize("bound,whole", [(1000, True), (2817, False)])
+def test_as_many_slots_as_a_call_takes(native, cuda, bound, whole):
+    """128 slots of one to three rows, some without any."""
+    rows = [(i % 4) for i in range(128)]
+    _check_plan(cuda, rows, [(37 * i) % 400 for i in range(128)], 4, 2, 64, bound, whole, seed=128)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("group", [3, 17, 33, 64, 65, 100, 127, 128])
+def test_prompts_of_many_query_heads_a_kv_head(native, cuda, d, group):
+    """Tiles that no token count fills exactly, down to one token a tile."""
+    from swarmlora_b200 import worker_ops as wo
+    g = _gen(cuda, group + d)
+    hkv = 2
+    q_lens, k_lens = [1, 5, 40, 0, 3], [300, 5, 170, 2, 1]
+    q, k, v = (_randn(g, sum(n), h, d) for n, h in ((q_lens, hkv * group), (k_lens, hkv), (k_lens, hkv)))
+    out = torch.full((sum(q_lens) + 2, hkv * group, d), 9.0, dtype=BF, device=cuda)
+    wo.prompt_attention(torch.cat([q, q[:2]]), k, v, q_lens, k_lens, out=out)
+    assert bool((out[sum(q_lens):] == 9.0).all())
+    for a, b, c, o in zip(q.split(q_lens), k.split(k_lens), v.split(k_lens), out.split([*q_lens, 2])):
+        want, mass = (ref.attend_fast(a, b, x, d ** -0.5) for x in (c, c.abs()))
+        off = (o.double() - want).abs()
+        assert bool((off <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -10) * mass + 1e-30).all())
+    assert wo.attention_device_error() == 0
