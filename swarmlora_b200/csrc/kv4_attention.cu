@@ -374,7 +374,6 @@ __global__ void __launch_bounds__(NW * 32, NT == 1 && NW == kWarps ? 3 : 2)
     uint32_t qb[NT][2 * W][2];
     float qs[NT][NG][2], qo[NT][NG][2];  // sum q, and -128 sum q
     int seen[NT][2], seen_g[NT];  // tokens that columns 2c, 2c + 1 and column g see
-    int all_see = 0x7fffffff;     // tokens that every column sees
     auto sees = [&](int col) {
       const int64_t n = min(len0 + col / p.group + 1, static_cast<int64_t>(p.max_len));
       return col < ncols ? static_cast<int>(max(n, int64_t{0})) : 0;
@@ -411,7 +410,8 @@ __global__ void __launch_bounds__(NW * 32, NT == 1 && NW == kWarps ? 3 : 2)
       seen[nt][1] = sees(col0 + c2 + 1);
       seen_g[nt] = sees(col);
     }
-    all_see = sees(col0);  // the pass's first column belongs to its first row
+    // from this block on some column does not see all of two blocks (the pass's first column belongs to its first row)
+    const int edge_from = sees(col0) / kBlockTok - 1;
     // m: reference (scaled, base 2), nm: 7 - m, bar_: the raw score that moves it, l: sum of the weights times 2^7
     float o[NT][2 * W][4], ps[NT][NG][4], corr[NT][NG], m[NT][2], nm[NT][2], bar_[NT][2], l[NT][2];
 #pragma unroll
@@ -624,7 +624,7 @@ __global__ void __launch_bounds__(NW * 32, NT == 1 && NW == kWarps ? 3 : 2)
       ++used;
       issue();  // into the stage that the previous pair left
       // some column ends here, or a block is missing
-      if (b * kBlockTok > all_see - 2 * kBlockTok || there != 3u) two(blk, b * kBlockTok, there, std::true_type{});
+      if (b >= edge_from || there != 3u) two(blk, b * kBlockTok, there, std::true_type{});
       else two(blk, b * kBlockTok, there, std::false_type{});
       __syncwarp();  // every lane has read the stage before it is filled again
     }
