@@ -447,7 +447,8 @@ int swl_attention_device_error(unsigned int* code);
  * (16-byte aligned); a block holds K and V of 16 tokens of one kv head: codes
  * 0..15 and, per 64 dimensions of a token, a bf16 scale s and minimum m, value =
  * s * code + m (4.5 bits a value, 3.6 times less than bf16). A group
- * with a NaN or an infinity reads back as NaN throughout. head_dim 64 or
+ * with a NaN or an infinity, or whose range is beyond fp32, reads back as NaN throughout. Attention
+ * sums values in fp32 under weights of up to 2^8: up to 2^90 no such sum overflows. head_dim 64 or
  * 128; page 16, 32, 64 .. 1024 tokens. Block tables are device arrays of
  * table_len page ids per slot; entries outside 0..num_pages-1 and positions
  * outside the table are treated as absent: nothing is written for them, a gather gives
@@ -476,7 +477,8 @@ int swl_kv4_gather(int nseg, const int* starts, const int* lens, const void* con
 /* Causal GQA attention over the 4-bit cache: rows[i] new rows of slot i, whose K and V are
  * already appended, at positions *seqlens[i] + t, as swl_paged_attention. hq a multiple
  * of hkv; out rows [rows[i], hq * head_dim] (stride a multiple of 8). max_len
- * bounds *seqlens[i] + rows[i]; longer contexts are cut there. `part`: scratch
+ * bounds *seqlens[i] + rows[i]; longer contexts are cut there. The division of the work is
+ * planned by it: a bound far above the contexts costs a second launch. `part`: scratch
  * of swl_kv4_part_floats fp32 values (0: may be NULL), used by this call alone
  * while it runs. */
 int64_t swl_kv4_part_floats(int nseg, const int* rows, int hq, int hkv, int head_dim, int max_len);

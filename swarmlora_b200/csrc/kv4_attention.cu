@@ -31,7 +31,7 @@
 //
 // What bounds it: integer logic, which runs at half rate. Turning a block's codes into operands
 // is 112 of the 200 or so logic operations it takes, a fifth of the time; without any
-// arithmetic the copies alone take 73 us where the whole takes 102 (16 slots of 16k-32k
+// arithmetic the copies alone take 73 us where the whole takes 103 (16 slots of 16k-32k
 // tokens, 8 kv heads of 128: 435 MB, 4.2 TB/s; 28 slots of 256-768 tokens 12.8 us). Four
 // warps with 168 registers, three CTAs an SM: 113 us before blocks shared their scores, against
 // 119 with 16 warps of 128 registers and 124 with 8 of 255. Measured and left out: fp8 operands for

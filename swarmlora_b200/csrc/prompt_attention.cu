@@ -21,12 +21,12 @@
 // A CTA stays and takes one item after the other, the next of the list whenever it is
 // free: the copies and score products of the next item run while the rows of the last
 // one are written. Against a list dealt out beforehand by length, sixteen prompts of 17 to
-// 2048 tokens went from 248 to 218 us and five of up to 2000 with heads of 64 from 38 to 33 (a row
+// 2048 tokens went from 248 to 218 us in bursts (250 in a loop) and five of up to 2000 with heads of 64 from 38 to 32 (a row
 // tile's 128 keys take 2.1 us, what is fixed in an item 3 to 4, so shares counted in keys are uneven).
 //
-// One prompt of 8191 tokens, 32 query and 8 kv heads of 128: 443 us in a burst at 1965 MHz
+// One prompt of 8191 tokens, 32 query and 8 kv heads of 128: 442 us in a burst at 1965 MHz
 // (1.24 PFLOP/s), 498 to 518 in a loop, where the power cap holds the clock at 1620 (1.06 to
-// 1.10; the figures here are of loops). At full clock what bounds it is the chain of one row
+// 1.10; the comparisons below are of loops). At full clock what bounds it is the chain of one row
 // tile (product, 128 exponentials a thread, product: 2.1 us, of which its products take 0.55),
 // two of which are in flight: tensor memory has no room for a third. Without the two issuing
 // warps' turns it is 607 us, with the turn handed over before the score product 574, half way
@@ -789,8 +789,8 @@ int make_plan(Plan* pl, int nseg, const int* q_lens, const int* k_lens, int hq, 
   if (items * hkv > (int64_t{1} << 30)) return set_error(SWL_ERR_ARG, "prompt_attention: too many query blocks");
   pl->items = static_cast<int>(items);
   // Few blocks with many keys: the keys are split over the idle SMs and joined by a second
-  // launch. Measured: a key tile takes 1.6 us, the second launch 3 us and its partial
-  // results, written and read once, pass at 3 TB/s. One row behind 8000 keys 99.6 -> 20.7 us, behind
+  // launch. Measured: a key tile takes 1.6 us where one row tile is at work alone, as in such blocks
+  // (2.1 with two, heads of 128), the second launch 3 us and its partial results, written and read once, pass at 3 TB/s. One row behind 8000 keys 99.6 -> 20.7 us, behind
   // 1000 16.4 -> 10.2; 8 chunks of 16 rows behind 768 keys would go from 16.4 to 18.0.
   const int64_t ctas = std::max<int64_t>(1, items * hkv);
   const int64_t limit = std::min<int64_t>(sm_count_prompt() / ctas, most);
