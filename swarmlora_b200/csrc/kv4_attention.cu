@@ -490,7 +490,8 @@ __global__ void __launch_bounds__(NW * 32, NT == 1 && NW == kWarps ? 3 : 2)
             f[k] = m[nt][k] == mn ? 1.f : ex2(m[nt][k] - mn);
             m[nt][k] = mn;
             nm[nt][k] = mn == -INFINITY ? 0.f : kHalfUp - mn;  // nothing seen yet: every weight is zero
-            bar_[nt][k] = (mn + kRescaleLog2) * p.inv_scale;
+            const float bar = (mn + kRescaleLog2) * p.inv_scale;
+            bar_[nt][k] = fmaf(-0x1p-21f, fabsf(bar), bar);  // rounded down: no weight passes 2^8, whatever the scores' size
             l[nt][k] *= f[k];
           }
 #pragma unroll

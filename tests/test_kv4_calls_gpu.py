@@ -420,3 +420,30 @@ def test_prompts_of_many_query_heads_a_kv_head(native, cuda, d, group):
         off = (o.double() - want).abs()
         assert bool((off <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -10) * mass + 1e-30).all())
     assert wo.attention_device_error() == 0
+
+
+@pytest.mark.parametrize("hq,rows", [(8, 1), (16, 1), (16, 3)])
+@pytest.mark.parametrize("power", [0, 20, 22, 23, 24, 25])
+def test_weights_of_huge_scores_stay_finite(native, cuda, hq, rows, power):
+    """Scores around -2^power (base 2), each of a warp's block pairs 9.4 above the last: next to 2^8, by which
+    a score may pass its reference before that moves. fp32 holds such scores to steps of up to 4, so
+    only what they cannot change is looked at: values of 1 have 1 as every weighted mean, up to the fp16 rounding of a weight (2^-11) and
+    the output's (2^-8)."""
+    from swarmlora_b200 import worker_ops as wo
+    hkv, d, n = 2, 128, 2800
+    warps = 6 if rows * hq // hkv <= 8 else 4
+    table = torch.arange(n // 16, dtype=torch.int32, device=cuda)
+    cache = wo.kv4_cache(n // 16, hkv, d, device=cuda)
+    step = torch.arange(n, device=cuda) // 32 // warps
+    k = torch.ones(n, hkv, d, device=cuda)
+    k[:, :, 64:] = (6.5 * step.clamp(max=19))[:, None, None]
+    ref.write_cache(cache, table, torch.arange(n, device=cuda), k, torch.ones(n, hkv, d, device=cuda))
+    for i in range(16):
+        q = torch.zeros(rows, hq, d, dtype=BF, device=cuda)
+        spread = 1.0 + (torch.arange(rows * hq, device=cuda).view(rows, hq) + i * rows * hq) % 128 / 128
+        q[..., :64] = (-spread * 2.0 ** power * 0.6931471805599453 / 64).to(BF)[..., None]
+        q[..., 64:] = 1.0 / 64
+        out = torch.empty(rows, hq * d, dtype=BF, device=cuda)
+        wo.paged_attention_kv4([rows], table[None], cache, torch.tensor([n - rows], dtype=torch.int32, device=cuda), out,
+                               q.flatten(1), hq, hkv, n, 1.0)
+        assert bool(((out.float() - 1.0).abs() <= 2.0 ** -8 + 2.0 ** -11).all()), out.float().sub(1).abs().max().item()
