@@ -447,3 +447,25 @@ def test_weights_of_huge_scores_stay_finite(native, cuda, hq, rows, power):
         wo.paged_attention_kv4([rows], table[None], cache, torch.tensor([n - rows], dtype=torch.int32, device=cuda), out,
                                q.flatten(1), hq, hkv, n, 1.0)
         assert bool(((out.float() - 1.0).abs() <= 2.0 ** -8 + 2.0 ** -11).all()), out.float().sub(1).abs().max().item()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows,ctx", [([1], [4000]), ([1, 1, 1], [40, 0, 3100]), ([3, 0, 1, 16], [2900, 7, 0, 333]), ([1] * 60, [5] * 60)])
+def test_what_scratch_holds_beforehand_does_not_matter(native, cuda, d, rows, ctx):
+    from swarmlora_b200 import worker_ops as wo
+    g = _gen(cuda, sum(ctx))
+    hq, hkv, total = 8, 2, [a + b for a, b in zip(rows, ctx)]
+    per = -(-max(total) // 16)
+    tables = torch.arange(len(rows) * per, dtype=torch.int32, device=cuda).reshape(-1, per)
+    cache = wo.kv4_cache(tables.numel(), hkv, d, device=cuda)
+    for t, n in zip(tables, total):
+        ref.write_cache(cache, t, torch.arange(n, device=cuda), *(_randn(g, n, hkv, d, dtype=torch.float32) for _ in range(2)))
+    q, lens = _randn(g, sum(rows), hq * d), torch.tensor(ctx, dtype=torch.int32, device=cuda)
+    need = wo.kv4_part_floats(rows, hq, hkv, 6000, head_dim=d)
+    assert need > 0
+    outs = []
+    for fill in (0.0, float("nan")):
+        part = torch.full((need,), fill, device=cuda)
+        outs.append(torch.full((sum(rows), hq * d), 9.0, dtype=BF, device=cuda))
+        wo.paged_attention_kv4(rows, tables, cache, lens, outs[-1], q, hq, hkv, 6000, d ** -0.5, head_dim=d, part=part)
+    assert bool(torch.isfinite(outs[0]).all()) and torch.equal(*outs)
